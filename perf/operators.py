@@ -197,14 +197,15 @@ def _inputs(case, seed):
 
 
 def _quantise(x, scheme):
-    """Codes and scales of heads x [..., d]: as they stand in the cache."""
+    """Codes and scales of heads x [..., d]: as they stand in the cache.  (Divisions by tensors: one by a number is torch's product with
+    the number's reciprocal.)"""
     x = x.float()
     top = x.abs().amax(-1, keepdim=True)
     one = torch.ones_like(top)
     if scheme == "int8":
-        scale = torch.where(top > 0, top, one) / 127
+        scale = torch.where(top > 0, top, one) / (127 * one)
         return torch.round(x / scale).clamp(-127, 127).to(torch.int8), scale
-    scale = torch.where(top > 0, top, one) / 448
+    scale = torch.where(top > 0, top, one) / (448 * one)
     return (x / scale).clamp(-448, 448).to(torch.float8_e4m3fn).view(torch.int8), scale
 
 
