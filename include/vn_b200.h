@@ -419,6 +419,56 @@ int32_t vn_tree_accept_sample(vn_ctx* ctx, const void* lists_dev, const int64_t*
                               uint64_t seed, uint32_t offset, int32_t* out_len_dev, int64_t* out_tokens_dev,
                               int32_t* keep_target_dev, int32_t* keep_draft_dev);
 
+/* ---- a paged cache of keys and values in 8 bits, and attention over it (no counterpart in the reference, whose caches hold
+ *      fp32: kv_cache_parallel.py:42-283) ------------------------------------------------------------------------------
+ * A head of a position is scale * code: "int8" scale = max|x| / 127, "fp8" (e4m3) max|x| / 448, code = round to nearest even of
+ * x / scale (both in fp32; a head of zeros has the scale of max|x| = 1, no scale is below 2^-126).  A head with a value that is not finite reads as NaN.
+ * Pages of 64 positions: vn_qkv_set_pages names the page of every 64 positions of a sequence (host table
+ * [max_batch][ceil(max_seq / 64)], -1: none); with pages = 0 the pool holds max_batch x max_seq positions and every sequence has
+ * its own pages from the start, else the pool has `pages` pages and no sequence has any.  Sequences may share pages that none of
+ * them writes.  Rows are float32 or bf16 (`dtype`), head_dim a multiple of 8 up to 256.
+ *
+ * A step's rows: ents_dev NULL: sequences 0 .. n_ent-1 bring T rows each, M = n_ent * T.  Else entry e = ents_dev[e] = {sequence,
+ * first row, rows, 0} (int32 x 4, 16-byte aligned, at most T rows each) and row_ent_dev [M] names the entry of every row, -1: a row
+ * of none, which is left as it was.  A sequence must not come twice in one append.
+ * A tree over the rows of an entry (T <= 64): seen_dev bit j of row i: row i sees row j of its entry (itself too, if it is to);
+ * depth_dev: tokens between the row and the committed ones.  Tables of T values, or of M with *_per_row != 0.  NULL: a
+ * chain, row i sees rows 0 .. i.
+ * All calls but create, destroy, set_pages, lengths, status and set_lengths of a host array are asynchronous on the context's stream,
+ * allocate nothing and may be captured.  Device tables are read when the kernels run; what they hold out of range is left
+ * out and reported by vn_qkv_status. */
+typedef struct vn_qkv vn_qkv;
+int32_t vn_qkv_create(vn_ctx* ctx, int32_t max_batch, int32_t max_seq, int32_t n_head, int32_t n_kv_head, int32_t head_dim, const char* scheme,
+                      int32_t dtype, int32_t pages, vn_qkv** out);
+int32_t vn_qkv_destroy(vn_qkv* c);
+int32_t vn_qkv_set_pages(vn_qkv* c, const int32_t* table_host);
+int32_t vn_qkv_lengths(vn_qkv* c, int32_t* out_host);                                  /* [max_batch] */
+int32_t vn_qkv_set_lengths(vn_qkv* c, const int32_t* lens, int32_t on_device);         /* [max_batch] */
+/* Conditions met by kernels since the last call, read after a stream synchronisation and cleared: *no_room: a position behind
+ * the capacity or without a page was to be written or read (VN_ERR_OVERFLOW); *bad_index: a sequence, row, count or kept row
+ * out of range (VN_ERR_INDEX). */
+int32_t vn_qkv_status(vn_qkv* c, int32_t* no_room, int32_t* bad_index);
+/* Writes a step's keys and values at positions length + offset + i; lengths stay.  rows_dev [M][ld]: the H query heads (only with
+ * queries != 0), the KH key heads, the KH value heads.  In the same pass, for query and key heads: x / sqrt(mean x^2 + eps) * norm
+ * (float32 [head_dim], NULL: none), then the rotation of `pairs` pairs (half-split, or neighbours with interleaved != 0) by
+ * cos_dev / sin_dev [rope_rows][pairs] at position length + offset + depth; the queries go to q_out_dev [M, H, head_dim]. */
+int32_t vn_qkv_append(vn_qkv* c, const void* rows_dev, int64_t ld, int32_t queries, int32_t n_ent, const int32_t* ents_dev, const int32_t* row_ent_dev,
+                      int32_t T, int32_t M, int32_t offset, const int32_t* depth_dev, int32_t depth_per_row, const float* q_norm_dev,
+                      const float* k_norm_dev, float eps, const float* cos_dev, const float* sin_dev, int32_t rope_rows, int32_t pairs,
+                      int32_t interleaved, void* q_out_dev);
+/* out = softmax(scale q k^T) v over the committed positions and the rows of the same step (appended at offset 0); query head h
+ * reads key/value head h / (H / KH).  window > 0: row at position p sees position j only if p - j < window (with a tree: the committed
+ * ones only).  A row that sees nothing gets zeros.  q_dev, out_dev [M, H, head_dim], 16-byte (float32) / 8-byte aligned. */
+int32_t vn_qkv_attention(vn_qkv* c, const void* q_dev, int32_t n_ent, const int32_t* ents_dev, const int32_t* row_ent_dev, int32_t T, int32_t M,
+                         const uint64_t* seen_dev, const int32_t* depth_dev, int32_t tree_per_row, int32_t window, float scale, void* out_dev);
+/* Values of a step's positions, [M, KH, head_dim] each, dtype VN_F32 or VN_BF16.  Row i of an entry reads position start + i;
+ * start = -1: length + offset + i; -2: length - rows + i (the last ones). */
+int32_t vn_qkv_read(vn_qkv* c, int32_t n_ent, const int32_t* ents_dev, const int32_t* row_ent_dev, int32_t T, int32_t M, int32_t start, int32_t offset,
+                    int32_t dtype, void* k_out_dev, void* v_out_dev);
+/* As vn_kv_commit: sequence b keeps n_keep[b] + keep_add of the n_new positions behind its length, the first ones, or those
+ * that keep_idx_dev[b * stride + j] names (n_new <= 64; any order), moved to length + j; then its length grows by that many. */
+int32_t vn_qkv_commit(vn_qkv* c, int32_t n_new, const int32_t* keep_idx_dev, int32_t stride, const int32_t* n_keep_dev, int32_t keep_add);
+
 /* Device-side round counter: while set, every Philox offset passed to vn_accept* / vn_sample is
  * incremented by *counter_dev, and vn_spec_advance adds one to it at the end of a round. */
 int32_t vn_set_offset_source(vn_ctx* ctx, const uint32_t* counter_dev);

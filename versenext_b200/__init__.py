@@ -15,6 +15,7 @@ Public surface (names follow the reference):
   get_backend / clear_backend_cache,
   DeviceBackend, B200Backend              verse_torch/device.py:219-389
   Context, DeviceArray                    device memory (plays torch.Tensor's role, tensor.py:394)
+  QuantKVCache                            keys and values in 8 bits with the attention that reads them
   sampling.accept / sample / argmax       acceptance and sampling kernels
 
 Everything computes in libvn_b200.so; importing this package does not need a
@@ -25,6 +26,7 @@ from . import _lib
 from .device import Context, DeviceArray, as_device
 from .backend import DeviceBackend, B200Backend, get_backend, clear_backend_cache
 from .speculative import SpeculativeDecoder, Tensor, no_grad
+from .quant_cache import QuantKVCache
 from .model import VerseNexLM, CometSparkNexLM, KVCache, build_verse_delta_pattern
 from .engine import SpecEngine
 from .composed import ComposedLM
@@ -42,6 +44,6 @@ from . import sampling
 from . import quant
 
 __all__ = ["Context", "DeviceArray", "as_device", "DeviceBackend", "B200Backend", "get_backend",
-           "clear_backend_cache", "SpeculativeDecoder", "Tensor", "no_grad", "sampling", "quant", "VerseNexLM", "CometSparkNexLM", "KVCache", "ComposedLM", "BozasunLM", "FuzudraLM", "GivozenLM", "MusutarLM",
+           "clear_backend_cache", "SpeculativeDecoder", "Tensor", "no_grad", "sampling", "quant", "VerseNexLM", "CometSparkNexLM", "KVCache", "QuantKVCache", "ComposedLM", "BozasunLM", "FuzudraLM", "GivozenLM", "MusutarLM",
            "load_model", "BatchEngine", "StepRunner", "build_verse_delta_pattern", "SpecEngine", "TreeSpecEngine",
            "ShardedSpecEngine", "Comm", "rank_seed", "VNFileReader", "load_vn"]

@@ -128,6 +128,16 @@ PROTOTYPES = {
     "vn_kv_set_lengths": [_p, _p],
     "vn_kv_commit": [_p, _i32, _p, _i32, _p, _i32],
     "vn_kv_read": [_p, _i32, _i32, _i32, _p, _i32],
+    "vn_qkv_create": [_p, _i32, _i32, _i32, _i32, _i32, C.c_char_p, _i32, _i32, C.POINTER(_p)],
+    "vn_qkv_destroy": [_p],
+    "vn_qkv_set_pages": [_p, _p],
+    "vn_qkv_lengths": [_p, _p],
+    "vn_qkv_set_lengths": [_p, _p, _i32],
+    "vn_qkv_status": [_p, C.POINTER(_i32), C.POINTER(_i32)],
+    "vn_qkv_append": [_p, _p, _i64, _i32, _i32, _p, _p, _i32, _i32, _i32, _p, _i32, _p, _p, _f32, _p, _p, _i32, _i32, _i32, _p],
+    "vn_qkv_attention": [_p, _p, _i32, _p, _p, _i32, _i32, _p, _p, _i32, _i32, _f32, _p],
+    "vn_qkv_read": [_p, _i32, _p, _p, _i32, _i32, _i32, _i32, _i32, _p, _p],
+    "vn_qkv_commit": [_p, _i32, _p, _i32, _p, _i32],
     "vn_model_forward_ragged": [_p, _p, _p, _i32, _p, _p, _i32, _p, _p, _p],
     "vn_model_set_probe": [_p, _p],
     "vn_model_forward": [_p, _p, _p, _i32, _i32, _p, _p, _p, _i32, _i32],

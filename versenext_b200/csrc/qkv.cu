@@ -1,0 +1,404 @@
+// The paged 8-bit cache's entry points and the kernels that write, read and keep positions; attention is in qkv_attn.cu.
+#include <string.h>
+
+#include <new>
+
+#include "qkv.cuh"
+
+namespace {
+
+using bf16 = __nv_bfloat16;
+
+struct AppendArgs {
+  QkvView v;
+  QkvStep step;
+  QkvTree tree;
+  const void* x = nullptr;             // rows [H queries |] KH keys | KH values
+  void* q = nullptr;                   // [M, H, d]
+  long long ld = 0;
+  int off = 0, H = 0;                  // H = 0: the rows hold no queries
+  const float *qn = nullptr, *kn = nullptr, *cs = nullptr, *sn = nullptr;
+  float eps = 0.f;
+  int pairs = 0, interleaved = 0, rope_rows = 0, vec = 0;
+};
+
+template <typename T> __device__ __forceinline__ float4 quad_of(const T* p, bool vec) {
+  if (vec) return load4(p);
+  return make_float4(to_f<T>(p[0]), to_f<T>(p[1]), to_f<T>(p[2]), to_f<T>(p[3]));
+}
+template <typename T> __device__ __forceinline__ void put_quad(T* p, float4 v, bool vec) {
+  if (vec) { store4(p, v); return; }
+  p[0] = from_f<T>(v.x); p[1] = from_f<T>(v.y); p[2] = from_f<T>(v.z); p[3] = from_f<T>(v.w);
+}
+
+__device__ __forceinline__ unsigned char code_of(float y, int scheme) {
+  if (scheme == QKV_I8) return (unsigned char)(signed char)max(-127, min(127, __float2int_rn(y)));
+  unsigned short r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(0.f), "f"(y));
+  return (unsigned char)r;
+}
+
+// One warp per (row, head); a lane takes quads lane, lane + 32 of the head, which is staged in shared memory for the rotation.
+// grid ceil(M units / 8), block (32, 8)
+template <typename T>
+__global__ void __launch_bounds__(256) qkv_append_kernel(AppendArgs a) {
+  __shared__ __align__(16) float s_head[8][256];
+  const int units = a.H + 2 * a.v.KH, lane = threadIdx.x;
+  const long long task = (long long)blockIdx.x * 8 + threadIdx.y;
+  const int unit = (int)(task % units);
+  if (task / units >= a.step.M) return;
+  const int row = (int)(task / units);
+  int slot, i, n;
+  if (!a.step.row(a.v, row, &slot, &i, &n)) return;
+  const bool is_q = unit < a.H, is_v = unit >= a.H + a.v.KH;
+  const int len = a.v.len(slot), pos = len + a.off + i, d = a.v.d;
+  const int turn = len + a.off + a.tree.away(row, i);
+  float* s = s_head[threadIdx.y];
+  const T* x = reinterpret_cast<const T*>(a.x) + row * a.ld + (long long)unit * d;
+  const float* w = is_v ? nullptr : is_q ? a.qn : a.kn;
+  float ss = 0.f;
+  for (int c = 4 * lane; c < d; c += 128) {
+    const float4 v = quad_of(x + c, a.vec);
+    *reinterpret_cast<float4*>(s + c) = v;
+    ss += v.x * v.x + v.y * v.y + v.z * v.z + v.w * v.w;
+  }
+  const float r = w ? sqrtf(warp_sum(ss) / (float)d + a.eps) : 1.f;
+  __syncwarp();
+  if (w) {
+    for (int c = lane; c < d; c += 32) s[c] = s[c] / r * w[c];
+    __syncwarp();
+  }
+  if (!is_v && a.pairs) {
+    const long long at = (long long)min(max(turn, 0), a.rope_rows - 1) * a.pairs;
+    for (int p = lane; p < a.pairs; p += 32) {
+      const int cu = a.interleaved ? 2 * p : p, cv = a.interleaved ? 2 * p + 1 : p + a.pairs;
+      const float u = s[cu], v = s[cv], cs = a.cs[at + p], sn = a.sn[at + p];
+      s[cu] = u * cs - v * sn;
+      s[cv] = v * cs + u * sn;
+    }
+    __syncwarp();
+  }
+  if (is_q) {
+    T* o = reinterpret_cast<T*>(a.q) + ((long long)row * a.H + unit) * d;
+    for (int c = 4 * lane; c < d; c += 128) put_quad(o + c, *reinterpret_cast<const float4*>(s + c), a.vec);
+    return;
+  }
+  const int head = unit - a.H - (is_v ? a.v.KH : 0);
+  const int page = pos >= 0 && pos < a.v.capacity() ? a.v.page(slot, pos / KV_PAGE) : -1;
+  if (page < 0) { if (lane == 0) a.v.status[0] = 1; return; }
+  float top = 0.f;
+  bool bad = false;
+  for (int c = lane; c < d; c += 32) { top = fmaxf(top, fabsf(s[c])); bad |= !isfinite(s[c]); }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  bad = __any_sync(0xffffffffu, bad);
+  const float scale = fmaxf((top > 0.f ? top : 1.f) / (a.v.scheme == QKV_I8 ? 127.f : 448.f), QKV_SCALE_MIN);
+  unsigned char* b = a.v.block(page, head, pos % KV_PAGE / QKV_BLOCK);
+  const int at = pos % QKV_BLOCK, P = a.v.P, t = qkv_turn(P / 16, at);
+  unsigned char* codes = b + (is_v ? QKV_BLOCK * P : 0) + at * P;
+  for (int c = 4 * lane; c < P; c += 128) {
+    uchar4 k = make_uchar4(0, 0, 0, 0);
+    if (c < d && !bad) {
+      const float4 v = *reinterpret_cast<const float4*>(s + c);
+      k = make_uchar4(code_of(v.x / scale, a.v.scheme), code_of(v.y / scale, a.v.scheme), code_of(v.z / scale, a.v.scheme), code_of(v.w / scale, a.v.scheme));
+    }
+    *reinterpret_cast<uchar4*>(codes + (((c >> 4) ^ t) << 4) + (c & 15)) = k;
+  }
+  if (lane == 0) reinterpret_cast<float*>(b + 2 * QKV_BLOCK * P)[(is_v ? QKV_BLOCK : 0) + at] = bad ? CUDART_NAN_F : scale;
+}
+
+// One thread per 8 channels of a head at a position.  grid (ceil(M KH d / 8 / 256), 2)
+template <typename O, int SCHEME>
+__global__ void __launch_bounds__(256) qkv_read_kernel(QkvView v, QkvStep step, int start, int off, O* __restrict__ k, O* __restrict__ vals, int vec) {
+  const long long t = (long long)blockIdx.x * 256 + threadIdx.x;
+  const int per = v.d / 8, c = (int)(t % per) * 8;
+  const long long rh = t / per;
+  const int head = (int)(rh % v.KH);
+  const long long row = rh / v.KH;
+  if (row >= step.M) return;
+  int slot, i, n;
+  if (!step.row(v, (int)row, &slot, &i, &n)) return;
+  const int pos = (start >= 0 ? start : v.len(slot) + off - (start == -2 ? n : 0)) + i;
+  const int page = pos >= 0 && pos < v.capacity() ? v.page(slot, pos / KV_PAGE) : -1;
+  float x[8];
+  if (page < 0) {
+    v.status[0] = 1;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = 0.f;
+  } else {
+    const unsigned char* b = v.block(page, head, pos % KV_PAGE / QKV_BLOCK);
+    const int at = pos % QKV_BLOCK;
+    const float scale = reinterpret_cast<const float*>(b + 2 * QKV_BLOCK * v.P)[blockIdx.y * QKV_BLOCK + at];
+    const uint2 u = *reinterpret_cast<const uint2*>(b + blockIdx.y * QKV_BLOCK * v.P + at * v.P + (((c >> 4) ^ qkv_turn(v.P / 16, at)) << 4) + (c & 15));
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = qkv_value<SCHEME>((unsigned char)((e < 4 ? u.x : u.y) >> (8 * (e & 3)))) * scale;
+  }
+  O* o = (blockIdx.y ? vals : k) + rh * v.d + c;
+  put_quad(o, make_float4(x[0], x[1], x[2], x[3]), vec);
+  put_quad(o + 4, make_float4(x[4], x[5], x[6], x[7]), vec);
+}
+
+// A block per (sequence, head): the kept positions are read whole before any is written, so that they may overlap in any
+// order; the block that finishes a sequence last moves its length.  grid (KH, sequences)
+__global__ void __launch_bounds__(256) qkv_commit_kernel(QkvView v, int n_new, const int* __restrict__ keep, int stride, const int* __restrict__ n_keep,
+                                                         int keep_add, int* __restrict__ tickets) {
+  __shared__ __align__(16) unsigned char s_codes[QKV_MAX_DRAFT][2][256];
+  __shared__ float s_scale[QKV_MAX_DRAFT][2];
+  const int head = blockIdx.x, slot = blockIdx.y, tid = threadIdx.x, P = v.P, CH = P / 16;
+  const int len = v.len(slot);
+  int n = n_keep[slot] + keep_add;
+  if (n < 0 || n > n_new || len + n > v.capacity()) {
+    if (tid == 0) v.status[1] = 1;
+    n = min(max(n, 0), min(n_new, v.capacity() - len));
+  }
+  auto move = [&](bool in) {
+    for (int j = tid / 32; j < n; j += 8) {
+      const int from = keep[(long long)slot * stride + j];
+      if (from == j) continue;
+      if (from < 0 || from >= n_new) { if (tid % 32 == 0) v.status[1] = 1; continue; }
+      const int src = len + from, dst = len + j, pos = in ? src : dst;
+      const int page_src = src < v.capacity() ? v.page(slot, src / KV_PAGE) : -1, page_dst = v.page(slot, dst / KV_PAGE);
+      if (page_src < 0 || page_dst < 0) { if (tid % 32 == 0) v.status[0] = 1; continue; }
+      const int page = in ? page_src : page_dst;
+      unsigned char* b = v.block(page, head, pos % KV_PAGE / QKV_BLOCK);
+      const int at = pos % QKV_BLOCK, t = qkv_turn(CH, at);
+      for (int x = tid % 32; x < 2 * CH; x += 32) {
+        const int which = x / CH, c = x % CH;
+        uint4* g = reinterpret_cast<uint4*>(b + (which * QKV_BLOCK + at) * P + ((c ^ t) << 4));
+        uint4* sh = reinterpret_cast<uint4*>(&s_codes[j][which][c << 4]);
+        if (in) *sh = *g; else *g = *sh;
+      }
+      if (tid % 32 < 2) {
+        float* g = reinterpret_cast<float*>(b + 2 * QKV_BLOCK * P) + (tid % 32) * QKV_BLOCK + at;
+        if (in) s_scale[j][tid % 32] = *g; else *g = s_scale[j][tid % 32];
+      }
+    }
+  };
+  if (keep) {
+    move(true);
+    __syncthreads();
+    move(false);
+  }
+  __syncthreads();
+  if (tid == 0) {
+    __threadfence();
+    if (atomicAdd(&tickets[slot], 1) == (int)gridDim.x - 1) {
+      tickets[slot] = 0;
+      v.lens[slot] = len + n;
+    }
+  }
+}
+
+__global__ void set_lengths_kernel(int* __restrict__ lens, const int* __restrict__ from, int n) {
+  const int i = blockIdx.x * 256 + threadIdx.x;
+  if (i < n) lens[i] = from[i];
+}
+
+bool aligned(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
+
+int32_t step_of(vn_qkv* c, int32_t n_ent, const int32_t* ents, const int32_t* row_ent, int32_t T, int32_t M, QkvStep* s) {
+  VN_REQUIRE(c->ctx, n_ent >= 0 && T >= 0 && M >= 0, "negative sizes of a step");
+  VN_REQUIRE(c->ctx, (ents == nullptr) == (row_ent == nullptr), "a ragged step has both tables");
+  VN_REQUIRE(c->ctx, aligned(ents, 16), "the table of entries is not aligned to 16 bytes");
+  VN_REQUIRE(c->ctx, ents || n_ent <= c->v.max_batch, "%d sequences in a cache of %d", n_ent, c->v.max_batch);
+  VN_REQUIRE(c->ctx, ents || M == (long long)n_ent * T, "%d rows are not %d entries of %d", M, n_ent, T);
+  s->ents = (const int4*)ents; s->row_ent = row_ent;
+  s->n_ent = n_ent; s->T = T; s->M = M;
+  return VN_OK;
+}
+
+#define VN_CHECK_QKV(c)                                                   \
+  do {                                                                    \
+    if (!(c)) return vn_fail(nullptr, VN_ERR_INVALID, "null cache");      \
+    VN_CHECK_CTX((c)->ctx);                                               \
+  } while (0)
+
+}  // namespace
+
+extern "C" {
+
+int32_t vn_qkv_create(vn_ctx* ctx, int32_t max_batch, int32_t max_seq, int32_t n_head, int32_t n_kv_head, int32_t head_dim, const char* scheme, int32_t dtype,
+                      int32_t pages, vn_qkv** out) {
+  VN_CHECK_CTX(ctx);
+  VN_REQUIRE(ctx, out && scheme, "null argument");
+  *out = nullptr;
+  const int kind = !strcmp(scheme, "int8") ? QKV_I8 : !strcmp(scheme, "fp8") ? QKV_E4M3 : -1;
+  VN_REQUIRE(ctx, kind >= 0, "unknown scheme '%s' (int8, fp8)", scheme);
+  VN_REQUIRE(ctx, dtype == VN_F32 || dtype == VN_BF16, "rows are float32 or bf16");
+  VN_REQUIRE(ctx, max_batch > 0 && max_batch <= 65535, "max_batch %d outside 1 .. 65535", max_batch);
+  VN_REQUIRE(ctx, max_seq > 0 && max_seq <= (1 << 30), "max_seq %d outside 1 .. 2^30", max_seq);
+  VN_REQUIRE(ctx, n_kv_head > 0 && n_head > 0 && n_head % n_kv_head == 0 && n_head <= 65535, "%d query heads over %d key/value heads", n_head, n_kv_head);
+  VN_REQUIRE(ctx, head_dim >= 8 && head_dim <= 256 && head_dim % 8 == 0, "head_dim %d: a multiple of 8 up to 256 is needed", head_dim);
+  const long long max_pages = ceil_div((long long)max_seq, (long long)KV_PAGE), all = max_pages * max_batch;
+  VN_REQUIRE(ctx, pages >= 0 && (pages || all <= (1ll << 30)), "%d pages", pages);
+  vn_qkv* c = new (std::nothrow) vn_qkv();
+  if (!c) return vn_fail(ctx, VN_ERR_OOM, "out of host memory");
+  c->ctx = ctx; c->dtype = dtype;
+  QkvView& v = c->v;
+  v.max_batch = max_batch; v.max_pages = (int)max_pages; v.n_pages = pages ? pages : (int)all;
+  v.H = n_head; v.KH = n_kv_head; v.d = head_dim; v.scheme = kind;
+  for (int p : {32, 64, 80, 96, 128, 192, 256})
+    if (!v.P && head_dim <= p) v.P = p;
+  const size_t pool = (size_t)v.n_pages * v.KH * 2 * v.block_bytes();
+  int32_t st = VN_OK;
+  auto get = [&](void** p, size_t bytes) {
+    cudaError_t e = cudaMalloc(p, bytes);
+    if (e == cudaSuccess) e = cudaMemsetAsync(*p, 0, bytes, ctx->stream);
+    if (e != cudaSuccess) {
+      cudaGetLastError();
+      st = vn_fail(ctx, e == cudaErrorMemoryAllocation ? VN_ERR_OOM : VN_ERR_CUDA, "cache of %zu bytes: %s", bytes, cudaGetErrorString(e));
+    }
+    return e == cudaSuccess;
+  };
+  if (get((void**)&v.pool, pool) && get((void**)&c->table, (size_t)all * sizeof(int)) && get((void**)&v.lens, (size_t)max_batch * sizeof(int)) &&
+      get((void**)&v.status, 2 * sizeof(int)) && get((void**)&c->tickets, (size_t)max_batch * sizeof(int))) {
+    v.table = c->table;
+    std::vector<int> t;
+    try { t.resize((size_t)all); } catch (...) { vn_qkv_destroy(c); return vn_fail(ctx, VN_ERR_OOM, "out of host memory"); }
+    for (long long i = 0; i < all; ++i) t[i] = pages ? -1 : (int)i;
+    cudaError_t e = cudaMemcpyAsync(c->table, t.data(), (size_t)all * sizeof(int), cudaMemcpyHostToDevice, ctx->stream);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->stream);
+    if (e != cudaSuccess) st = vn_fail(ctx, VN_ERR_CUDA, "cache set-up: %s", cudaGetErrorString(e));
+  }
+  if (st != VN_OK) { vn_qkv_destroy(c); return st; }
+  *out = c;
+  return VN_OK;
+}
+
+int32_t vn_qkv_destroy(vn_qkv* c) {
+  if (!c) return VN_OK;
+  cudaSetDevice(c->ctx->device);
+  cudaStreamSynchronize(c->ctx->stream);
+  for (void* p : {(void*)c->v.pool, (void*)c->table, (void*)c->v.lens, (void*)c->v.status, c->parts, (void*)c->tickets})
+    if (p) cudaFree(p);
+  delete c;
+  return VN_OK;
+}
+
+int32_t vn_qkv_set_pages(vn_qkv* c, const int32_t* table) {
+  VN_CHECK_QKV(c);
+  VN_REQUIRE(c->ctx, table, "table is null");
+  const size_t n = (size_t)c->v.max_batch * c->v.max_pages;
+  for (size_t i = 0; i < n; ++i)
+    if (table[i] < -1 || table[i] >= c->v.n_pages) return vn_fail(c->ctx, VN_ERR_INDEX, "page %d outside the pool of %d", table[i], c->v.n_pages);
+  VN_CUDA(c->ctx, cudaMemcpyAsync(c->table, table, n * sizeof(int), cudaMemcpyHostToDevice, c->ctx->stream));
+  VN_CUDA(c->ctx, cudaStreamSynchronize(c->ctx->stream));
+  return VN_OK;
+}
+
+int32_t vn_qkv_lengths(vn_qkv* c, int32_t* out) {
+  VN_CHECK_QKV(c);
+  VN_REQUIRE(c->ctx, out, "out is null");
+  VN_CUDA(c->ctx, cudaMemcpyAsync(out, c->v.lens, (size_t)c->v.max_batch * sizeof(int), cudaMemcpyDeviceToHost, c->ctx->stream));
+  VN_CUDA(c->ctx, cudaStreamSynchronize(c->ctx->stream));
+  return VN_OK;
+}
+
+int32_t vn_qkv_set_lengths(vn_qkv* c, const int32_t* lens, int32_t on_device) {
+  VN_CHECK_QKV(c);
+  VN_REQUIRE(c->ctx, lens, "lens is null");
+  if (on_device) {
+    VN_LAUNCH(c->ctx, set_lengths_kernel, ceil_div(c->v.max_batch, 256), 256, 0, c->v.lens, lens, c->v.max_batch);
+    return VN_OK;
+  }
+  for (int i = 0; i < c->v.max_batch; ++i)
+    if (lens[i] < 0 || lens[i] > c->v.capacity()) return vn_fail(c->ctx, VN_ERR_OVERFLOW, "length %d of sequence %d outside 0 .. %d", lens[i], i, c->v.capacity());
+  VN_CUDA(c->ctx, cudaMemcpyAsync(c->v.lens, lens, (size_t)c->v.max_batch * sizeof(int), cudaMemcpyHostToDevice, c->ctx->stream));
+  VN_CUDA(c->ctx, cudaStreamSynchronize(c->ctx->stream));
+  return VN_OK;
+}
+
+int32_t vn_qkv_status(vn_qkv* c, int32_t* no_room, int32_t* bad_index) {
+  VN_CHECK_QKV(c);
+  int s[2];
+  VN_CUDA(c->ctx, cudaMemcpyAsync(s, c->v.status, sizeof s, cudaMemcpyDeviceToHost, c->ctx->stream));
+  VN_CUDA(c->ctx, cudaMemsetAsync(c->v.status, 0, sizeof s, c->ctx->stream));
+  VN_CUDA(c->ctx, cudaStreamSynchronize(c->ctx->stream));
+  if (no_room) *no_room = s[0];
+  if (bad_index) *bad_index = s[1];
+  if (s[0]) return vn_fail(c->ctx, VN_ERR_OVERFLOW, "a position behind the cache's end, or without a page, was written or read");
+  if (s[1]) return vn_fail(c->ctx, VN_ERR_INDEX, "a sequence, row or count outside its range was met");
+  return VN_OK;
+}
+
+int32_t vn_qkv_append(vn_qkv* c, const void* rows, int64_t ld, int32_t queries, int32_t n_ent, const int32_t* ents, const int32_t* row_ent, int32_t T, int32_t M,
+                      int32_t offset, const int32_t* depth, int32_t depth_per_row, const float* q_norm, const float* k_norm, float eps, const float* cos_,
+                      const float* sin_, int32_t rope_rows, int32_t pairs, int32_t interleaved, void* q_out) {
+  VN_CHECK_QKV(c);
+  AppendArgs a;
+  a.v = c->v;
+  if (int32_t st = step_of(c, n_ent, ents, row_ent, T, M, &a.step)) return st;
+  a.H = queries ? c->v.H : 0;
+  const int width = (a.H + 2 * c->v.KH) * c->v.d, es = c->dtype == VN_F32 ? 4 : 2;
+  VN_REQUIRE(c->ctx, M == 0 || (rows && (q_out || !queries)), "null rows");
+  VN_REQUIRE(c->ctx, ld >= width, "rows of %lld values, %d are needed", (long long)ld, width);
+  VN_REQUIRE(c->ctx, aligned(rows, es) && aligned(q_out, es), "rows are not aligned to their values");
+  VN_REQUIRE(c->ctx, offset >= 0, "offset %d", offset);
+  VN_REQUIRE(c->ctx, pairs >= 0 && 2 * pairs <= c->v.d, "%d rotated pairs in heads of %d", pairs, c->v.d);
+  VN_REQUIRE(c->ctx, !pairs || (cos_ && sin_ && rope_rows >= c->v.capacity()), "rotation: tables of %d positions for a cache of %d", rope_rows, c->v.capacity());
+  VN_REQUIRE(c->ctx, !depth || T <= QKV_MAX_DRAFT, "a tree of %d rows, at most %d", T, QKV_MAX_DRAFT);
+  if (M == 0 || T == 0) return VN_OK;
+  a.tree.depth = depth; a.tree.per_row = depth_per_row;
+  a.x = rows; a.q = q_out; a.ld = ld; a.off = offset;
+  a.qn = q_norm; a.kn = k_norm; a.eps = eps;
+  a.cs = cos_; a.sn = sin_; a.pairs = pairs; a.interleaved = interleaved; a.rope_rows = rope_rows;
+  a.vec = aligned(rows, 4 * es) && aligned(q_out, 4 * es) && ld % 4 == 0;
+  const long long tasks = (long long)M * (a.H + 2 * c->v.KH);
+  VN_REQUIRE(c->ctx, tasks < (1ll << 33), "%d rows are too many for one call", M);
+  const dim3 grid((unsigned)ceil_div(tasks, 8ll)), block(32, 8);
+  if (es == 4) VN_LAUNCH_NAMED(c->ctx, "qkv_append_kernel", qkv_append_kernel<float>, grid, block, 0, a);
+  else VN_LAUNCH_NAMED(c->ctx, "qkv_append_kernel", qkv_append_kernel<bf16>, grid, block, 0, a);
+  return VN_OK;
+}
+
+int32_t vn_qkv_read(vn_qkv* c, int32_t n_ent, const int32_t* ents, const int32_t* row_ent, int32_t T, int32_t M, int32_t start, int32_t offset, int32_t dtype,
+                    void* k_out, void* v_out) {
+  VN_CHECK_QKV(c);
+  QkvStep s;
+  if (int32_t st = step_of(c, n_ent, ents, row_ent, T, M, &s)) return st;
+  VN_REQUIRE(c->ctx, dtype == VN_F32 || dtype == VN_BF16, "values are read as float32 or bf16");
+  VN_REQUIRE(c->ctx, start >= -2 && offset >= 0, "start %d, offset %d", start, offset);
+  if (M == 0 || T == 0) return VN_OK;
+  VN_REQUIRE(c->ctx, k_out && v_out, "null output");
+  const int es = dtype == VN_F32 ? 4 : 2;
+  VN_REQUIRE(c->ctx, aligned(k_out, es) && aligned(v_out, es), "outputs are not aligned to their values");
+  const int vec = aligned(k_out, 4 * es) && aligned(v_out, 4 * es);
+  const long long items = (long long)M * c->v.KH * (c->v.d / 8);
+  VN_REQUIRE(c->ctx, items < (1ll << 38), "%d rows are too many for one call", M);
+  const dim3 grid((unsigned)ceil_div(items, 256ll), 2);
+#define READ(O, S) VN_LAUNCH_NAMED(c->ctx, "qkv_read_kernel", (qkv_read_kernel<O, S>), grid, 256, 0, c->v, s, start, offset, (O*)k_out, (O*)v_out, vec)
+  if (c->v.scheme == QKV_I8) { if (es == 4) READ(float, QKV_I8); else READ(bf16, QKV_I8); }
+  else { if (es == 4) READ(float, QKV_E4M3); else READ(bf16, QKV_E4M3); }
+#undef READ
+  return VN_OK;
+}
+
+int32_t vn_qkv_commit(vn_qkv* c, int32_t n_new, const int32_t* keep_idx, int32_t stride, const int32_t* n_keep, int32_t keep_add) {
+  VN_CHECK_QKV(c);
+  VN_REQUIRE(c->ctx, n_keep, "n_keep is null");
+  VN_REQUIRE(c->ctx, n_new >= 0, "n_new %d", n_new);
+  VN_REQUIRE(c->ctx, !keep_idx || (n_new <= QKV_MAX_DRAFT && stride >= 0), "rows are picked from at most %d, not %d", QKV_MAX_DRAFT, n_new);
+  VN_LAUNCH(c->ctx, qkv_commit_kernel, dim3(keep_idx ? c->v.KH : 1, c->v.max_batch), 256, 0, c->v, n_new, keep_idx, stride, n_keep, keep_add, c->tickets);
+  return VN_OK;
+}
+
+int32_t vn_qkv_attention(vn_qkv* c, const void* q, int32_t n_ent, const int32_t* ents, const int32_t* row_ent, int32_t T, int32_t M, const uint64_t* seen,
+                         const int32_t* depth, int32_t tree_per_row, int32_t window, float scale, void* out) {
+  VN_CHECK_QKV(c);
+  QkvAttnArgs a;
+  a.v = c->v;
+  if (int32_t st = step_of(c, n_ent, ents, row_ent, T, M, &a.step)) return st;
+  VN_REQUIRE(c->ctx, (seen == nullptr) == (depth == nullptr), "a tree has both tables");
+  VN_REQUIRE(c->ctx, !seen || T <= QKV_MAX_DRAFT, "a tree of %d rows, at most %d", T, QKV_MAX_DRAFT);
+  VN_REQUIRE(c->ctx, window >= 0, "window %d", window);
+  VN_REQUIRE(c->ctx, isfinite(scale) && scale > 0.f, "a scale above zero is needed");
+  if (M == 0 || T == 0) return VN_OK;
+  VN_REQUIRE(c->ctx, q && out, "null rows");
+  const int es = c->dtype == VN_F32 ? 4 : 2;
+  VN_REQUIRE(c->ctx, aligned(q, 4 * es) && aligned(out, 4 * es), "rows are not aligned to four values");
+  a.tree.seen = (const unsigned long long*)seen; a.tree.depth = depth; a.tree.per_row = tree_per_row;
+  a.q = q; a.out = out; a.window = window; a.scale = scale;
+  return qkv_attention(c, a);
+}
+
+}  // extern "C"
