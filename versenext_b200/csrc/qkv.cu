@@ -1,6 +1,7 @@
-// The paged 8-bit cache's entry points and the kernels that write, read and keep positions; attention is in qkv_attn.cu.
+// The paged 8-bit cache's entry points and the kernels that write, read and keep positions; attention is in qkv_attn.cuh.
 #include <string.h>
 
+#include <algorithm>
 #include <new>
 
 #include "qkv.cuh"
@@ -240,6 +241,7 @@ int32_t vn_qkv_create(vn_ctx* ctx, int32_t max_batch, int32_t max_seq, int32_t n
   for (int p : {32, 64, 80, 96, 128, 192, 256})
     if (!v.P && head_dim <= p) v.P = p;
   const size_t pool = (size_t)v.n_pages * v.KH * 2 * v.block_bytes();
+  const int ctas = QKV_MAX_CTAS * ctx->sm_count;
   int32_t st = VN_OK;
   auto get = [&](void** p, size_t bytes) {
     cudaError_t e = cudaMalloc(p, bytes);
@@ -251,7 +253,8 @@ int32_t vn_qkv_create(vn_ctx* ctx, int32_t max_batch, int32_t max_seq, int32_t n
     return e == cudaSuccess;
   };
   if (get((void**)&v.pool, pool) && get((void**)&c->table, (size_t)all * sizeof(int)) && get((void**)&v.lens, (size_t)max_batch * sizeof(int)) &&
-      get((void**)&v.status, 2 * sizeof(int)) && get((void**)&c->tickets, (size_t)max_batch * sizeof(int))) {
+      get((void**)&v.status, 3 * sizeof(int)) && get((void**)&c->tickets, (size_t)std::max(max_batch, ctas) * sizeof(int)) &&
+      get((void**)&c->part_o, (size_t)2 * ctas * QKV_PART * sizeof(float)) && get((void**)&c->part_ml, (size_t)2 * ctas * 32 * sizeof(float2))) {
     v.table = c->table;
     std::vector<int> t;
     try { t.resize((size_t)all); } catch (...) { vn_qkv_destroy(c); return vn_fail(ctx, VN_ERR_OOM, "out of host memory"); }
@@ -269,7 +272,7 @@ int32_t vn_qkv_destroy(vn_qkv* c) {
   if (!c) return VN_OK;
   cudaSetDevice(c->ctx->device);
   cudaStreamSynchronize(c->ctx->stream);
-  for (void* p : {(void*)c->v.pool, (void*)c->table, (void*)c->v.lens, (void*)c->v.status, c->parts, (void*)c->tickets})
+  for (void* p : {(void*)c->v.pool, (void*)c->table, (void*)c->v.lens, (void*)c->v.status, (void*)c->part_o, (void*)c->part_ml, (void*)c->tickets})
     if (p) cudaFree(p);
   delete c;
   return VN_OK;
@@ -310,12 +313,13 @@ int32_t vn_qkv_set_lengths(vn_qkv* c, const int32_t* lens, int32_t on_device) {
 
 int32_t vn_qkv_status(vn_qkv* c, int32_t* no_room, int32_t* bad_index) {
   VN_CHECK_QKV(c);
-  int s[2];
+  int s[3];
   VN_CUDA(c->ctx, cudaMemcpyAsync(s, c->v.status, sizeof s, cudaMemcpyDeviceToHost, c->ctx->stream));
   VN_CUDA(c->ctx, cudaMemsetAsync(c->v.status, 0, sizeof s, c->ctx->stream));
   VN_CUDA(c->ctx, cudaStreamSynchronize(c->ctx->stream));
   if (no_room) *no_room = s[0];
   if (bad_index) *bad_index = s[1];
+  if (s[2]) return vn_fail(c->ctx, VN_ERR_TIMEOUT, "a copy from the cache did not arrive");
   if (s[0]) return vn_fail(c->ctx, VN_ERR_OVERFLOW, "a position behind the cache's end, or without a page, was written or read");
   if (s[1]) return vn_fail(c->ctx, VN_ERR_INDEX, "a sequence, row or count outside its range was met");
   return VN_OK;
@@ -398,7 +402,8 @@ int32_t vn_qkv_attention(vn_qkv* c, const void* q, int32_t n_ent, const int32_t*
   VN_REQUIRE(c->ctx, aligned(q, 4 * es) && aligned(out, 4 * es), "rows are not aligned to four values");
   a.tree.seen = (const unsigned long long*)seen; a.tree.depth = depth; a.tree.per_row = tree_per_row;
   a.q = q; a.out = out; a.window = window; a.scale = scale;
-  return qkv_attention(c, a);
+  a.part_o = c->part_o; a.part_ml = c->part_ml; a.tickets = c->tickets;
+  return c->v.scheme == QKV_I8 ? qkv_attention_i8(c, a) : qkv_attention_e4m3(c, a);
 }
 
 }  // extern "C"

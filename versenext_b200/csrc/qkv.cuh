@@ -20,7 +20,7 @@ struct QkvView {
   unsigned char* pool = nullptr;
   const int* table = nullptr;                       // [max_batch][max_pages] page of a sequence's positions 64 i .., -1: none
   int* lens = nullptr;                              // [max_batch] committed positions
-  int* status = nullptr;                            // [2] a position without a page was wanted; a bad slot, row or length was met
+  int* status = nullptr;                            // [3] a position without a page was wanted; a bad slot, row or length was met; a copy did not arrive
   int max_batch = 0, max_pages = 0, n_pages = 0, H = 0, KH = 0, d = 0, P = 0, scheme = 0;
   __host__ __device__ __forceinline__ int capacity() const { return max_pages * KV_PAGE; }
   __host__ __device__ __forceinline__ int block_bytes() const { return QKV_BLOCK * (2 * P + 8); }
@@ -84,8 +84,8 @@ struct vn_qkv {
   QkvView v;
   int dtype = VN_BF16;
   int* table = nullptr;
-  void* parts = nullptr;                            // attention: partial results of blocks of a unit's keys
-  size_t part_bytes = 0;
+  float* part_o = nullptr;                          // attention: [2 CTAs][rows][P] results of a part of a unit's keys
+  float2* part_ml = nullptr;                        // [2 CTAs][rows] maximum and sum of its weights
   int* tickets = nullptr;                           // zero between kernels
 };
 
@@ -101,7 +101,10 @@ struct QkvAttnArgs {
   float2* part_ml = nullptr;
   int* tickets = nullptr;
 };
-int32_t qkv_attention(vn_qkv* c, const QkvAttnArgs& a);
+constexpr int QKV_MAX_CTAS = 3;                     // of the attention kernel on an SM
+constexpr int QKV_PART = 32 * 128;                  // values of a part: rows x padded head size, at most
+int32_t qkv_attention_i8(vn_qkv* c, const QkvAttnArgs& a);
+int32_t qkv_attention_e4m3(vn_qkv* c, const QkvAttnArgs& a);
 
 // value of one code
 template <int SCHEME> __device__ __forceinline__ float qkv_value(unsigned char c) {
