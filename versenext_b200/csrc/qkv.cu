@@ -33,7 +33,7 @@ template <typename T> __device__ __forceinline__ void put_quad(T* p, float4 v, b
 }
 
 __device__ __forceinline__ unsigned char code_of(float y, int scheme) {
-  if (scheme == QKV_I8) return (unsigned char)(signed char)max(-127, min(127, __float2int_rn(y)));
+  if (scheme == QKV_I8) return (unsigned char)(max(-127, min(127, __float2int_rn(y))) + 128);
   unsigned short r;
   asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(0.f), "f"(y));
   return (unsigned char)r;
@@ -98,7 +98,8 @@ __global__ void __launch_bounds__(256) qkv_append_kernel(AppendArgs a) {
   const int at = pos % QKV_BLOCK, P = a.v.P, t = qkv_turn(P / 16, at);
   unsigned char* codes = b + (is_v ? QKV_BLOCK * P : 0) + at * P;
   for (int c = 4 * lane; c < P; c += 128) {
-    uchar4 k = make_uchar4(0, 0, 0, 0);
+    const unsigned char none = a.v.scheme == QKV_I8 ? 128 : 0;
+    uchar4 k = make_uchar4(none, none, none, none);
     if (c < d && !bad) {
       const float4 v = *reinterpret_cast<const float4*>(s + c);
       k = make_uchar4(code_of(v.x / scale, a.v.scheme), code_of(v.y / scale, a.v.scheme), code_of(v.z / scale, a.v.scheme), code_of(v.w / scale, a.v.scheme));

@@ -4,7 +4,7 @@
 // keys, 32 of the values (P = padded head size); it is one piece of memory, so that a reader brings it in with one copy.  A
 // page is 64 positions = two blocks per head: block((page KH + head) 2 + half).  A head at a position is scale * code, with
 // scale = max |x| / 127 (int8) or / 448 (e4m3), at least 2^-126; where it holds a value that is not finite its scale is NaN and its codes are 0.
-// Within a block the 16-byte chunks of a position's codes are permuted by its number (chunk c stands at c ^ turn), so that the
+// int8 codes stand with 128 added.  Within a block the 16-byte chunks of a position's codes are permuted by its number (chunk c stands at c ^ turn), so that the
 // eight positions of a matrix that ldmatrix reads lie in different shared memory banks.
 #pragma once
 #include "rows.cuh"
@@ -108,7 +108,7 @@ int32_t qkv_attention_e4m3(vn_qkv* c, const QkvAttnArgs& a);
 
 // value of one code
 template <int SCHEME> __device__ __forceinline__ float qkv_value(unsigned char c) {
-  if (SCHEME == QKV_I8) return (float)(signed char)c;
+  if (SCHEME == QKV_I8) return (float)((int)c - 128);
   // e4m3 in a half: the same sign, exponent and mantissa fields, 2^8 apart
   const unsigned short h = (unsigned short)((c & 0x80) << 8 | (c & 0x7f) << 7);
   return __half2float(__ushort_as_half(h)) * 256.f;

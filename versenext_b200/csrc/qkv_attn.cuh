@@ -8,7 +8,8 @@
 // far, times 2^15, so that a half holds weights down to 2^-39 of the largest.
 //
 // What bounds it is the memory of the codes (few rows) or the mma.sync rate and the conversions (many): one warp reads and converts a
-// block of 32 positions for 16 MT rows (tokens x heads of a group), four warps of a CTA take every fourth block.  The blocks of
+// block of 32 positions for 8 NT rows (tokens x heads of a group), four warps of a CTA take every fourth block.  Positions are the
+// rows of the products and queries their columns (8 at a time): S = K q^T, O = V^T p^T, with p transposed by movmatrix between.  The blocks of
 // all (entry, rows, head) units form one line that is cut into equal shares for the CTAs, whatever the lengths; a unit that several
 // CTAs have is merged, in their order, by the one that ends last.
 #pragma once
@@ -21,15 +22,20 @@ constexpr int WARPS = 4, THREADS = 32 * WARPS;
 constexpr int MIN_SHARE = WARPS;                    // blocks of a CTA at least
 constexpr unsigned long long WAIT_CYCLES = 4000000000ull;   // a copy that has not come after about two seconds never will
 
-template <typename T, int P, int MT>
+template <typename T, int P, int NT>
 struct AttnCfg {
   static constexpr int NQ = sizeof(T) == 4 ? 2 : 1;           // halves of a query or weight
-  static constexpr int RT = 16 * MT, CH = P / 16, BLOCK = QKV_BLOCK * (2 * P + 8);
+  static constexpr int RT = 8 * NT, CH = P / 16, BLOCK = QKV_BLOCK * (2 * P + 8);
   static constexpr int QP = 2 * P + ((2 * P) % 64 == 0 ? 32 : 0);   // bytes of a staged query row: four rows' 32-byte pieces in 128 bytes of banks
-  static constexpr int STAGES = P <= 64 ? 4 : P <= 128 && MT * NQ == 1 ? 3 : 2;
-  static constexpr bool QREG = MT * NQ == 1 && P <= 128;      // query fragments in registers
-  static constexpr int RING = 0, Q = RING + WARPS * STAGES * BLOCK, MERGE = Q + NQ * RT * QP, ML = MERGE + 8192, ROWS = ML + WARPS * RT * 8,
-                       RF = ROWS + RT * 16, BARS = RF + RT * 4, SMEM = BARS + WARPS * STAGES * 8, PLAN = MERGE;   // the plan is read before anything is merged
+  static constexpr int STAGES = P <= 64 ? 4 : P <= 128 && NT >= 2 && NT * NQ <= 2 ? 3 : 2;
+  static constexpr bool QREG = NT * NQ <= 2 && NT * NQ * P <= 256;      // query fragments in registers
+  static constexpr int SUB = NT >= 4 ? 1 : 2;                 // chunks of 16 channels that are merged at a time
+  static constexpr int MP = 20;                               // pitch of a merged row: 16 lanes' pairs in different banks
+  static constexpr int CTAS = P > 192 || (P > 128 && NQ * NT > 1) ? 1 : P * NT <= 128 ? 3 : 2;
+  static constexpr int RING = 0, Q = RING + WARPS * STAGES * BLOCK, MERGE = Q + NQ * RT * QP, MERGE_BYTES = SUB * WARPS * RT * MP * 4, ML = MERGE + MERGE_BYTES,
+                       ROWS = ML + WARPS * RT * 8, RF = ROWS + RT * 16, BARS = RF + RT * 8, SMEM = BARS + WARPS * STAGES * 8, PLAN = MERGE;
+  static_assert(MERGE_BYTES >= (THREADS + 1) * 8, "the plan is read before anything is merged, from the same place");
+  static_assert(RT * P <= QKV_PART, "a part fits its place");
 };
 
 struct RowInfo { int t, away; unsigned long long seen; };    // t < 0: no row
@@ -61,6 +67,11 @@ __device__ __forceinline__ unsigned pack_f16(float lo, float hi) {
   return *reinterpret_cast<const unsigned*>(&h);
 }
 __device__ __forceinline__ float2 unpack_f16(unsigned u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
+__device__ __forceinline__ unsigned transposed(unsigned u) {
+  unsigned v;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(v) : "r"(u));
+  return v;
+}
 __device__ __forceinline__ float ex2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -68,19 +79,28 @@ __device__ __forceinline__ float ex2(float x) {
 }
 __device__ __forceinline__ float pow2(int biased) { return __uint_as_float((unsigned)min(max(biased, 0), 254) << 23); }   // 2^(biased - 127), 0 below
 
-// two codes of a register as halves.  int8: with the sign bit flipped a code plus 128 is put under the exponent of 1024, from which
-// 1152 is taken off.  e4m3: sign, exponent and mantissa moved to a half's places, 2^8 too small (the factors r and R allow for it).
-// PAIR: bytes 0 and 1 (0), 2 and 3 (1), 0 and 2 (2), 1 and 3 (3); u: the register, for int8 with its sign bits flipped
-template <int SCHEME, int PAIR> __device__ __forceinline__ unsigned halves_of(unsigned u) {
+// two codes of a register as halves.  int8: a code plus 128 is put under the exponent of 1024, from which 1152 is taken off (BIAS: it
+// is left there).  e4m3: the type's own conversion.
+// PAIR: bytes 0 and 1 (0), 2 and 3 (1); e4m3 takes neighbours only, so 0 and 2, 1 and 3 are brought together first
+__device__ __forceinline__ unsigned halves_of_e4m3(unsigned short u) {
+  unsigned r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(u));
+  return r;
+}
+template <int SCHEME, bool EVERY_OTHER, bool BIAS> __device__ __forceinline__ void halves_of(unsigned u, unsigned& lo, unsigned& hi) {
   if (SCHEME == QKV_I8) {
-    constexpr unsigned sel = PAIR == 0 ? 0x4140 : PAIR == 1 ? 0x4342 : PAIR == 2 ? 0x4240 : 0x4341;
-    const unsigned x = __byte_perm(u, 0x64646464u, sel);
-    const __half2 h = __hsub2(*reinterpret_cast<const __half2*>(&x), __half2half2(__ushort_as_half(0x6480)));
-    return *reinterpret_cast<const unsigned*>(&h);
+    lo = __byte_perm(u, 0x64646464u, EVERY_OTHER ? 0x4240 : 0x4140);
+    hi = __byte_perm(u, 0x64646464u, EVERY_OTHER ? 0x4341 : 0x4342);
+    if (BIAS) return;
+    const __half2 off = __half2half2(__ushort_as_half(0x6480));
+    const __half2 x = __hsub2(*reinterpret_cast<const __half2*>(&lo), off), y = __hsub2(*reinterpret_cast<const __half2*>(&hi), off);
+    lo = *reinterpret_cast<const unsigned*>(&x);
+    hi = *reinterpret_cast<const unsigned*>(&y);
+  } else {
+    if (EVERY_OTHER) u = __byte_perm(u, 0u, 0x3120);
+    lo = halves_of_e4m3((unsigned short)u);
+    hi = halves_of_e4m3((unsigned short)(u >> 16));
   }
-  constexpr unsigned sel = PAIR == 0 ? 0x1404 : PAIR == 1 ? 0x3424 : PAIR == 2 ? 0x2404 : 0x3414;
-  const unsigned x = __byte_perm(u, 0u, sel);
-  return ((x >> 1) & 0x3f803f80u) | (x & 0x80008000u);
 }
 
 // what a unit -- RT rows of an entry and one head -- reads
@@ -115,11 +135,11 @@ __device__ __forceinline__ bool unit_of(const QkvAttnArgs& a, int rts, long long
   return true;
 }
 
-template <typename T, int SCHEME, int P, int MT>
-__global__ void __launch_bounds__(THREADS, P > 192 ? 1 : 2) qkv_attn_kernel(QkvAttnArgs a, int rts) {
-  using C = AttnCfg<T, P, MT>;
-  static_assert(C::RT * P <= QKV_PART, "a part fits its place");
+template <typename T, int SCHEME, int P, int NT>
+__global__ void __launch_bounds__(THREADS, (AttnCfg<T, P, NT>::CTAS)) qkv_attn_kernel(QkvAttnArgs a, int rts) {
+  using C = AttnCfg<T, P, NT>;
   constexpr int RT = C::RT, CH = C::CH, ST = C::STAGES, NQ = C::NQ;
+  constexpr bool BIAS = SCHEME == QKV_I8 && NQ == 1;         // keys 1152 too large: taken off the sums instead, at the cost of some bits of them
   extern __shared__ __align__(128) unsigned char smem[];
   const QkvView& v = a.v;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rg = lane >> 2, rc = lane & 3;
@@ -128,7 +148,7 @@ __global__ void __launch_bounds__(THREADS, P > 192 ? 1 : 2) qkv_attn_kernel(QkvA
   unsigned char* ring = smem + C::RING + warp * ST * C::BLOCK;
   const unsigned ring_s = s_base + C::RING + warp * ST * C::BLOCK, bars = s_base + C::BARS + warp * ST * 8;
   RowInfo* s_rows = reinterpret_cast<RowInfo*>(smem + C::ROWS);
-  float* s_rf = reinterpret_cast<float*>(smem + C::RF);
+  float2* s_rf = reinterpret_cast<float2*>(smem + C::RF);    // r of a row, and what its sums begin with
   float2* s_ml = reinterpret_cast<float2*>(smem + C::ML);
   float* s_merge = reinterpret_cast<float*>(smem + C::MERGE);
   long long* s_plan = reinterpret_cast<long long*>(smem + C::PLAN);
@@ -226,6 +246,7 @@ __global__ void __launch_bounds__(THREADS, P > 192 ? 1 : 2) qkv_attn_kernel(QkvA
       top = __reduce_max_sync(0xffffffffu, top);
       const int e = top >= 0x7f800000u ? 140 : min(max((int)(top >> 23), 27), 254);      // a row that is not finite is left as it is
       const float up = pow2(267 - e);
+      float sum = 0.f;
 #pragma unroll
       for (int y = 0; y < (P > 128 ? 2 : 1); ++y) {
         const int c = 4 * lane + 128 * y;
@@ -234,13 +255,18 @@ __global__ void __launch_bounds__(THREADS, P > 192 ? 1 : 2) qkv_attn_kernel(QkvA
         uint2 h = make_uint2(pack_f16(w.x, w.y), pack_f16(w.z, w.w));
         unsigned char* to = smem + C::Q + r * C::QP + 2 * c;
         *reinterpret_cast<uint2*>(to) = h;
+        if (BIAS) {
+          const float2 p0 = unpack_f16(h.x), p1 = unpack_f16(h.y);
+          sum += (p0.x + p0.y) + (p1.x + p1.y);
+        }
         if (NQ == 2) {
           const float2 p0 = unpack_f16(h.x), p1 = unpack_f16(h.y);
           *reinterpret_cast<uint2*>(to + RT * C::QP) = make_uint2(pack_f16(w.x - p0.x, w.y - p0.y), pack_f16(w.z - p1.x, w.w - p1.y));
         }
       }
+      if (BIAS) sum = warp_sum(sum);
       if (lane == 0) {
-        s_rf[r] = fmaxf(a.scale * 1.4426950408889634f * pow2(e - 13 + (SCHEME == QKV_E4M3 ? 8 : 0)), 1.17549435e-38f);
+        s_rf[r] = make_float2(fmaxf(a.scale * 1.4426950408889634f * pow2(e - 13), 1.17549435e-38f), -1152.f * sum);
         RowInfo info = {-1, 0, 0};
         if (ok) {
           info.t = t;
@@ -256,30 +282,33 @@ __global__ void __launch_bounds__(THREADS, P > 192 ? 1 : 2) qkv_attn_kernel(QkvA
   stage_queries();
   __syncthreads();
   while (true) {
-    // ---- the warp's blocks of this segment
-    float acc[MT][CH][2][4], m_run[MT][2], l_run[MT][2], rf[MT][2];
-    unsigned qf[C::QREG ? CH : 1][4];
+    // ---- the warp's blocks of this segment.  A thread's rows are 8 nt + 2 rc + x (x = 0, 1), its positions 8 j + rg of a block
+    float acc[CH][NT][4], m_run[NT][2], l_run[NT][2], rf[NT][2], first[NT][2];
+    unsigned qf[C::QREG ? CH : 1][NT * NQ][2];
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
+    for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
       for (int k = 0; k < CH; ++k)
 #pragma unroll
-        for (int x = 0; x < 4; ++x) acc[mt][k][0][x] = acc[mt][k][1][x] = 0.f;
+        for (int x = 0; x < 4; ++x) acc[k][nt][x] = 0.f;
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        m_run[mt][h] = -CUDART_INF_F;
-        l_run[mt][h] = 0.f;
-        rf[mt][h] = s_rf[16 * mt + rg + 8 * h];
+      for (int x = 0; x < 2; ++x) {
+        m_run[nt][x] = -CUDART_INF_F;
+        l_run[nt][x] = 0.f;
+        const float2 r = s_rf[8 * nt + 2 * rc + x];
+        rf[nt][x] = r.x;
+        first[nt][x] = r.y;
       }
     }
-    auto query = [&](int mt, int half, int k, unsigned (&q)[4]) {
-      const unsigned char* p = smem + C::Q + half * RT * C::QP + (16 * mt + rg) * C::QP + 32 * k + 8 * rc;
-      const uint2 x = *reinterpret_cast<const uint2*>(p), y = *reinterpret_cast<const uint2*>(p + 8 * C::QP);
-      q[0] = x.x; q[1] = y.x; q[2] = x.y; q[3] = y.y;
+    auto query = [&](int nt, int half, int k, unsigned (&q)[2]) {
+      const uint2 x = *reinterpret_cast<const uint2*>(smem + C::Q + half * RT * C::QP + (8 * nt + rg) * C::QP + 32 * k + 8 * rc);
+      q[0] = x.x; q[1] = x.y;
     };
     if (C::QREG)
 #pragma unroll
-      for (int k = 0; k < CH; ++k) query(0, 0, k, qf[C::QREG ? k : 0]);
+      for (int k = 0; k < CH; ++k)
+#pragma unroll
+        for (int j = 0; j < NT * NQ; ++j) query(j / NQ, j % NQ, k, qf[C::QREG ? k : 0][j]);
     int R = 16;                                              // biased exponent of the largest scale of values met
     for (int k = 0, i = seg_a + warp; i < seg_b; ++k, i += WARPS, ++it) {
       if ((k & 31) == 0 && k) { page_cur = page_nxt; page_nxt = pages_of(k + 32); }
@@ -296,156 +325,127 @@ __global__ void __launch_bounds__(THREADS, P > 192 ? 1 : 2) qkv_attn_kernel(QkvA
         const int turn = qkv_turn(CH, lane);
         const int k0 = i * QKV_BLOCK;
         const bool full = k0 >= u.full_lo && k0 + QKV_BLOCK <= u.full_hi;
-        // ---- scores
-        float t[MT][4][4];
+        // ---- scores: register j of a read holds channels 4 rc .. + 3 of position 8 j + rg
+        float t[2][NT][4];
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int nb = 0; nb < 4; ++nb)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) t[mt][nb][x] = 0.f;
+          for (int x = 0; x < 4; ++x) t[0][nt][x] = t[1][nt][x] = BIAS ? first[nt][x & 1] : 0.f;
 #pragma unroll
         for (int kc = 0; kc < CH; ++kc) {
-          unsigned r[4];
+          unsigned r[4], ka[2][4];
           asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(row_s + ((kc ^ turn) << 4)));
-          unsigned b[4][2];
 #pragma unroll
-          for (int nb = 0; nb < 4; ++nb) {
-            if (SCHEME == QKV_I8) r[nb] ^= 0x80808080u;
-            b[nb][0] = halves_of<SCHEME, 0>(r[nb]);
-            b[nb][1] = halves_of<SCHEME, 1>(r[nb]);
-          }
+          for (int j = 0; j < 4; ++j) halves_of<SCHEME, false, BIAS>(r[j], ka[j >> 1][j & 1], ka[j >> 1][2 + (j & 1)]);
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int half = 0; half < NQ; ++half) {
-              unsigned q[4];
-              if (C::QREG) {
-#pragma unroll
-                for (int x = 0; x < 4; ++x) q[x] = qf[C::QREG ? kc : 0][x];
-              } else {
-                query(mt, half, kc, q);
-              }
-#pragma unroll
-              for (int nb = 0; nb < 4; ++nb) mma_f16(t[mt][nb], q, b[nb][0], b[nb][1]);
+              unsigned q[2];
+              if (C::QREG) { q[0] = qf[C::QREG ? kc : 0][nt * NQ + half][0]; q[1] = qf[C::QREG ? kc : 0][nt * NQ + half][1]; }
+              else query(nt, half, kc, q);
+              mma_f16(t[0][nt], ka[0], q[0], q[1]);
+              mma_f16(t[1][nt], ka[1], q[0], q[1]);
             }
         }
         // ---- scales of the block: the largest of the values' that count
         {
-          const float vs = sc[QKV_BLOCK + lane];
-          const unsigned b = __float_as_uint(vs);
+          const unsigned b = __float_as_uint(sc[QKV_BLOCK + lane]);
           const bool counts = (full || (k0 + lane >= u.lo && k0 + lane < u.hi)) && b < 0x7f800000u;
           const int e = (int)(__reduce_max_sync(0xffffffffu, counts ? b : 0u) >> 23);
           if (e > R) {
             const float f = pow2(127 + R - e);
             R = e;
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
+            for (int c = 0; c < CH; ++c)
 #pragma unroll
-              for (int c = 0; c < CH; ++c)
+              for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int x = 0; x < 4; ++x) { acc[mt][c][0][x] *= f; acc[mt][c][1][x] *= f; }
+                for (int x = 0; x < 4; ++x) acc[c][nt][x] *= f;
           }
         }
         const float rs = pow2(268 - R);
+        float ks[4], vs[4];
 #pragma unroll
-        for (int nb = 0; nb < 4; ++nb) {
-          const float2 ks = *reinterpret_cast<const float2*>(sc + 8 * nb + 2 * rc);
+        for (int j = 0; j < 4; ++j) { ks[j] = sc[8 * j + rg]; vs[j] = sc[QKV_BLOCK + 8 * j + rg] * rs; }
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int x = 0; x < 4; ++x) t[mt][nb][x] *= x & 1 ? ks.y : ks.x;
-        }
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) t[j >> 1][nt][2 * (j & 1) + x] *= ks[j];
         if (!full) {
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const RowInfo row = s_rows[16 * mt + rg + 8 * h];
+            for (int x = 0; x < 2; ++x) {
+              const RowInfo row = s_rows[8 * nt + 2 * rc + x];
 #pragma unroll
-              for (int nb = 0; nb < 4; ++nb)
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                  const int key = k0 + 8 * nb + 2 * rc + x, j = key - u.len;
-                  bool see;
-                  if (j < 0) see = a.window == 0 || u.len + row.away - key < a.window;
-                  else if (a.tree.seen) see = j < u.n && ((row.seen >> j) & 1);
-                  else see = j <= row.t && (a.window == 0 || row.t - j < a.window);
-                  if (row.t < 0 || !see || key >= u.hi) t[mt][nb][2 * h + x] = -CUDART_INF_F;
-                }
+              for (int j = 0; j < 4; ++j) {
+                const int key = k0 + 8 * j + rg, n = key - u.len;
+                bool see;
+                if (n < 0) see = a.window == 0 || u.len + row.away - key < a.window;
+                else if (a.tree.seen) see = n < u.n && ((row.seen >> n) & 1);
+                else see = n <= row.t && (a.window == 0 || row.t - n < a.window);
+                if (row.t < 0 || !see || key >= u.hi) t[j >> 1][nt][2 * (j & 1) + x] = -CUDART_INF_F;
+              }
             }
         }
         // ---- weights
-        unsigned pa[MT][NQ][2][4];                           // halves of the weights of 16 keys, as the product takes them
+        unsigned pb[NT][NQ][4];                              // of positions 8 j + 2 rc, + 1 and row 8 nt + rg
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
+        for (int nt = 0; nt < NT; ++nt) {
           float f[2], base[2];
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float mx = t[mt][0][2 * h];
+          for (int x = 0; x < 2; ++x) {
+            float mx = fmaxf(fmaxf(t[0][nt][x], t[0][nt][2 + x]), fmaxf(t[1][nt][x], t[1][nt][2 + x]));
 #pragma unroll
-            for (int nb = 0; nb < 4; ++nb) mx = fmaxf(mx, fmaxf(t[mt][nb][2 * h], t[mt][nb][2 * h + 1]));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-            mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-            const float m = fmaxf(m_run[mt][h], mx * rf[mt][h]);
-            base[h] = m == -CUDART_INF_F ? 0.f : m;          // nothing seen yet: every weight becomes exp2(-inf) = 0
-            f[h] = ex2(m_run[mt][h] - base[h]);
-            m_run[mt][h] = m;
+            for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+            const float m = fmaxf(m_run[nt][x], mx * rf[nt][x]);
+            base[x] = m == -CUDART_INF_F ? 0.f : m;          // nothing seen yet: every weight becomes exp2(-inf) = 0
+            f[x] = ex2(m_run[nt][x] - base[x]);
+            m_run[nt][x] = m;
           }
           if (__any_sync(0xffffffffu, f[0] != 1.f || f[1] != 1.f)) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              l_run[mt][h] *= f[h];
+            for (int x = 0; x < 2; ++x) {
+              l_run[nt][x] *= f[x];
 #pragma unroll
-              for (int c = 0; c < CH; ++c)
-#pragma unroll
-                for (int x = 0; x < 2; ++x) { acc[mt][c][0][2 * h + x] *= f[h]; acc[mt][c][1][2 * h + x] *= f[h]; }
+              for (int c = 0; c < CH; ++c) { acc[c][nt][x] *= f[x]; acc[c][nt][2 + x] *= f[x]; }
             }
           }
 #pragma unroll
-          for (int nb = 0; nb < 4; ++nb) {
-            float2 vs = *reinterpret_cast<const float2*>(sc + QKV_BLOCK + 8 * nb + 2 * rc);
-            vs.x *= rs; vs.y *= rs;
+          for (int j = 0; j < 4; ++j) {
+            float w[2];
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const float s0 = t[mt][nb][2 * h], s1 = t[mt][nb][2 * h + 1];
-              const float p0 = ex2(fmaf(s0, rf[mt][h], -base[h])), p1 = ex2(fmaf(s1, rf[mt][h], -base[h]));
-              l_run[mt][h] += p0 + p1;                       // this lane's share; the four lanes of a row are summed at the end
-              float w0 = p0 * vs.x, w1 = p1 * vs.y;
-              if (!full) {                                   // what a row does not see may have any scale, NaN too
-                if (s0 == -CUDART_INF_F) w0 = 0.f;
-                if (s1 == -CUDART_INF_F) w1 = 0.f;
-              }
-              const unsigned hi = pack_f16(w0, w1);
-              pa[mt][0][nb >> 1][h + 2 * (nb & 1)] = hi;
-              if (NQ == 2) {
-                const float2 w = unpack_f16(hi);
-                pa[mt][NQ - 1][nb >> 1][h + 2 * (nb & 1)] = pack_f16(w0 - w.x, w1 - w.y);
-              }
+            for (int x = 0; x < 2; ++x) {
+              const float s1 = t[j >> 1][nt][2 * (j & 1) + x], p = ex2(fmaf(s1, rf[nt][x], -base[x]));
+              l_run[nt][x] += p;                             // this lane's share; the eight lanes of a row are summed at the end
+              w[x] = p * vs[j];
+              if (!full && s1 == -CUDART_INF_F) w[x] = 0.f;  // what a row does not see may have any scale, NaN too
+            }
+            const unsigned hi = pack_f16(w[0], w[1]);
+            pb[nt][0][j] = transposed(hi);
+            if (NQ == 2) {
+              const float2 g = unpack_f16(hi);
+              pb[nt][NQ - 1][j] = transposed(pack_f16(w[0] - g.x, w[1] - g.y));
             }
           }
         }
-        // ---- values: register j of a transposed read holds channels 2 n, 2 n + 1 of positions 8 j + 2 rc, + 1 (n = lane / 4)
+        // ---- values: register j of a transposed read holds channels 2 rg, 2 rg + 1 of positions 8 j + 2 rc, + 1; row m of the
+        // product is channel 2 m (m < 8) or 2 (m - 8) + 1
 #pragma unroll
         for (int kc = 0; kc < CH; ++kc) {
-          unsigned r[4];
+          unsigned r[4], va[2][4];
           asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(row_s + QKV_BLOCK * P + ((kc ^ turn) << 4)));
-          unsigned b[2][4];
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            if (SCHEME == QKV_I8) r[j] ^= 0x80808080u;
-            b[0][j] = halves_of<SCHEME, 2>(r[j]);
-            b[1][j] = halves_of<SCHEME, 3>(r[j]);
-          }
+          for (int j = 0; j < 4; ++j) halves_of<SCHEME, true, false>(r[j], va[j >> 1][2 * (j & 1)], va[j >> 1][2 * (j & 1) + 1]);
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int half = 0; half < NQ; ++half)
 #pragma unroll
-              for (int ks = 0; ks < 2; ++ks) {
-                mma_f16(acc[mt][kc][0], pa[mt][half][ks], b[0][2 * ks], b[0][2 * ks + 1]);
-                mma_f16(acc[mt][kc][1], pa[mt][half][ks], b[1][2 * ks], b[1][2 * ks + 1]);
-              }
+              for (int ks2 = 0; ks2 < 2; ++ks2) mma_f16(acc[kc][nt], va[ks2], pb[nt][half][2 * ks2], pb[nt][half][2 * ks2 + 1]);
         }
       }
       __syncwarp();                                          // all lanes are done with the stage
@@ -471,32 +471,30 @@ __global__ void __launch_bounds__(THREADS, P > 192 ? 1 : 2) qkv_attn_kernel(QkvA
       begin_segment();
     }
     // ---- the four warps' results of a row
-    const float r_inv = pow2(R - 14 + (SCHEME == QKV_E4M3 ? 8 : 0));
+    const float r_inv = pow2(R - 14);
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float l = l_run[mt][h];
-        l += __shfl_xor_sync(0xffffffffu, l, 1);
-        l += __shfl_xor_sync(0xffffffffu, l, 2);
-        if (rc == 0) s_ml[warp * RT + 16 * mt + rg + 8 * h] = make_float2(m_run[mt][h], l);
+      for (int x = 0; x < 2; ++x) {
+        float l = l_run[nt][x];
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+        if (rg == 0) s_ml[warp * RT + 8 * nt + 2 * rc + x] = make_float2(m_run[nt][x], l);
       }
     __syncthreads();
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int r = 16 * mt + rg + 8 * h;
+      for (int x = 0; x < 2; ++x) {
+        const int r = 8 * nt + 2 * rc + x;
         float m = -CUDART_INF_F;
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) m = fmaxf(m, s_ml[w * RT + r].x);
-        const float f = m_run[mt][h] == -CUDART_INF_F ? 0.f : ex2(m_run[mt][h] - m) * r_inv;
+        const float f = m_run[nt][x] == -CUDART_INF_F ? 0.f : ex2(m_run[nt][x] - m) * r_inv;
 #pragma unroll
-        for (int c = 0; c < CH; ++c)
-#pragma unroll
-          for (int x = 0; x < 2; ++x) { acc[mt][c][0][2 * h + x] *= f; acc[mt][c][1][2 * h + x] *= f; }
+        for (int c = 0; c < CH; ++c) { acc[c][nt][x] *= f; acc[c][nt][2 + x] *= f; }
       }
-    constexpr int SUB = 2 / MT;                              // chunks of 16 channels that are exchanged at a time
+    constexpr int SUB = C::SUB, MP = C::MP;
     const int o_sub = tid / (RT * 4), o_row = tid / 4 % RT, o_c = 4 * (tid % 4), f = du.f0 + o_row;
     const int part = 2 * (int)blockIdx.x + ((int)blockIdx.x == cta0 ? 1 : 0);
     float m_all = -CUDART_INF_F, l_all = 0.f;
@@ -515,22 +513,20 @@ __global__ void __launch_bounds__(THREADS, P > 192 ? 1 : 2) qkv_attn_kernel(QkvA
 #pragma unroll
       for (int sub = 0; sub < SUB; ++sub) {
         if (c0 + sub >= CH) break;
+        const int cc = c0 + sub < CH ? c0 + sub : 0;
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float (&x)[2][4] = acc[mt][c0 + sub < CH ? c0 + sub : 0];
-            *reinterpret_cast<float4*>(s_merge + ((sub * WARPS + warp) * RT + 16 * mt + rg + 8 * h) * 16 + 4 * rc) =
-                make_float4(x[0][2 * h], x[1][2 * h], x[0][2 * h + 1], x[1][2 * h + 1]);
-          }
+          for (int x = 0; x < 2; ++x)
+            *reinterpret_cast<float2*>(s_merge + ((sub * WARPS + warp) * RT + 8 * nt + 2 * rc + x) * MP + 2 * rg) = make_float2(acc[cc][nt][x], acc[cc][nt][2 + x]);
       }
       __syncthreads();
       const int c = 16 * (c0 + o_sub) + o_c;
-      if (f < du.nf && c < P) {
+      if (o_sub < SUB && f < du.nf && c < P) {
         float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
         for (int w = 0; w < WARPS; ++w) {
-          const float4 y = *reinterpret_cast<const float4*>(s_merge + ((o_sub * WARPS + w) * RT + o_row) * 16 + o_c);
+          const float4 y = *reinterpret_cast<const float4*>(s_merge + ((o_sub * WARPS + w) * RT + o_row) * MP + o_c);
           x = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
         }
         if (!whole) store4(part_o + c, x);
@@ -577,11 +573,11 @@ __global__ void __launch_bounds__(THREADS, P > 192 ? 1 : 2) qkv_attn_kernel(QkvA
   }
 }
 
-template <typename T, int SCHEME, int P, int MT>
+template <typename T, int SCHEME, int P, int NT>
 int32_t launch(vn_qkv* c, const QkvAttnArgs& a) {
-  using C = AttnCfg<T, P, MT>;
+  using C = AttnCfg<T, P, NT>;
   vn_ctx* ctx = c->ctx;
-  auto kernel = qkv_attn_kernel<T, SCHEME, P, MT>;
+  auto kernel = qkv_attn_kernel<T, SCHEME, P, NT>;
   static int per_sm[64] = {};
   int& occ = per_sm[ctx->device & 63];
   if (!occ) {
@@ -602,20 +598,22 @@ int32_t launch(vn_qkv* c, const QkvAttnArgs& a) {
 
 template <int SCHEME>
 int32_t pick(vn_qkv* c, const QkvAttnArgs& a) {
-  // 32 rows share the conversions of a block where there are more than 16 and registers for their results
-  const bool wide = (long long)a.step.T * (a.v.H / a.v.KH) > 16;
-#define GO(P, MT) return c->dtype == VN_F32 ? launch<float, SCHEME, P, MT>(c, a) : launch<bf16, SCHEME, P, MT>(c, a)
-#define GO2(P) do { if (wide) GO(P, 2); else GO(P, 1); } while (0)
+  // as few columns as hold the rows of an entry; 32 share the conversions of a block where there are more than 16
+  const long long rows = (long long)a.step.T * (a.v.H / a.v.KH);
+#define GO(P, NT) return c->dtype == VN_F32 ? launch<float, SCHEME, P, NT>(c, a) : launch<bf16, SCHEME, P, NT>(c, a)
+#define GO2(P) do { if (rows <= 8) GO(P, 1); else GO(P, 2); } while (0)
+#define GO4(P) do { if (rows <= 8) GO(P, 1); else if (rows <= 16) GO(P, 2); else GO(P, 4); } while (0)
   switch (a.v.P) {
-    case 32: GO2(32);
-    case 64: GO2(64);
-    case 80: GO2(80);
-    case 96: GO2(96);
-    case 128: GO2(128);
-    case 192: GO(192, 1);
-    case 256: GO(256, 1);
+    case 32: GO4(32);
+    case 64: GO4(64);
+    case 80: GO4(80);
+    case 96: GO4(96);
+    case 128: GO4(128);
+    case 192: GO2(192);
+    case 256: GO2(256);
     default: return vn_fail(c->ctx, VN_ERR_UNSUPPORTED, "pitch %d", a.v.P);
   }
+#undef GO4
 #undef GO2
 #undef GO
 }

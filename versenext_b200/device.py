@@ -11,6 +11,7 @@ role that `torch.Tensor` plays for the reference's GPU path
 from __future__ import annotations
 
 import ctypes as C
+import math
 import threading
 
 import numpy as np
@@ -209,7 +210,7 @@ class DeviceArray:
 
     @property
     def size(self):
-        return int(np.prod(self.shape, dtype=np.int64))
+        return math.prod(self.shape)
 
     @property
     def nbytes(self):
