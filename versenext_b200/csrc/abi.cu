@@ -38,6 +38,7 @@ int32_t vn_ctx_destroy(vn_ctx* ctx) {
   if (ctx->ws) cudaFree(ctx->ws);
   if (ctx->flush) cudaFree(ctx->flush);
   if (ctx->tickets) cudaFree(ctx->tickets);
+  if (ctx->qkv_parts) cudaFree(ctx->qkv_parts);
   cudaStreamDestroy(ctx->stream);
   delete ctx;
   return VN_OK;

@@ -27,6 +27,8 @@ struct vn_ctx {
   // arrival counters for kernels whose last CTA finishes a row's work (VN_TICKETS ints, zero between kernels:
   // whoever takes the last ticket sets the counter back)
   int* tickets = nullptr;
+  // attention over 8-bit caches: partial results, of one size for all caches; made with the first of them
+  void* qkv_parts = nullptr;
   int sm_count = 148;
   // when set, every Philox offset of the acceptance / sampling kernels is incremented by *offset_src
   // (a round counter that lives on the device, so that a captured graph draws fresh numbers on every replay)

@@ -1,7 +1,6 @@
 // The paged 8-bit cache's entry points and the kernels that write, read and keep positions; attention is in qkv_attn.cuh.
 #include <string.h>
 
-#include <algorithm>
 #include <new>
 
 #include "qkv.cuh"
@@ -196,6 +195,16 @@ __global__ void set_lengths_kernel(int* __restrict__ lens, const int* __restrict
   if (i < n) lens[i] = from[i];
 }
 
+// layout of vn_ctx::qkv_parts: two parts for every CTA that the attention kernel may have
+struct Parts { size_t ml, cuts, bytes; };
+Parts parts_of(const vn_ctx* ctx) {
+  Parts p;
+  p.ml = (size_t)2 * ctx->sm_count * QKV_PART * sizeof(float);
+  p.cuts = p.ml + (size_t)2 * ctx->sm_count * QKV_MAX_CTAS * 128 * sizeof(float2);
+  p.bytes = p.cuts + (size_t)ctx->sm_count * QKV_MAX_CTAS * sizeof(QkvCut);
+  return p;
+}
+
 bool aligned(const void* p, size_t n) { return ((uintptr_t)p & (n - 1)) == 0; }
 
 int32_t step_of(vn_qkv* c, int32_t n_ent, const int32_t* ents, const int32_t* row_ent, int32_t T, int32_t M, QkvStep* s) {
@@ -242,7 +251,6 @@ int32_t vn_qkv_create(vn_ctx* ctx, int32_t max_batch, int32_t max_seq, int32_t n
   for (int p : {32, 64, 80, 96, 128, 192, 256})
     if (!v.P && head_dim <= p) v.P = p;
   const size_t pool = (size_t)v.n_pages * v.KH * 2 * v.block_bytes();
-  const int ctas = QKV_MAX_CTAS * ctx->sm_count;
   int32_t st = VN_OK;
   auto get = [&](void** p, size_t bytes) {
     cudaError_t e = cudaMalloc(p, bytes);
@@ -254,8 +262,8 @@ int32_t vn_qkv_create(vn_ctx* ctx, int32_t max_batch, int32_t max_seq, int32_t n
     return e == cudaSuccess;
   };
   if (get((void**)&v.pool, pool) && get((void**)&c->table, (size_t)all * sizeof(int)) && get((void**)&v.lens, (size_t)max_batch * sizeof(int)) &&
-      get((void**)&v.status, 3 * sizeof(int)) && get((void**)&c->tickets, (size_t)std::max(max_batch, ctas) * sizeof(int)) &&
-      get((void**)&c->part_o, (size_t)2 * ctas * QKV_PART * sizeof(float)) && get((void**)&c->part_ml, (size_t)2 * ctas * 32 * sizeof(float2))) {
+      get((void**)&v.status, 3 * sizeof(int)) && get((void**)&c->tickets, (size_t)max_batch * sizeof(int)) &&
+      (ctx->qkv_parts || get(&ctx->qkv_parts, parts_of(ctx).bytes))) {
     v.table = c->table;
     std::vector<int> t;
     try { t.resize((size_t)all); } catch (...) { vn_qkv_destroy(c); return vn_fail(ctx, VN_ERR_OOM, "out of host memory"); }
@@ -273,7 +281,7 @@ int32_t vn_qkv_destroy(vn_qkv* c) {
   if (!c) return VN_OK;
   cudaSetDevice(c->ctx->device);
   cudaStreamSynchronize(c->ctx->stream);
-  for (void* p : {(void*)c->v.pool, (void*)c->table, (void*)c->v.lens, (void*)c->v.status, (void*)c->part_o, (void*)c->part_ml, (void*)c->tickets})
+  for (void* p : {(void*)c->v.pool, (void*)c->table, (void*)c->v.lens, (void*)c->v.status, (void*)c->tickets})
     if (p) cudaFree(p);
   delete c;
   return VN_OK;
@@ -403,7 +411,10 @@ int32_t vn_qkv_attention(vn_qkv* c, const void* q, int32_t n_ent, const int32_t*
   VN_REQUIRE(c->ctx, aligned(q, 4 * es) && aligned(out, 4 * es), "rows are not aligned to four values");
   a.tree.seen = (const unsigned long long*)seen; a.tree.depth = depth; a.tree.per_row = tree_per_row;
   a.q = q; a.out = out; a.window = window; a.scale = scale;
-  a.part_o = c->part_o; a.part_ml = c->part_ml; a.tickets = c->tickets;
+  const Parts p = parts_of(c->ctx);
+  a.part_o = (float*)c->ctx->qkv_parts;
+  a.part_ml = (float2*)((char*)c->ctx->qkv_parts + p.ml);
+  a.cuts = (QkvCut*)((char*)c->ctx->qkv_parts + p.cuts);
   return c->v.scheme == QKV_I8 ? qkv_attention_i8(c, a) : qkv_attention_e4m3(c, a);
 }
 

@@ -84,10 +84,11 @@ struct vn_qkv {
   QkvView v;
   int dtype = VN_BF16;
   int* table = nullptr;
-  float* part_o = nullptr;                          // attention: [2 CTAs][rows][P] results of a part of a unit's keys
-  float2* part_ml = nullptr;                        // [2 CTAs][rows] maximum and sum of its weights
   int* tickets = nullptr;                           // zero between kernels
 };
+
+// a unit whose blocks several CTAs have, by its first CTA: rows f0 .. of nf (tokens x heads of the group) from row r0 on; n parts, 0: none
+struct QkvCut { int r0, f0, nf, head, n; };
 
 struct QkvAttnArgs {
   QkvView v;
@@ -97,12 +98,12 @@ struct QkvAttnArgs {
   void* out = nullptr;
   int window = 0;
   float scale = 1.f;
-  float* part_o = nullptr;
+  float* part_o = nullptr;                          // [2 CTAs][rows of a unit][P] results of a CTA's first and last unit
   float2* part_ml = nullptr;
-  int* tickets = nullptr;
+  QkvCut* cuts = nullptr;                           // [CTAs]
 };
 constexpr int QKV_MAX_CTAS = 3;                     // of the attention kernel on an SM
-constexpr int QKV_PART = 32 * 128;                  // values of a part: rows x padded head size, at most
+constexpr int QKV_PART = 2 * 128 * 128;             // values of parts: CTAs on an SM x rows x padded head size, at most
 int32_t qkv_attention_i8(vn_qkv* c, const QkvAttnArgs& a);
 int32_t qkv_attention_e4m3(vn_qkv* c, const QkvAttnArgs& a);
 

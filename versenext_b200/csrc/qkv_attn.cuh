@@ -10,8 +10,9 @@
 // What bounds it is the memory of the codes (few rows) or the mma.sync rate and the conversions (many): one warp reads and converts a
 // block of 32 positions for 8 NT rows (tokens x heads of a group), four warps of a CTA take every fourth block.  Positions are the
 // rows of the products and queries their columns (8 at a time): S = K q^T, O = V^T p^T, with p transposed by movmatrix between.  The blocks of
-// all (entry, rows, head) units form one line that is cut into equal shares for the CTAs, whatever the lengths; a unit that several
-// CTAs have is merged, in their order, by the one that ends last.
+// all (entry, rows, head) units form one line that is cut into equal shares for the CTAs, whatever the lengths; the parts of a unit that
+// several CTAs have are merged, in their order, by a second kernel that has all SMs for it (one CTA that merged a unit's parts by
+// itself took 10 to 15 us for 7 parts of 64 rows or 56 parts of 8).
 #pragma once
 #include "qkv.cuh"
 
@@ -20,27 +21,32 @@ namespace qkv_detail {
 using bf16 = __nv_bfloat16;
 constexpr int WARPS = 4, THREADS = 32 * WARPS;
 constexpr int MIN_SHARE = WARPS;                    // blocks of a CTA at least
+constexpr int UNCUT = 8;                            // blocks of a unit that is never cut
 constexpr unsigned long long WAIT_CYCLES = 4000000000ull;   // a copy that has not come after about two seconds never will
 
-template <typename T, int P, int NT>
+// RS = 1: the warps share a unit's rows and split its blocks; RS = 4: they split its rows and share its blocks
+template <typename T, int P, int NT, int RS>
 struct AttnCfg {
   static constexpr int NQ = sizeof(T) == 4 ? 2 : 1;           // halves of a query or weight
-  static constexpr int RT = 8 * NT, CH = P / 16, BLOCK = QKV_BLOCK * (2 * P + 8);
+  static constexpr int WR = 8 * NT, RT = WR * RS, CH = P / 16, BLOCK = QKV_BLOCK * (2 * P + 8);   // rows of a warp, of a unit
+  static constexpr int RINGS = WARPS / RS;
   static constexpr int QP = 2 * P + ((2 * P) % 64 == 0 ? 32 : 0);   // bytes of a staged query row: four rows' 32-byte pieces in 128 bytes of banks
-  static constexpr int STAGES = P <= 64 ? 4 : P <= 128 && NT >= 2 && NT * NQ <= 2 ? 3 : 2;
-  static constexpr bool QREG = NT * NQ <= 2 && NT * NQ * P <= 256;      // query fragments in registers
-  static constexpr int SUB = NT >= 4 ? 1 : 2;                 // chunks of 16 channels that are merged at a time
+  static constexpr int STAGES = RS > 1 ? 4 : P <= 64 ? 4 : P <= 128 && NT >= 2 && NT * NQ <= 2 ? 3 : 2;
+  static constexpr int CTAS = RS > 1 ? (P * NT <= 256 && NT < 4 && NQ == 1 ? 3 : P * NT <= 512 ? 2 : 1) : P > 192 || (P > 128 && NQ * NT > 1) ? 1 : P * NT <= 128 ? 3 : 2;
+  static constexpr bool QREG = NT * NQ <= 2 && NT * NQ * P <= (RS > 1 ? 128 : 256);      // query fragments in registers
+  static constexpr int SUB = RS > 1 ? 0 : NT >= 4 ? 1 : 2;    // chunks of 16 channels that are merged at a time
   static constexpr int MP = 20;                               // pitch of a merged row: 16 lanes' pairs in different banks
-  static constexpr int CTAS = P > 192 || (P > 128 && NQ * NT > 1) ? 1 : P * NT <= 128 ? 3 : 2;
-  static constexpr int RING = 0, Q = RING + WARPS * STAGES * BLOCK, MERGE = Q + NQ * RT * QP, MERGE_BYTES = SUB * WARPS * RT * MP * 4, ML = MERGE + MERGE_BYTES,
-                       ROWS = ML + WARPS * RT * 8, RF = ROWS + RT * 16, BARS = RF + RT * 8, SMEM = BARS + WARPS * STAGES * 8, PLAN = MERGE;
-  static_assert(MERGE_BYTES >= (THREADS + 1) * 8, "the plan is read before anything is merged, from the same place");
-  static_assert(RT * P <= QKV_PART, "a part fits its place");
+  static constexpr int RING = 0, Q = RING + RINGS * STAGES * BLOCK, MERGE = Q + NQ * RT * QP,
+                       MERGE_BYTES = SUB * WARPS * RT * MP * 4 > (THREADS + 8) * 4 ? SUB * WARPS * RT * MP * 4 : (THREADS + 8) * 4, ML = MERGE + MERGE_BYTES,
+                       ROWS = ML + (RS > 1 ? 0 : WARPS * RT * 8), RF = ROWS + RT * 16, BARS = RF + RT * 8, SMEM = BARS + RINGS * STAGES * 16,
+                       PLAN = MERGE;                          // read before anything is merged
+  static_assert(CTAS * RT * P <= QKV_PART, "parts fit their place");
 };
 
 struct RowInfo { int t, away; unsigned long long seen; };    // t < 0: no row
 
-__device__ __forceinline__ void mbar_init1(unsigned bar) { asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bar)); }
+__device__ __forceinline__ void mbar_init(unsigned bar, int count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count)); }
+__device__ __forceinline__ void mbar_arrive1(unsigned bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
 __device__ __forceinline__ bool mbar_try1(unsigned bar, unsigned parity) {
   unsigned ok;
   asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
@@ -111,14 +117,14 @@ struct Unit {
 };
 
 template <int RT>
-__device__ __forceinline__ bool unit_of(const QkvAttnArgs& a, int rts, long long z, Unit& u) {
-  const int e = (int)(z / rts), rt = (int)(z % rts), G = a.v.H / a.v.KH;
+__device__ __forceinline__ bool unit_of(const QkvAttnArgs& a, int rts, int z, Unit& u) {
+  const int e = rts == 1 ? z : z / rts, rt = rts == 1 ? 0 : z - e * rts, G = a.v.H / a.v.KH;
   u.tiles = 0;
   if (!a.step.entry(a.v, e, &u.slot, &u.r0, &u.n)) return false;
   u.f0 = rt * RT;
   u.nf = u.n * G;
   if (u.f0 >= u.nf) return false;
-  const int t0 = u.f0 / G, t1 = (min(u.f0 + RT, u.nf) - 1) / G;
+  const int t0 = rts == 1 ? 0 : u.f0 / G, t1 = rts == 1 ? u.n - 1 : (min(u.f0 + RT, u.nf) - 1) / G;
   u.len = a.v.len(u.slot);
   const bool tree = a.tree.seen != nullptr;
   u.hi = min(u.len + (tree ? u.n : t1 + 1), a.v.capacity());
@@ -135,9 +141,10 @@ __device__ __forceinline__ bool unit_of(const QkvAttnArgs& a, int rts, long long
   return true;
 }
 
-template <typename T, int SCHEME, int P, int NT>
-__global__ void __launch_bounds__(THREADS, (AttnCfg<T, P, NT>::CTAS)) qkv_attn_kernel(QkvAttnArgs a, int rts) {
-  using C = AttnCfg<T, P, NT>;
+template <typename T, int SCHEME, int P, int NT, int RS>
+__global__ void __launch_bounds__(THREADS, (AttnCfg<T, P, NT, RS>::CTAS)) qkv_attn_kernel(QkvAttnArgs a, int rts, bool split) {
+  pdl_trigger();
+  using C = AttnCfg<T, P, NT, RS>;
   constexpr int RT = C::RT, CH = C::CH, ST = C::STAGES, NQ = C::NQ;
   constexpr bool BIAS = SCHEME == QKV_I8 && NQ == 1;         // keys 1152 too large: taken off the sums instead, at the cost of some bits of them
   extern __shared__ __align__(128) unsigned char smem[];
@@ -145,62 +152,65 @@ __global__ void __launch_bounds__(THREADS, (AttnCfg<T, P, NT>::CTAS)) qkv_attn_k
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rg = lane >> 2, rc = lane & 3;
   const int G = v.H / v.KH;
   const unsigned s_base = (unsigned)__cvta_generic_to_shared(smem);
-  unsigned char* ring = smem + C::RING + warp * ST * C::BLOCK;
-  const unsigned ring_s = s_base + C::RING + warp * ST * C::BLOCK, bars = s_base + C::BARS + warp * ST * 8;
+  constexpr int RINGS = C::RINGS, WR = C::WR;
+  const int kw = RS > 1 ? 0 : warp, row0 = RS > 1 ? warp * WR : 0;            // which of the blocks, which of the rows are the warp's
+  unsigned char* ring = smem + C::RING + kw * ST * C::BLOCK;
+  const unsigned ring_s = s_base + C::RING + kw * ST * C::BLOCK, bars = s_base + C::BARS + kw * ST * 16;   // a stage is full, is empty
   RowInfo* s_rows = reinterpret_cast<RowInfo*>(smem + C::ROWS);
   float2* s_rf = reinterpret_cast<float2*>(smem + C::RF);    // r of a row, and what its sums begin with
   float2* s_ml = reinterpret_cast<float2*>(smem + C::ML);
   float* s_merge = reinterpret_cast<float*>(smem + C::MERGE);
-  long long* s_plan = reinterpret_cast<long long*>(smem + C::PLAN);
+  int* s_plan = reinterpret_cast<int*>(smem + C::PLAN);
 
-  if (lane < ST) mbar_init1(bars + 8 * lane);
-  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-  // ---- the line of blocks and this CTA's share
-  const long long Z = (long long)a.step.n_ent * rts, zc = (Z + THREADS - 1) / THREADS;
+  // ---- the line of blocks (or of units, where they are not cut) and this CTA's share
+  const int Z = a.step.n_ent * rts, zc = (Z + THREADS - 1) / THREADS;
   Unit u;
+  auto weight = [&]() { return (split ? u.tiles : min(u.tiles, 1)) * v.KH; };
   {
-    long long sum = 0;
-    for (long long z = tid * zc; z < min(Z, (tid + 1) * zc); ++z) {
+    int sum = 0;
+    for (int z = tid * zc; z < min(Z, (tid + 1) * zc); ++z) {
       unit_of<RT>(a, rts, z, u);
-      sum += (long long)u.tiles * v.KH;
+      sum += weight();
     }
-    long long up = sum;
+    if (lane < ST && (RS == 1 || warp == 0)) { mbar_init(bars + 16 * lane, 1); mbar_init(bars + 16 * lane + 8, RS); }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    int up = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long t = __shfl_up_sync(0xffffffffu, up, o);
+      const int t = __shfl_up_sync(0xffffffffu, up, o);
       if (lane >= o) up += t;
     }
-    long long* s_tot = s_plan + THREADS - WARPS + 1;          // overwritten below
+    int* s_tot = s_plan + THREADS + 1;
     if (lane == 31) s_tot[warp] = up;
     __syncthreads();
-    for (int w = 0; w < warp; ++w) up += s_tot[w];
-    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < WARPS - 1; ++w) up += w < warp ? s_tot[w] : 0;
     s_plan[tid + 1] = up;
     if (tid == 0) s_plan[0] = 0;
     __syncthreads();
   }
-  const long long W = s_plan[THREADS];
-  const long long share = max((W + gridDim.x - 1) / gridDim.x, (long long)MIN_SHARE);
-  long long at = blockIdx.x * share;
-  const long long end = min(W, at + share);
+  const int W = s_plan[THREADS];
+  const int share = max((W + (int)gridDim.x - 1) / (int)gridDim.x, split ? MIN_SHARE : 1);
+  int at = (int)min((long long)blockIdx.x * share, (long long)W);
+  const int end = (int)min((long long)at + share, (long long)W);
+  if (tid == 0) a.cuts[blockIdx.x].n = 0;                    // no unit of this CTA goes on in the next, until one does
   if (at >= end) return;
-  long long z;
-  int head, tile;                                            // where the share begins
+  int z, head, tile;                                         // where the share begins
   {
     int j = 0;
 #pragma unroll
     for (int o = THREADS / 2; o > 0; o >>= 1)
       if (s_plan[j + o] <= at) j += o;
     z = j * zc;
-    long long rem = at - s_plan[j];
+    int rem = at - s_plan[j];
     for (;; ++z) {
       unit_of<RT>(a, rts, z, u);
-      const long long n = (long long)u.tiles * v.KH;
+      const int n = weight();
       if (rem < n) break;
       rem -= n;
     }
-    head = (int)(rem / u.tiles);
-    tile = (int)(rem % u.tiles);
+    head = split ? rem / u.tiles : rem;
+    tile = split ? rem - head * u.tiles : 0;
   }
 
   unsigned it = 0, put = 0;                                  // blocks taken and asked for
@@ -208,80 +218,109 @@ __global__ void __launch_bounds__(THREADS, (AttnCfg<T, P, NT>::CTAS)) qkv_attn_k
   int page_cur = -1, page_nxt = -1;                          // pages of the warp's next 32 and 64 blocks of a segment
   int seg_a = 0, seg_b = 0;
   auto pages_of = [&](int k0) {
-    const int i = seg_a + warp + WARPS * (k0 + lane);
+    const int i = seg_a + kw + RINGS * (k0 + lane);
     return i < seg_b ? v.page(u.slot, i * QKV_BLOCK / KV_PAGE) : -1;
   };
+  auto came = [&](unsigned bar, unsigned parity) {           // bounded wait
+    if (!mbar_try1(bar, parity) && !mbar_wait_long(bar, parity, dead ? 1000000ull : WAIT_CYCLES)) dead = true;
+  };
   auto ask = [&](int k, int page) {                          // block k of the warp's in this segment
+    if (RS > 1 && warp) return;
     if (lane == 0) {
-      const unsigned s = put % ST, bar = bars + 8 * s;
-      const int i = seg_a + warp + WARPS * k;
+      const unsigned s = put % ST, bar = bars + 16 * s;
+      const int i = seg_a + kw + RINGS * k;
+      if (RS > 1 && put >= ST) came(bar + 8, (put / ST - 1) & 1);
       if (page >= 0 && !dead) fetch_block(ring_s + s * C::BLOCK, v.block(page, head, i & 1), C::BLOCK, bar);
-      else asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
+      else mbar_arrive1(bar);
     }
     ++put;
   };
+  constexpr int AHEAD = RS > 1 ? ST - 1 : ST;                // blocks asked for before their turn; shared ones leave a stage to the slowest warp
   auto begin_segment = [&]() {
     seg_a = u.tile0 + tile;
-    seg_b = (int)min((long long)(u.tile0 + u.tiles), seg_a + (end - at));
+    seg_b = split ? min(u.tile0 + u.tiles, seg_a + (end - at)) : u.tile0 + u.tiles;
     page_cur = pages_of(0);
     page_nxt = pages_of(32);
 #pragma unroll
-    for (int k = 0; k < ST; ++k)
-      if (seg_a + warp + WARPS * k < seg_b) ask(k, __shfl_sync(0xffffffffu, page_cur, k));
+    for (int k = 0; k < AHEAD; ++k)
+      if (seg_a + kw + RINGS * k < seg_b) ask(k, __shfl_sync(0xffffffffu, page_cur, k));
   };
-  auto stage_queries = [&]() {
-    for (int r = warp; r < RT; r += WARPS) {
-      const int f = u.f0 + r, t = f / G;
-      const bool ok = f < u.nf;
-      const T* q = reinterpret_cast<const T*>(a.q) + ((long long)(u.r0 + (ok ? t : 0)) * v.H + head * G + (ok ? f % G : 0)) * v.d;
-      float4 x[P > 128 ? 2 : 1];
-      unsigned top = 0;
+  auto stage_queries = [&]() {                               // a warp brings a quarter of the rows, up to 16 asked for at a time
+    constexpr int Y = P > 128 ? 2 : 1, PER = RT / WARPS, BATCH = PER < 16 / Y ? PER : 16 / Y;
+#pragma unroll 1
+    for (int rb = 0; rb < PER; rb += BATCH) {
+      float4 x[BATCH][Y];
 #pragma unroll
-      for (int y = 0; y < (P > 128 ? 2 : 1); ++y) {
-        const int c = 4 * lane + 128 * y;
-        x[y] = ok && c < v.d ? load4(q + c) : make_float4(0.f, 0.f, 0.f, 0.f);
-        top = max(top, max(max(__float_as_uint(x[y].x) & 0x7fffffffu, __float_as_uint(x[y].y) & 0x7fffffffu),
-                           max(__float_as_uint(x[y].z) & 0x7fffffffu, __float_as_uint(x[y].w) & 0x7fffffffu)));
-      }
-      top = __reduce_max_sync(0xffffffffu, top);
-      const int e = top >= 0x7f800000u ? 140 : min(max((int)(top >> 23), 27), 254);      // a row that is not finite is left as it is
-      const float up = pow2(267 - e);
-      float sum = 0.f;
+      for (int b = 0; b < BATCH; ++b) {
+        const int f = u.f0 + warp * PER + rb + b, t = f / G;
+        const bool ok = f < u.nf;
+        const T* q = reinterpret_cast<const T*>(a.q) + ((long long)(u.r0 + (ok ? t : 0)) * v.H + head * G + (ok ? f - t * G : 0)) * v.d;
 #pragma unroll
-      for (int y = 0; y < (P > 128 ? 2 : 1); ++y) {
-        const int c = 4 * lane + 128 * y;
-        if (c >= P) break;
-        const float4 w = scaled(x[y], up);
-        uint2 h = make_uint2(pack_f16(w.x, w.y), pack_f16(w.z, w.w));
-        unsigned char* to = smem + C::Q + r * C::QP + 2 * c;
-        *reinterpret_cast<uint2*>(to) = h;
-        if (BIAS) {
-          const float2 p0 = unpack_f16(h.x), p1 = unpack_f16(h.y);
-          sum += (p0.x + p0.y) + (p1.x + p1.y);
-        }
-        if (NQ == 2) {
-          const float2 p0 = unpack_f16(h.x), p1 = unpack_f16(h.y);
-          *reinterpret_cast<uint2*>(to + RT * C::QP) = make_uint2(pack_f16(w.x - p0.x, w.y - p0.y), pack_f16(w.z - p1.x, w.w - p1.y));
+        for (int y = 0; y < Y; ++y) {
+          const int c = 4 * lane + 128 * y;
+          x[b][y] = ok && c < v.d ? load4(q + c) : make_float4(0.f, 0.f, 0.f, 0.f);
         }
       }
-      if (BIAS) sum = warp_sum(sum);
-      if (lane == 0) {
-        s_rf[r] = make_float2(fmaxf(a.scale * 1.4426950408889634f * pow2(e - 13), 1.17549435e-38f), -1152.f * sum);
-        RowInfo info = {-1, 0, 0};
-        if (ok) {
-          info.t = t;
-          info.away = a.tree.away(u.r0 + t, t);
-          if (a.tree.seen) info.seen = a.tree.seen[a.tree.per_row ? u.r0 + t : t];
-        }
-        s_rows[r] = info;
+      // each reduction for all rows before the next step: a shuffle waits for nothing but the one before it in its own row
+      unsigned top[BATCH];
+      float up[BATCH], sum[BATCH];
+#pragma unroll
+      for (int b = 0; b < BATCH; ++b) {
+        top[b] = 0;
+#pragma unroll
+        for (int y = 0; y < Y; ++y)
+          top[b] = max(top[b], max(max(__float_as_uint(x[b][y].x) & 0x7fffffffu, __float_as_uint(x[b][y].y) & 0x7fffffffu),
+                                   max(__float_as_uint(x[b][y].z) & 0x7fffffffu, __float_as_uint(x[b][y].w) & 0x7fffffffu)));
       }
+#pragma unroll
+      for (int b = 0; b < BATCH; ++b) top[b] = __reduce_max_sync(0xffffffffu, top[b]);
+#pragma unroll
+      for (int b = 0; b < BATCH; ++b) {
+        top[b] = top[b] >= 0x7f800000u ? 140 : min(max(top[b] >> 23, 27u), 254u);      // a row that is not finite is left as it is
+        up[b] = pow2(267 - (int)top[b]);
+        sum[b] = 0.f;
+#pragma unroll
+        for (int y = 0; y < Y; ++y) {
+          const int c = 4 * lane + 128 * y;
+          if (c >= P) break;
+          const float4 w = scaled(x[b][y], up[b]);
+          const uint2 h = make_uint2(pack_f16(w.x, w.y), pack_f16(w.z, w.w));
+          unsigned char* to = smem + C::Q + (warp * PER + rb + b) * C::QP + 2 * c;
+          *reinterpret_cast<uint2*>(to) = h;
+          const float2 p0 = unpack_f16(h.x), p1 = unpack_f16(h.y);
+          if (BIAS) sum[b] += (p0.x + p0.y) + (p1.x + p1.y);
+          if (NQ == 2) *reinterpret_cast<uint2*>(to + RT * C::QP) = make_uint2(pack_f16(w.x - p0.x, w.y - p0.y), pack_f16(w.z - p1.x, w.w - p1.y));
+        }
+      }
+      if (BIAS)
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1)
+#pragma unroll
+          for (int b = 0; b < BATCH; ++b) sum[b] += __shfl_xor_sync(0xffffffffu, sum[b], o);
+      if (lane == 0)
+#pragma unroll
+        for (int b = 0; b < BATCH; ++b)
+          s_rf[warp * PER + rb + b] = make_float2(fmaxf(a.scale * 1.4426950408889634f * pow2((int)top[b] - 13), 1.17549435e-38f), -1152.f * sum[b]);
+    }
+  };
+  auto describe_rows = [&]() {
+    if (tid < RT) {
+      RowInfo info = {-1, 0, 0};
+      const int f = u.f0 + tid, t = f / G;
+      if (f < u.nf) {
+        info.t = t;
+        info.away = a.tree.away(u.r0 + t, t);
+        if (a.tree.seen) info.seen = a.tree.seen[a.tree.per_row ? u.r0 + t : t];
+      }
+      s_rows[tid] = info;
     }
   };
 
   begin_segment();
-  stage_queries();
-  __syncthreads();
   while (true) {
+    describe_rows();
+    stage_queries();
+    __syncthreads();
     // ---- the warp's blocks of this segment.  A thread's rows are 8 nt + 2 rc + x (x = 0, 1), its positions 8 j + rg of a block
     float acc[CH][NT][4], m_run[NT][2], l_run[NT][2], rf[NT][2], first[NT][2];
     unsigned qf[C::QREG ? CH : 1][NT * NQ][2];
@@ -295,13 +334,13 @@ __global__ void __launch_bounds__(THREADS, (AttnCfg<T, P, NT>::CTAS)) qkv_attn_k
       for (int x = 0; x < 2; ++x) {
         m_run[nt][x] = -CUDART_INF_F;
         l_run[nt][x] = 0.f;
-        const float2 r = s_rf[8 * nt + 2 * rc + x];
+        const float2 r = s_rf[row0 + 8 * nt + 2 * rc + x];
         rf[nt][x] = r.x;
         first[nt][x] = r.y;
       }
     }
     auto query = [&](int nt, int half, int k, unsigned (&q)[2]) {
-      const uint2 x = *reinterpret_cast<const uint2*>(smem + C::Q + half * RT * C::QP + (8 * nt + rg) * C::QP + 32 * k + 8 * rc);
+      const uint2 x = *reinterpret_cast<const uint2*>(smem + C::Q + half * RT * C::QP + (row0 + 8 * nt + rg) * C::QP + 32 * k + 8 * rc);
       q[0] = x.x; q[1] = x.y;
     };
     if (C::QREG)
@@ -310,11 +349,11 @@ __global__ void __launch_bounds__(THREADS, (AttnCfg<T, P, NT>::CTAS)) qkv_attn_k
 #pragma unroll
         for (int j = 0; j < NT * NQ; ++j) query(j / NQ, j % NQ, k, qf[C::QREG ? k : 0][j]);
     int R = 16;                                              // biased exponent of the largest scale of values met
-    for (int k = 0, i = seg_a + warp; i < seg_b; ++k, i += WARPS, ++it) {
+    for (int k = 0, i = seg_a + kw; i < seg_b; ++k, i += RINGS, ++it) {
       if ((k & 31) == 0 && k) { page_cur = page_nxt; page_nxt = pages_of(k + 32); }
       const int page = __shfl_sync(0xffffffffu, page_cur, k & 31);
       const unsigned s = it % ST;
-      if (!mbar_try1(bars + 8 * s, (it / ST) & 1) && !mbar_wait_long(bars + 8 * s, (it / ST) & 1, dead ? 1000000ull : WAIT_CYCLES)) dead = true;
+      came(bars + 16 * s, (it / ST) & 1);
       dead = __any_sync(0xffffffffu, dead);
       const unsigned char* blk = ring + s * C::BLOCK;
       if (page < 0 || dead) {
@@ -379,7 +418,7 @@ __global__ void __launch_bounds__(THREADS, (AttnCfg<T, P, NT>::CTAS)) qkv_attn_k
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-              const RowInfo row = s_rows[8 * nt + 2 * rc + x];
+              const RowInfo row = s_rows[row0 + 8 * nt + 2 * rc + x];
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
                 const int key = k0 + 8 * j + rg, n = key - u.len;
@@ -393,33 +432,45 @@ __global__ void __launch_bounds__(THREADS, (AttnCfg<T, P, NT>::CTAS)) qkv_attn_k
         }
         // ---- weights
         unsigned pb[NT][NQ][4];                              // of positions 8 j + 2 rc, + 1 and row 8 nt + rg
+        float base[NT][2], f[NT][2];
+        bool grew = false;
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float f[2], base[2];
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int x = 0; x < 2; ++x) base[nt][x] = fmaxf(fmaxf(t[0][nt][x], t[0][nt][2 + x]), fmaxf(t[1][nt][x], t[1][nt][2 + x]));
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) base[nt][x] = fmaxf(base[nt][x], __shfl_xor_sync(0xffffffffu, base[nt][x], o));
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            float mx = fmaxf(fmaxf(t[0][nt][x], t[0][nt][2 + x]), fmaxf(t[1][nt][x], t[1][nt][2 + x]));
-#pragma unroll
-            for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-            const float m = fmaxf(m_run[nt][x], mx * rf[nt][x]);
-            base[x] = m == -CUDART_INF_F ? 0.f : m;          // nothing seen yet: every weight becomes exp2(-inf) = 0
-            f[x] = ex2(m_run[nt][x] - base[x]);
+            const float m = fmaxf(m_run[nt][x], base[nt][x] * rf[nt][x]);
+            base[nt][x] = m == -CUDART_INF_F ? 0.f : m;      // nothing seen yet: every weight becomes exp2(-inf) = 0
+            f[nt][x] = ex2(m_run[nt][x] - base[nt][x]);
             m_run[nt][x] = m;
+            grew |= f[nt][x] != 1.f;
           }
-          if (__any_sync(0xffffffffu, f[0] != 1.f || f[1] != 1.f)) {
+        if (__any_sync(0xffffffffu, grew))
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-              l_run[nt][x] *= f[x];
+              l_run[nt][x] *= f[nt][x];
 #pragma unroll
-              for (int c = 0; c < CH; ++c) { acc[c][nt][x] *= f[x]; acc[c][nt][2 + x] *= f[x]; }
+              for (int c = 0; c < CH; ++c) { acc[c][nt][x] *= f[nt][x]; acc[c][nt][2 + x] *= f[nt][x]; }
             }
-          }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             float w[2];
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-              const float s1 = t[j >> 1][nt][2 * (j & 1) + x], p = ex2(fmaf(s1, rf[nt][x], -base[x]));
+              const float s1 = t[j >> 1][nt][2 * (j & 1) + x], p = ex2(fmaf(s1, rf[nt][x], -base[nt][x]));
               l_run[nt][x] += p;                             // this lane's share; the eight lanes of a row are summed at the end
               w[x] = p * vs[j];
               if (!full && s1 == -CUDART_INF_F) w[x] = 0.f;  // what a row does not see may have any scale, NaN too
@@ -431,7 +482,6 @@ __global__ void __launch_bounds__(THREADS, (AttnCfg<T, P, NT>::CTAS)) qkv_attn_k
               pb[nt][NQ - 1][j] = transposed(pack_f16(w[0] - g.x, w[1] - g.y));
             }
           }
-        }
         // ---- values: register j of a transposed read holds channels 2 rg, 2 rg + 1 of positions 8 j + 2 rc, + 1; row m of the
         // product is channel 2 m (m < 8) or 2 (m - 8) + 1
 #pragma unroll
@@ -449,18 +499,18 @@ __global__ void __launch_bounds__(THREADS, (AttnCfg<T, P, NT>::CTAS)) qkv_attn_k
         }
       }
       __syncwarp();                                          // all lanes are done with the stage
-      if (i + WARPS * ST < seg_b) {
-        const int kn = k + ST;
+      if (RS > 1 && lane == 0) mbar_arrive1(bars + 16 * s + 8);
+      if (i + RINGS * AHEAD < seg_b) {
+        const int kn = k + AHEAD;
         ask(kn, __shfl_sync(0xffffffffu, (kn >> 5) == (k >> 5) ? page_cur : page_nxt, kn & 31));
       }
     }
     // ---- the next segment's first blocks are on their way while this one is merged
     const Unit du = u;
-    const int d_head = head;
-    const long long u_begin = at - tile, seg_n = seg_b - seg_a;
-    const bool whole = seg_n == du.tiles;
-    const int cta0 = (int)(u_begin / share), cta1 = (int)((u_begin + du.tiles - 1) / share);
-    at += seg_n;
+    const int d_head = head, done = split ? seg_b - seg_a : 1, u_begin = at - tile;
+    const bool whole = !split || done == du.tiles, goes_on = !whole && u_begin + du.tiles > end;
+    const bool begun = !whole && tile == 0;                  // this CTA has the unit's first part
+    at += done;
     const bool more = at < end;
     if (more) {
       tile = 0;
@@ -470,40 +520,67 @@ __global__ void __launch_bounds__(THREADS, (AttnCfg<T, P, NT>::CTAS)) qkv_attn_k
       }
       begin_segment();
     }
-    // ---- the four warps' results of a row
     const float r_inv = pow2(R - 14);
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+    for (int o = 4; o < 32; o <<= 1)
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        float l = l_run[nt][x];
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-        if (rg == 0) s_ml[warp * RT + 8 * nt + 2 * rc + x] = make_float2(m_run[nt][x], l);
-      }
-    __syncthreads();
+        for (int x = 0; x < 2; ++x) l_run[nt][x] += __shfl_xor_sync(0xffffffffu, l_run[nt][x], o);
+    const int part = 2 * (int)blockIdx.x + (begun ? 1 : 0);
+    if constexpr (RS > 1) {
+      // ---- a warp's rows are its own: straight to memory, 32 bytes of a row (bf16) at a time
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int r = 8 * nt + 2 * rc + x;
-        float m = -CUDART_INF_F;
+        for (int x = 0; x < 2; ++x) {
+          const float l = l_run[nt][x];
+          const int r = row0 + 8 * nt + 2 * rc + x, f = du.f0 + r;
+          if (f >= du.nf) continue;
+          const float inv = whole ? (l == 0.f ? 0.f : r_inv / l) : r_inv;    // nothing seen: zero
+          T* out = reinterpret_cast<T*>(a.out) + ((long long)(du.r0 + f / G) * v.H + d_head * G + f % G) * v.d + 2 * rg;
+          float* part_o = a.part_o + ((long long)part * RT + r) * P + 2 * rg;
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) m = fmaxf(m, s_ml[w * RT + r].x);
-        const float f = m_run[nt][x] == -CUDART_INF_F ? 0.f : ex2(m_run[nt][x] - m) * r_inv;
+          for (int c = 0; c < CH; ++c) {
+            const float2 y = make_float2(acc[c][nt][x] * inv, acc[c][nt][2 + x] * inv);
+            if (!whole) *reinterpret_cast<float2*>(part_o + 16 * c) = y;
+            else if (16 * c + 2 * rg < v.d) {
+              if constexpr (sizeof(T) == 4) *reinterpret_cast<float2*>(out + 16 * c) = y;
+              else *reinterpret_cast<__nv_bfloat162*>(out + 16 * c) = __floats2bfloat162_rn(y.x, y.y);
+            }
+          }
+          if (!whole && rg == 0) a.part_ml[part * RT + r] = make_float2(m_run[nt][x], l);
+        }
+      __syncthreads();
+    } else {
+      // ---- the four warps' results of a row
 #pragma unroll
-        for (int c = 0; c < CH; ++c) { acc[c][nt][x] *= f; acc[c][nt][2 + x] *= f; }
-      }
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int x = 0; x < 2; ++x)
+          if (rg == 0) s_ml[warp * RT + 8 * nt + 2 * rc + x] = make_float2(m_run[nt][x], l_run[nt][x]);
+      __syncthreads();
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+          const int r = 8 * nt + 2 * rc + x;
+          float m = -CUDART_INF_F;
+#pragma unroll
+          for (int w = 0; w < WARPS; ++w) m = fmaxf(m, s_ml[w * RT + r].x);
+          const float f = m_run[nt][x] == -CUDART_INF_F ? 0.f : ex2(m_run[nt][x] - m) * r_inv;
+#pragma unroll
+          for (int c = 0; c < CH; ++c) { acc[c][nt][x] *= f; acc[c][nt][2 + x] *= f; }
+        }
     constexpr int SUB = C::SUB, MP = C::MP;
     const int o_sub = tid / (RT * 4), o_row = tid / 4 % RT, o_c = 4 * (tid % 4), f = du.f0 + o_row;
-    const int part = 2 * (int)blockIdx.x + ((int)blockIdx.x == cta0 ? 1 : 0);
     float m_all = -CUDART_INF_F, l_all = 0.f;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) m_all = fmaxf(m_all, s_ml[w * RT + o_row].x);
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) {
       const float2 x = s_ml[w * RT + o_row];
-      if (x.x != -CUDART_INF_F) l_all += x.y * ex2(x.x - m_all);
+      l_all += x.y * (x.x == -CUDART_INF_F ? 0.f : ex2(x.x - m_all));       // a sum that is not a number stays one
     }
     const float inv = l_all == 0.f ? 0.f : 1.f / l_all;      // nothing seen: zero
     T* out = reinterpret_cast<T*>(a.out) + ((long long)(du.r0 + f / G) * v.H + d_head * G + f % G) * v.d;
@@ -534,50 +611,71 @@ __global__ void __launch_bounds__(THREADS, (AttnCfg<T, P, NT>::CTAS)) qkv_attn_k
       }
       __syncthreads();
     }
-    // ---- a unit of several CTAs
-    if (!whole) {
-      if (f < du.nf && tid % 4 == 0 && o_sub == 0) a.part_ml[part * RT + o_row] = make_float2(m_all, l_all);
-      __shared__ int s_last;
-      __threadfence();
-      __syncthreads();
-      if (tid == 0) {
-        s_last = atomicAdd(&a.tickets[cta0], 1) == cta1 - cta0;
-        if (s_last) a.tickets[cta0] = 0;
-      }
-      __syncthreads();
-      if (s_last) {
-        __threadfence();
-        const int n = cta1 - cta0 + 1, rows = min(RT, du.nf - du.f0);
-        auto slot_of = [&](int j) { return 2 * (cta0 + j) + (j == 0 ? 1 : 0); };
-        for (int x = tid; x < rows * (P / 4); x += THREADS) {
-          const int r = x / (P / 4), c = x % (P / 4) * 4, ff = du.f0 + r;
-          float m = -CUDART_INF_F, l = 0.f;
-          for (int j = 0; j < n; ++j) m = fmaxf(m, __ldcg(&a.part_ml[slot_of(j) * RT + r]).x);
-          float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-          for (int j = 0; j < n; ++j) {
-            const float2 ml = __ldcg(&a.part_ml[slot_of(j) * RT + r]);
-            const float4 y = __ldcg(reinterpret_cast<const float4*>(a.part_o + ((long long)slot_of(j) * RT + r) * P + c));
-            const float w = ml.x == -CUDART_INF_F ? 0.f : ex2(ml.x - m);
-            l = fmaf(ml.y, w, l);
-            o = make_float4(fmaf(y.x, w, o.x), fmaf(y.y, w, o.y), fmaf(y.z, w, o.z), fmaf(y.w, w, o.w));
-          }
-          if (c < v.d)
-            store4(reinterpret_cast<T*>(a.out) + ((long long)(du.r0 + ff / G) * v.H + d_head * G + ff % G) * v.d + c, scaled(o, l == 0.f ? 0.f : 1.f / l));
-        }
-      }
+    if (!whole && f < du.nf && tid % 4 == 0 && o_sub == 0) a.part_ml[part * RT + o_row] = make_float2(m_all, l_all);
     }
+    if (begun && goes_on && tid == 0)                        // the CTAs that have its blocks: this one and the next ones
+      a.cuts[blockIdx.x] = {du.r0, du.f0, du.nf, d_head, (u_begin + du.tiles - 1) / share - (int)blockIdx.x + 1};
     if (!more) break;
-    stage_queries();
-    __syncthreads();
   }
 }
 
-template <typename T, int SCHEME, int P, int NT>
+// Parts of the units that were cut, in the order of their CTAs: a warp per row.  grid (CTAs of the attention, row groups), block 128
+template <typename T, int P>
+__global__ void __launch_bounds__(THREADS) qkv_merge_kernel(QkvAttnArgs a, int RT) {
+  constexpr int Y = P > 128 ? 2 : 1, IN = Y > 1 ? 8 : 16;    // parts asked for at a time
+  pdl_wait();
+  const QkvCut o = a.cuts[blockIdx.x];
+  const int lane = threadIdx.x & 31, rows = min(RT, o.nf - o.f0), G = a.v.H / a.v.KH;
+  for (int r = blockIdx.y * WARPS + (threadIdx.x >> 5); o.n > 0 && r < rows; r += gridDim.y * WARPS) {
+    auto at = [&](int j) { return (long long)(2 * (blockIdx.x + j) + (j == 0 ? 1 : 0)) * RT + r; };
+    float m = -CUDART_INF_F, l = 0.f;
+    for (int j = lane; j < o.n; j += 32) m = fmaxf(m, a.part_ml[at(j)].x);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+    float4 sum[Y];
+#pragma unroll
+    for (int y = 0; y < Y; ++y) sum[y] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int j0 = 0; j0 < o.n; j0 += 32) {
+      float w = 0.f;
+      if (j0 + lane < o.n) {
+        const float2 ml = a.part_ml[at(j0 + lane)];
+        // nothing seen: no weight; a sum without a maximum is no number
+        w = ml.x == -CUDART_INF_F ? (ml.y == 0.f ? 0.f : CUDART_NAN_F) : ex2(ml.x - m);
+        l += ml.y * w;
+      }
+#pragma unroll 1
+      for (int j1 = 0; j1 < 32 && j0 + j1 < o.n; j1 += IN) {
+        float4 x[IN][Y];
+#pragma unroll
+        for (int j = 0; j < IN; ++j)
+#pragma unroll
+          for (int y = 0; y < Y; ++y) {
+            const int c = 4 * lane + 128 * y;
+            x[j][y] = c < P ? *reinterpret_cast<const float4*>(a.part_o + at(min(j0 + j1 + j, o.n - 1)) * P + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+          }
+#pragma unroll
+        for (int j = 0; j < IN; ++j) {
+          const float f = __shfl_sync(0xffffffffu, w, j1 + j);
+#pragma unroll
+          for (int y = 0; y < Y; ++y)
+            sum[y] = make_float4(fmaf(x[j][y].x, f, sum[y].x), fmaf(x[j][y].y, f, sum[y].y), fmaf(x[j][y].z, f, sum[y].z), fmaf(x[j][y].w, f, sum[y].w));
+        }
+      }
+    }
+    l = warp_sum(l);
+    const int f = o.f0 + r;
+    T* out = reinterpret_cast<T*>(a.out) + ((long long)(o.r0 + f / G) * a.v.H + o.head * G + f % G) * a.v.d;
+#pragma unroll
+    for (int y = 0; y < Y; ++y)
+      if (4 * lane + 128 * y < a.v.d) store4(out + 4 * lane + 128 * y, scaled(sum[y], l == 0.f ? 0.f : 1.f / l));
+  }
+}
+
+template <typename T, int SCHEME, int P, int NT, int RS>
 int32_t launch(vn_qkv* c, const QkvAttnArgs& a) {
-  using C = AttnCfg<T, P, NT>;
+  using C = AttnCfg<T, P, NT, RS>;
   vn_ctx* ctx = c->ctx;
-  auto kernel = qkv_attn_kernel<T, SCHEME, P, NT>;
+  auto kernel = qkv_attn_kernel<T, SCHEME, P, NT, RS>;
   static int per_sm[64] = {};
   int& occ = per_sm[ctx->device & 63];
   if (!occ) {
@@ -585,24 +683,27 @@ int32_t launch(vn_qkv* c, const QkvAttnArgs& a) {
     int n = 0;
     VN_CUDA(ctx, cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, THREADS, C::SMEM));
     VN_REQUIRE(ctx, n > 0, "qkv_attn_kernel does not fit an SM");
-    occ = min(n, QKV_MAX_CTAS);
+    occ = min(n, C::CTAS);
   }
   const long long rts = ceil_div((long long)a.step.T * (a.v.H / a.v.KH), (long long)C::RT);
-  VN_REQUIRE(ctx, rts < (1ll << 31), "too many rows");
-  // no more CTAs than there can be shares of blocks
-  const double most = (double)a.step.n_ent * (double)rts * a.v.KH * (a.v.capacity() / QKV_BLOCK) / MIN_SHARE + 1;
-  const unsigned grid = (unsigned)min((double)occ * ctx->sm_count, most);
-  VN_LAUNCH_NAMED(ctx, "qkv_attn_kernel", kernel, grid, THREADS, C::SMEM, a, (int)rts);
+  const long long blocks = rts * a.step.n_ent * a.v.KH, tiles = a.v.capacity() / QKV_BLOCK;
+  VN_REQUIRE(ctx, rts < (1ll << 31) && blocks < (1ll << 31) / tiles - THREADS, "%d rows over %d positions are too many for one call: bring them in portions", a.step.M, a.v.capacity());
+  // units of a few blocks stay whole: cutting them saves less than the merge costs
+  const bool split = tiles > UNCUT;
+  // no more CTAs than there can be shares
+  const unsigned grid = (unsigned)min((long long)occ * ctx->sm_count, split ? ceil_div(blocks * tiles, (long long)MIN_SHARE) : blocks);
+  VN_LAUNCH_NAMED(ctx, "qkv_attn_kernel", kernel, grid, THREADS, C::SMEM, a, (int)rts, split);
+  if (split) VN_LAUNCH_PDL_LEVEL(ctx, 1, "qkv_merge_kernel", (qkv_merge_kernel<T, P>), dim3(grid, min(C::RT / WARPS, 16)), THREADS, 0, a, C::RT);
   return VN_OK;
 }
 
 template <int SCHEME>
 int32_t pick(vn_qkv* c, const QkvAttnArgs& a) {
-  // as few columns as hold the rows of an entry; 32 share the conversions of a block where there are more than 16
+  // as few columns as hold the rows of an entry; from 17 rows on the warps split the rows
   const long long rows = (long long)a.step.T * (a.v.H / a.v.KH);
-#define GO(P, NT) return c->dtype == VN_F32 ? launch<float, SCHEME, P, NT>(c, a) : launch<bf16, SCHEME, P, NT>(c, a)
-#define GO2(P) do { if (rows <= 8) GO(P, 1); else GO(P, 2); } while (0)
-#define GO4(P) do { if (rows <= 8) GO(P, 1); else if (rows <= 16) GO(P, 2); else GO(P, 4); } while (0)
+#define GO(P, NT, RS) return c->dtype == VN_F32 ? launch<float, SCHEME, P, NT, RS>(c, a) : launch<bf16, SCHEME, P, NT, RS>(c, a)
+#define GO2(P) do { if (rows <= 8) GO(P, 1, 1); else if (rows <= 16) GO(P, 2, 1); else GO(P, 2, 4); } while (0)
+#define GO4(P) do { if (rows <= 8) GO(P, 1, 1); else if (rows <= 16) GO(P, 2, 1); else if (rows <= 64) GO(P, 2, 4); else GO(P, 4, 4); } while (0)
   switch (a.v.P) {
     case 32: GO4(32);
     case 64: GO4(64);
