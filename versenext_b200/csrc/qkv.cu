@@ -195,13 +195,15 @@ __global__ void set_lengths_kernel(int* __restrict__ lens, const int* __restrict
   if (i < n) lens[i] = from[i];
 }
 
-// layout of vn_ctx::qkv_parts: two parts for every CTA that the attention kernel may have
-struct Parts { size_t ml, cuts, bytes; };
+// layout of vn_ctx::qkv_parts: two parts for every share (CTA, or warp with a quarter of the rows) that the attention kernel may have
+struct Parts { size_t ml, cuts, n_cuts, bytes; int max_cuts; };
 Parts parts_of(const vn_ctx* ctx) {
   Parts p;
   p.ml = (size_t)2 * ctx->sm_count * QKV_PART * sizeof(float);
   p.cuts = p.ml + (size_t)2 * ctx->sm_count * QKV_MAX_CTAS * 128 * sizeof(float2);
-  p.bytes = p.cuts + (size_t)ctx->sm_count * QKV_MAX_CTAS * sizeof(QkvCut);
+  p.max_cuts = ctx->sm_count * QKV_MAX_CTAS * 4;
+  p.n_cuts = p.cuts + (size_t)p.max_cuts * sizeof(QkvCut);
+  p.bytes = p.n_cuts + 3 * sizeof(int);
   return p;
 }
 
@@ -415,6 +417,8 @@ int32_t vn_qkv_attention(vn_qkv* c, const void* q, int32_t n_ent, const int32_t*
   a.part_o = (float*)c->ctx->qkv_parts;
   a.part_ml = (float2*)((char*)c->ctx->qkv_parts + p.ml);
   a.cuts = (QkvCut*)((char*)c->ctx->qkv_parts + p.cuts);
+  a.n_cuts = (int*)((char*)c->ctx->qkv_parts + p.n_cuts);
+  a.max_cuts = p.max_cuts;
   return c->v.scheme == QKV_I8 ? qkv_attention_i8(c, a) : qkv_attention_e4m3(c, a);
 }
 

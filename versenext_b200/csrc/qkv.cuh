@@ -87,8 +87,8 @@ struct vn_qkv {
   int* tickets = nullptr;                           // zero between kernels
 };
 
-// a unit whose blocks several CTAs have, by its first CTA: rows f0 .. of nf (tokens x heads of the group) from row r0 on; n parts, 0: none
-struct QkvCut { int r0, f0, nf, head, n; };
+// a unit whose blocks several shares have, the first of them `first`: rows f0 .. of nf (tokens x heads of the group) from row r0 on; n parts
+struct QkvCut { int r0, f0, nf, head, first, n; };
 
 struct QkvAttnArgs {
   QkvView v;
@@ -98,9 +98,11 @@ struct QkvAttnArgs {
   void* out = nullptr;
   int window = 0;
   float scale = 1.f;
-  float* part_o = nullptr;                          // [2 CTAs][rows of a unit][P] results of a CTA's first and last unit
+  float* part_o = nullptr;                          // [2 shares][rows of a unit][P] results of a share's first and last unit
   float2* part_ml = nullptr;
-  QkvCut* cuts = nullptr;                           // [CTAs]
+  QkvCut* cuts = nullptr;                           // [max_cuts] units to merge: with few parts from the front, with many from the back
+  int* n_cuts = nullptr;                            // [3] how many of each, and CTAs that are done with them; zero between calls
+  int max_cuts = 0;
 };
 constexpr int QKV_MAX_CTAS = 3;                     // of the attention kernel on an SM
 constexpr int QKV_PART = 2 * 128 * 128;             // values of parts: CTAs on an SM x rows x padded head size, at most

@@ -7,11 +7,12 @@
 // split into two halves of 11 bits for fp32 rows.  A weight p_j s_j is taken relative to a power of two R above every s_j met so
 // far, times 2^15, so that a half holds weights down to 2^-39 of the largest.
 //
-// What bounds it is the memory of the codes (few rows) or the mma.sync rate and the conversions (many): one warp reads and converts a
-// block of 32 positions for 8 NT rows (tokens x heads of a group), four warps of a CTA take every fourth block.  Positions are the
-// rows of the products and queries their columns (8 at a time): S = K q^T, O = V^T p^T, with p transposed by movmatrix between.  The blocks of
-// all (entry, rows, head) units form one line that is cut into equal shares for the CTAs, whatever the lengths; the parts of a unit that
-// several CTAs have are merged, in their order, by a second kernel that has all SMs for it (one CTA that merged a unit's parts by
+// What bounds it is the memory of the codes (few rows) or the mma.sync rate and the conversions (many).  Positions are the rows of the
+// products and queries their columns (8 at a time): S = K q^T, O = V^T p^T, with p transposed by movmatrix between.  A warp takes
+// blocks of 32 positions for 8 NT rows (tokens x heads of a group) and waits for no other warp.  The blocks of all (entry, rows, head) units
+// form one line that is cut into equal shares, whatever the lengths: a share for every warp (RS = 1), or, with more rows than a warp has,
+// one for every CTA, whose four warps have rows of their own and share the blocks that come in (RS = 4).  The parts of a unit that
+// several shares have are merged, in their order, by a second kernel that has all SMs for it (one CTA that merged a unit's parts by
 // itself took 10 to 15 us for 7 parts of 64 rows or 56 parts of 8).
 #pragma once
 #include "qkv.cuh"
@@ -20,30 +21,23 @@ namespace qkv_detail {
 
 using bf16 = __nv_bfloat16;
 constexpr int WARPS = 4, THREADS = 32 * WARPS;
-constexpr int MIN_SHARE = WARPS;                    // blocks of a CTA at least
+constexpr int MIN_SHARE = 4;                        // blocks of a share at least
+constexpr int MERGE_WARPS = 8, MANY = 16;           // warps of a merging CTA; parts that one of them takes
 constexpr int UNCUT = 8;                            // blocks of a unit that is never cut
 constexpr unsigned long long WAIT_CYCLES = 4000000000ull;   // a copy that has not come after about two seconds never will
 
-// RS = 1: the warps share a unit's rows and split its blocks; RS = 4: they split its rows and share its blocks
 template <typename T, int P, int NT, int RS>
 struct AttnCfg {
   static constexpr int NQ = sizeof(T) == 4 ? 2 : 1;           // halves of a query or weight
   static constexpr int WR = 8 * NT, RT = WR * RS, CH = P / 16, BLOCK = QKV_BLOCK * (2 * P + 8);   // rows of a warp, of a unit
   static constexpr int RINGS = WARPS / RS;
-  static constexpr int QP = 2 * P + ((2 * P) % 64 == 0 ? 32 : 0);   // bytes of a staged query row: four rows' 32-byte pieces in 128 bytes of banks
-  static constexpr int STAGES = RS > 1 ? 4 : P <= 64 ? 4 : P <= 128 && NT >= 2 && NT * NQ <= 2 ? 3 : 2;
-  static constexpr int CTAS = RS > 1 ? (P * NT <= 256 && NT < 4 && NQ == 1 ? 3 : P * NT <= 512 ? 2 : 1) : P > 192 || (P > 128 && NQ * NT > 1) ? 1 : P * NT <= 128 ? 3 : 2;
-  static constexpr bool QREG = NT * NQ <= 2 && NT * NQ * P <= (RS > 1 ? 128 : 256);      // query fragments in registers
-  static constexpr int SUB = RS > 1 ? 0 : NT >= 4 ? 1 : 2;    // chunks of 16 channels that are merged at a time
-  static constexpr int MP = 20;                               // pitch of a merged row: 16 lanes' pairs in different banks
-  static constexpr int RING = 0, Q = RING + RINGS * STAGES * BLOCK, MERGE = Q + NQ * RT * QP,
-                       MERGE_BYTES = SUB * WARPS * RT * MP * 4 > (THREADS + 8) * 4 ? SUB * WARPS * RT * MP * 4 : (THREADS + 8) * 4, ML = MERGE + MERGE_BYTES,
-                       ROWS = ML + (RS > 1 ? 0 : WARPS * RT * 8), RF = ROWS + RT * 16, BARS = RF + RT * 8, SMEM = BARS + RINGS * STAGES * 16,
-                       PLAN = MERGE;                          // read before anything is merged
-  static_assert(CTAS * RT * P <= QKV_PART, "parts fit their place");
+  static constexpr int CTAS = P > 192 ? 1 : NT < 4 && P * NT * NQ <= 256 && P * NT <= 128 ? 3 : P * NT <= 256 && NT < 4 && NQ == 1 && RS > 1 ? 3 : P * NT <= 512 ? 2 : 1;
+  static constexpr bool QREG = NT * NQ <= 2 && NT * NQ * P <= (RS > 1 ? 128 : 256);      // query fragments in registers, else a thread's own in shared memory
+  static constexpr int STAGES = RS > 1 ? 4 : P <= 64 ? 4 : CTAS == 2 && P * NT <= 256 && QREG ? 3 : 2;
+  static constexpr int RING = 0, Q = RING + RINGS * STAGES * BLOCK, BARS = Q + (QREG ? 0 : WARPS * CH * NT * NQ * 256), PLAN = BARS + RINGS * STAGES * 16,
+                       SMEM = PLAN + (THREADS + 8) * 4;
+  static_assert(CTAS * WARPS * WR * P <= QKV_PART, "parts fit their place");
 };
-
-struct RowInfo { int t, away; unsigned long long seen; };    // t < 0: no row
 
 __device__ __forceinline__ void mbar_init(unsigned bar, int count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count)); }
 __device__ __forceinline__ void mbar_arrive1(unsigned bar) { asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
@@ -145,25 +139,24 @@ template <typename T, int SCHEME, int P, int NT, int RS>
 __global__ void __launch_bounds__(THREADS, (AttnCfg<T, P, NT, RS>::CTAS)) qkv_attn_kernel(QkvAttnArgs a, int rts, bool split) {
   pdl_trigger();
   using C = AttnCfg<T, P, NT, RS>;
-  constexpr int RT = C::RT, CH = C::CH, ST = C::STAGES, NQ = C::NQ;
+  constexpr int RT = C::RT, CH = C::CH, ST = C::STAGES, NQ = C::NQ, RINGS = C::RINGS, WR = C::WR;
   constexpr bool BIAS = SCHEME == QKV_I8 && NQ == 1;         // keys 1152 too large: taken off the sums instead, at the cost of some bits of them
   extern __shared__ __align__(128) unsigned char smem[];
   const QkvView& v = a.v;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, rg = lane >> 2, rc = lane & 3;
   const int G = v.H / v.KH;
+  const int ring_no = RS > 1 ? 0 : warp, row0 = RS > 1 ? warp * WR : 0;       // the warp's ring of blocks, its rows in a unit
   const unsigned s_base = (unsigned)__cvta_generic_to_shared(smem);
-  constexpr int RINGS = C::RINGS, WR = C::WR;
-  const int kw = RS > 1 ? 0 : warp, row0 = RS > 1 ? warp * WR : 0;            // which of the blocks, which of the rows are the warp's
-  unsigned char* ring = smem + C::RING + kw * ST * C::BLOCK;
-  const unsigned ring_s = s_base + C::RING + kw * ST * C::BLOCK, bars = s_base + C::BARS + kw * ST * 16;   // a stage is full, is empty
-  RowInfo* s_rows = reinterpret_cast<RowInfo*>(smem + C::ROWS);
-  float2* s_rf = reinterpret_cast<float2*>(smem + C::RF);    // r of a row, and what its sums begin with
-  float2* s_ml = reinterpret_cast<float2*>(smem + C::ML);
-  float* s_merge = reinterpret_cast<float*>(smem + C::MERGE);
+  unsigned char* ring = smem + C::RING + ring_no * ST * C::BLOCK;
+  const unsigned ring_s = s_base + C::RING + ring_no * ST * C::BLOCK, bars = s_base + C::BARS + ring_no * ST * 16;   // a stage is full, is empty
   int* s_plan = reinterpret_cast<int*>(smem + C::PLAN);
+  if (lane < ST && (RS == 1 || warp == 0)) { mbar_init(bars + 16 * lane, 1); mbar_init(bars + 16 * lane + 8, RS); }
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  pdl_wait();
 
-  // ---- the line of blocks (or of units, where they are not cut) and this CTA's share
+  // ---- the line of blocks (or of units, where they are not cut) and the share of this warp or CTA
   const int Z = a.step.n_ent * rts, zc = (Z + THREADS - 1) / THREADS;
+  const int worker = RS > 1 ? blockIdx.x : blockIdx.x * WARPS + warp, workers = RS > 1 ? gridDim.x : gridDim.x * WARPS;
   Unit u;
   auto weight = [&]() { return (split ? u.tiles : min(u.tiles, 1)) * v.KH; };
   {
@@ -172,8 +165,6 @@ __global__ void __launch_bounds__(THREADS, (AttnCfg<T, P, NT, RS>::CTAS)) qkv_at
       unit_of<RT>(a, rts, z, u);
       sum += weight();
     }
-    if (lane < ST && (RS == 1 || warp == 0)) { mbar_init(bars + 16 * lane, 1); mbar_init(bars + 16 * lane + 8, RS); }
-    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     int up = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -190,10 +181,9 @@ __global__ void __launch_bounds__(THREADS, (AttnCfg<T, P, NT, RS>::CTAS)) qkv_at
     __syncthreads();
   }
   const int W = s_plan[THREADS];
-  const int share = max((W + (int)gridDim.x - 1) / (int)gridDim.x, split ? MIN_SHARE : 1);
-  int at = (int)min((long long)blockIdx.x * share, (long long)W);
+  const int share = max((W + workers - 1) / workers, split ? MIN_SHARE : 1);
+  int at = (int)min((long long)worker * share, (long long)W);
   const int end = (int)min((long long)at + share, (long long)W);
-  if (tid == 0) a.cuts[blockIdx.x].n = 0;                    // no unit of this CTA goes on in the next, until one does
   if (at >= end) return;
   int z, head, tile;                                         // where the share begins
   {
@@ -215,22 +205,21 @@ __global__ void __launch_bounds__(THREADS, (AttnCfg<T, P, NT, RS>::CTAS)) qkv_at
 
   unsigned it = 0, put = 0;                                  // blocks taken and asked for
   bool dead = false;                                         // a copy did not come: nothing is computed any more
-  int page_cur = -1, page_nxt = -1;                          // pages of the warp's next 32 and 64 blocks of a segment
+  int page_cur = -1, page_nxt = -1;                          // pages of the next 32 and 64 blocks of a segment
   int seg_a = 0, seg_b = 0;
   auto pages_of = [&](int k0) {
-    const int i = seg_a + kw + RINGS * (k0 + lane);
+    const int i = seg_a + k0 + lane;
     return i < seg_b ? v.page(u.slot, i * QKV_BLOCK / KV_PAGE) : -1;
   };
   auto came = [&](unsigned bar, unsigned parity) {           // bounded wait
     if (!mbar_try1(bar, parity) && !mbar_wait_long(bar, parity, dead ? 1000000ull : WAIT_CYCLES)) dead = true;
   };
-  auto ask = [&](int k, int page) {                          // block k of the warp's in this segment
+  auto ask = [&](int k, int page) {                          // block k of this segment
     if (RS > 1 && warp) return;
     if (lane == 0) {
       const unsigned s = put % ST, bar = bars + 16 * s;
-      const int i = seg_a + kw + RINGS * k;
       if (RS > 1 && put >= ST) came(bar + 8, (put / ST - 1) & 1);
-      if (page >= 0 && !dead) fetch_block(ring_s + s * C::BLOCK, v.block(page, head, i & 1), C::BLOCK, bar);
+      if (page >= 0 && !dead) fetch_block(ring_s + s * C::BLOCK, v.block(page, head, (seg_a + k) & 1), C::BLOCK, bar);
       else mbar_arrive1(bar);
     }
     ++put;
@@ -243,87 +232,63 @@ __global__ void __launch_bounds__(THREADS, (AttnCfg<T, P, NT, RS>::CTAS)) qkv_at
     page_nxt = pages_of(32);
 #pragma unroll
     for (int k = 0; k < AHEAD; ++k)
-      if (seg_a + kw + RINGS * k < seg_b) ask(k, __shfl_sync(0xffffffffu, page_cur, k));
-  };
-  auto stage_queries = [&]() {                               // a warp brings a quarter of the rows, up to 16 asked for at a time
-    constexpr int Y = P > 128 ? 2 : 1, PER = RT / WARPS, BATCH = PER < 16 / Y ? PER : 16 / Y;
-#pragma unroll 1
-    for (int rb = 0; rb < PER; rb += BATCH) {
-      float4 x[BATCH][Y];
-#pragma unroll
-      for (int b = 0; b < BATCH; ++b) {
-        const int f = u.f0 + warp * PER + rb + b, t = f / G;
-        const bool ok = f < u.nf;
-        const T* q = reinterpret_cast<const T*>(a.q) + ((long long)(u.r0 + (ok ? t : 0)) * v.H + head * G + (ok ? f - t * G : 0)) * v.d;
-#pragma unroll
-        for (int y = 0; y < Y; ++y) {
-          const int c = 4 * lane + 128 * y;
-          x[b][y] = ok && c < v.d ? load4(q + c) : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
-      }
-      // each reduction for all rows before the next step: a shuffle waits for nothing but the one before it in its own row
-      unsigned top[BATCH];
-      float up[BATCH], sum[BATCH];
-#pragma unroll
-      for (int b = 0; b < BATCH; ++b) {
-        top[b] = 0;
-#pragma unroll
-        for (int y = 0; y < Y; ++y)
-          top[b] = max(top[b], max(max(__float_as_uint(x[b][y].x) & 0x7fffffffu, __float_as_uint(x[b][y].y) & 0x7fffffffu),
-                                   max(__float_as_uint(x[b][y].z) & 0x7fffffffu, __float_as_uint(x[b][y].w) & 0x7fffffffu)));
-      }
-#pragma unroll
-      for (int b = 0; b < BATCH; ++b) top[b] = __reduce_max_sync(0xffffffffu, top[b]);
-#pragma unroll
-      for (int b = 0; b < BATCH; ++b) {
-        top[b] = top[b] >= 0x7f800000u ? 140 : min(max(top[b] >> 23, 27u), 254u);      // a row that is not finite is left as it is
-        up[b] = pow2(267 - (int)top[b]);
-        sum[b] = 0.f;
-#pragma unroll
-        for (int y = 0; y < Y; ++y) {
-          const int c = 4 * lane + 128 * y;
-          if (c >= P) break;
-          const float4 w = scaled(x[b][y], up[b]);
-          const uint2 h = make_uint2(pack_f16(w.x, w.y), pack_f16(w.z, w.w));
-          unsigned char* to = smem + C::Q + (warp * PER + rb + b) * C::QP + 2 * c;
-          *reinterpret_cast<uint2*>(to) = h;
-          const float2 p0 = unpack_f16(h.x), p1 = unpack_f16(h.y);
-          if (BIAS) sum[b] += (p0.x + p0.y) + (p1.x + p1.y);
-          if (NQ == 2) *reinterpret_cast<uint2*>(to + RT * C::QP) = make_uint2(pack_f16(w.x - p0.x, w.y - p0.y), pack_f16(w.z - p1.x, w.w - p1.y));
-        }
-      }
-      if (BIAS)
-#pragma unroll
-        for (int o = 16; o > 0; o >>= 1)
-#pragma unroll
-          for (int b = 0; b < BATCH; ++b) sum[b] += __shfl_xor_sync(0xffffffffu, sum[b], o);
-      if (lane == 0)
-#pragma unroll
-        for (int b = 0; b < BATCH; ++b)
-          s_rf[warp * PER + rb + b] = make_float2(fmaxf(a.scale * 1.4426950408889634f * pow2((int)top[b] - 13), 1.17549435e-38f), -1152.f * sum[b]);
-    }
-  };
-  auto describe_rows = [&]() {
-    if (tid < RT) {
-      RowInfo info = {-1, 0, 0};
-      const int f = u.f0 + tid, t = f / G;
-      if (f < u.nf) {
-        info.t = t;
-        info.away = a.tree.away(u.r0 + t, t);
-        if (a.tree.seen) info.seen = a.tree.seen[a.tree.per_row ? u.r0 + t : t];
-      }
-      s_rows[tid] = info;
-    }
+      if (seg_a + k < seg_b) ask(k, __shfl_sync(0xffffffffu, page_cur, k));
   };
 
   begin_segment();
   while (true) {
-    describe_rows();
-    stage_queries();
-    __syncthreads();
-    // ---- the warp's blocks of this segment.  A thread's rows are 8 nt + 2 rc + x (x = 0, 1), its positions 8 j + rg of a block
-    float acc[CH][NT][4], m_run[NT][2], l_run[NT][2], rf[NT][2], first[NT][2];
+    // ---- queries: a thread takes channels 16 k + 4 rc .. + 3 of row 8 nt + rg, which is what the product wants of it
+    float rf[NT][2], first[NT][2];                           // of rows 8 nt + 2 rc + x: r, and what their sums begin with
+    int row_t[NT][2];                                        // their tokens, -1: no row
     unsigned qf[C::QREG ? CH : 1][NT * NQ][2];
+    uint2* s_q = reinterpret_cast<uint2*>(smem + C::Q) + warp * CH * NT * NQ * 32 + lane;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int f = u.f0 + row0 + 8 * nt + rg, t = f / G;
+      const bool ok = f < u.nf;
+      const T* q = reinterpret_cast<const T*>(a.q) + ((long long)(u.r0 + (ok ? t : 0)) * v.H + head * G + (ok ? f - t * G : 0)) * v.d + 4 * rc;
+      float4 x[CH];
+#pragma unroll
+      for (int k = 0; k < CH; ++k) x[k] = ok && 16 * k + 4 * rc < v.d ? load4(q + 16 * k) : make_float4(0.f, 0.f, 0.f, 0.f);
+      unsigned top = 0;
+#pragma unroll
+      for (int k = 0; k < CH; ++k)
+        top = max(top, max(max(__float_as_uint(x[k].x) & 0x7fffffffu, __float_as_uint(x[k].y) & 0x7fffffffu),
+                           max(__float_as_uint(x[k].z) & 0x7fffffffu, __float_as_uint(x[k].w) & 0x7fffffffu)));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const int e = top >= 0x7f800000u ? 140 : min(max((int)(top >> 23), 27), 254);      // a row that is not finite is left as it is
+      const float up = pow2(267 - e);
+      float sum = 0.f;
+#pragma unroll
+      for (int k = 0; k < CH; ++k) {
+        const float4 w = scaled(x[k], up);
+        const uint2 h = make_uint2(pack_f16(w.x, w.y), pack_f16(w.z, w.w));
+        const float2 p0 = unpack_f16(h.x), p1 = unpack_f16(h.y);
+        if (BIAS) sum += (p0.x + p0.y) + (p1.x + p1.y);
+        const uint2 lo = NQ == 2 ? make_uint2(pack_f16(w.x - p0.x, w.y - p0.y), pack_f16(w.z - p1.x, w.w - p1.y)) : h;
+        if (C::QREG) {
+          qf[C::QREG ? k : 0][nt * NQ][0] = h.x; qf[C::QREG ? k : 0][nt * NQ][1] = h.y;
+          if (NQ == 2) { qf[C::QREG ? k : 0][nt * NQ + NQ - 1][0] = lo.x; qf[C::QREG ? k : 0][nt * NQ + NQ - 1][1] = lo.y; }
+        } else {
+          s_q[(k * NT * NQ + nt * NQ) * 32] = h;
+          if (NQ == 2) s_q[(k * NT * NQ + nt * NQ + NQ - 1) * 32] = lo;
+        }
+      }
+      if (BIAS) {
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+      }
+      const float r = fmaxf(a.scale * 1.4426950408889634f * pow2(e - 13), 1.17549435e-38f);
+#pragma unroll
+      for (int x2 = 0; x2 < 2; ++x2) {
+        rf[nt][x2] = __shfl_sync(0xffffffffu, r, 4 * (2 * rc + x2));
+        first[nt][x2] = BIAS ? -1152.f * __shfl_sync(0xffffffffu, sum, 4 * (2 * rc + x2)) : 0.f;
+        row_t[nt][x2] = __shfl_sync(0xffffffffu, ok ? t : -1, 4 * (2 * rc + x2));
+      }
+    }
+    // ---- the blocks of this segment.  A thread's rows are 8 nt + 2 rc + x (x = 0, 1), its positions 8 j + rg of a block
+    float acc[CH][NT][4], m_run[NT][2], l_run[NT][2];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -331,25 +296,12 @@ __global__ void __launch_bounds__(THREADS, (AttnCfg<T, P, NT, RS>::CTAS)) qkv_at
 #pragma unroll
         for (int x = 0; x < 4; ++x) acc[k][nt][x] = 0.f;
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        m_run[nt][x] = -CUDART_INF_F;
-        l_run[nt][x] = 0.f;
-        const float2 r = s_rf[row0 + 8 * nt + 2 * rc + x];
-        rf[nt][x] = r.x;
-        first[nt][x] = r.y;
-      }
+      for (int x = 0; x < 2; ++x) { m_run[nt][x] = -CUDART_INF_F; l_run[nt][x] = 0.f; }
     }
-    auto query = [&](int nt, int half, int k, unsigned (&q)[2]) {
-      const uint2 x = *reinterpret_cast<const uint2*>(smem + C::Q + half * RT * C::QP + (row0 + 8 * nt + rg) * C::QP + 32 * k + 8 * rc);
-      q[0] = x.x; q[1] = x.y;
-    };
-    if (C::QREG)
-#pragma unroll
-      for (int k = 0; k < CH; ++k)
-#pragma unroll
-        for (int j = 0; j < NT * NQ; ++j) query(j / NQ, j % NQ, k, qf[C::QREG ? k : 0][j]);
     int R = 16;                                              // biased exponent of the largest scale of values met
-    for (int k = 0, i = seg_a + kw; i < seg_b; ++k, i += RINGS, ++it) {
+#pragma unroll 1
+    for (int i = seg_a; i < seg_b; ++i, ++it) {
+      const int k = i - seg_a;
       if ((k & 31) == 0 && k) { page_cur = page_nxt; page_nxt = pages_of(k + 32); }
       const int page = __shfl_sync(0xffffffffu, page_cur, k & 31);
       const unsigned s = it % ST;
@@ -382,7 +334,7 @@ __global__ void __launch_bounds__(THREADS, (AttnCfg<T, P, NT, RS>::CTAS)) qkv_at
             for (int half = 0; half < NQ; ++half) {
               unsigned q[2];
               if (C::QREG) { q[0] = qf[C::QREG ? kc : 0][nt * NQ + half][0]; q[1] = qf[C::QREG ? kc : 0][nt * NQ + half][1]; }
-              else query(nt, half, kc, q);
+              else { const uint2 y = s_q[(kc * NT * NQ + nt * NQ + half) * 32]; q[0] = y.x; q[1] = y.y; }
               mma_f16(t[0][nt], ka[0], q[0], q[1]);
               mma_f16(t[1][nt], ka[1], q[0], q[1]);
             }
@@ -418,15 +370,16 @@ __global__ void __launch_bounds__(THREADS, (AttnCfg<T, P, NT, RS>::CTAS)) qkv_at
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-              const RowInfo row = s_rows[row0 + 8 * nt + 2 * rc + x];
+              const int tok = row_t[nt][x], away = tok < 0 ? 0 : a.tree.away(u.r0 + tok, tok);
+              const unsigned long long seen = a.tree.seen && tok >= 0 ? a.tree.seen[a.tree.per_row ? u.r0 + tok : tok] : 0;
 #pragma unroll
               for (int j = 0; j < 4; ++j) {
                 const int key = k0 + 8 * j + rg, n = key - u.len;
                 bool see;
-                if (n < 0) see = a.window == 0 || u.len + row.away - key < a.window;
-                else if (a.tree.seen) see = n < u.n && ((row.seen >> n) & 1);
-                else see = n <= row.t && (a.window == 0 || row.t - n < a.window);
-                if (row.t < 0 || !see || key >= u.hi) t[j >> 1][nt][2 * (j & 1) + x] = -CUDART_INF_F;
+                if (n < 0) see = a.window == 0 || u.len + away - key < a.window;
+                else if (a.tree.seen) see = n < u.n && ((seen >> n) & 1);
+                else see = n <= tok && (a.window == 0 || tok - n < a.window);
+                if (tok < 0 || !see || key >= u.hi) t[j >> 1][nt][2 * (j & 1) + x] = -CUDART_INF_F;
               }
             }
         }
@@ -500,16 +453,16 @@ __global__ void __launch_bounds__(THREADS, (AttnCfg<T, P, NT, RS>::CTAS)) qkv_at
       }
       __syncwarp();                                          // all lanes are done with the stage
       if (RS > 1 && lane == 0) mbar_arrive1(bars + 16 * s + 8);
-      if (i + RINGS * AHEAD < seg_b) {
+      if (i + AHEAD < seg_b) {
         const int kn = k + AHEAD;
         ask(kn, __shfl_sync(0xffffffffu, (kn >> 5) == (k >> 5) ? page_cur : page_nxt, kn & 31));
       }
     }
-    // ---- the next segment's first blocks are on their way while this one is merged
+    // ---- the next segment's first blocks are on their way while this one is written
     const Unit du = u;
     const int d_head = head, done = split ? seg_b - seg_a : 1, u_begin = at - tile;
-    const bool whole = !split || done == du.tiles, goes_on = !whole && u_begin + du.tiles > end;
-    const bool begun = !whole && tile == 0;                  // this CTA has the unit's first part
+    const bool whole = !split || done == du.tiles, begun = !whole && tile == 0;      // begun: the unit's first part is here
+    const int last = whole ? worker : (u_begin + du.tiles - 1) / share;              // who has its last
     at += done;
     const bool more = at < end;
     if (more) {
@@ -520,139 +473,98 @@ __global__ void __launch_bounds__(THREADS, (AttnCfg<T, P, NT, RS>::CTAS)) qkv_at
       }
       begin_segment();
     }
+    // ---- a warp's rows are its own: straight to memory, 32 bytes of a row (bf16) at a time
     const float r_inv = pow2(R - 14);
+    const int part = 2 * worker + (begun ? 1 : 0);
 #pragma unroll
     for (int o = 4; o < 32; o <<= 1)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int x = 0; x < 2; ++x) l_run[nt][x] += __shfl_xor_sync(0xffffffffu, l_run[nt][x], o);
-    const int part = 2 * (int)blockIdx.x + (begun ? 1 : 0);
-    if constexpr (RS > 1) {
-      // ---- a warp's rows are its own: straight to memory, 32 bytes of a row (bf16) at a time
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const float l = l_run[nt][x];
-          const int r = row0 + 8 * nt + 2 * rc + x, f = du.f0 + r;
-          if (f >= du.nf) continue;
-          const float inv = whole ? (l == 0.f ? 0.f : r_inv / l) : r_inv;    // nothing seen: zero
-          T* out = reinterpret_cast<T*>(a.out) + ((long long)(du.r0 + f / G) * v.H + d_head * G + f % G) * v.d + 2 * rg;
-          float* part_o = a.part_o + ((long long)part * RT + r) * P + 2 * rg;
+      for (int x = 0; x < 2; ++x) {
+        const int r = row0 + 8 * nt + 2 * rc + x, tok = row_t[nt][x];
+        const float l = l_run[nt][x];
+        if (tok < 0) continue;
+        const float inv = whole ? (l == 0.f ? 0.f : r_inv / l) : r_inv;      // nothing seen: zero
+        T* out = reinterpret_cast<T*>(a.out) + ((long long)(du.r0 + tok) * v.H + d_head * G + (du.f0 + r - tok * G)) * v.d + 2 * rg;
+        float* part_o = a.part_o + ((long long)part * RT + r) * P + 2 * rg;
 #pragma unroll
-          for (int c = 0; c < CH; ++c) {
-            const float2 y = make_float2(acc[c][nt][x] * inv, acc[c][nt][2 + x] * inv);
-            if (!whole) *reinterpret_cast<float2*>(part_o + 16 * c) = y;
-            else if (16 * c + 2 * rg < v.d) {
-              if constexpr (sizeof(T) == 4) *reinterpret_cast<float2*>(out + 16 * c) = y;
-              else *reinterpret_cast<__nv_bfloat162*>(out + 16 * c) = __floats2bfloat162_rn(y.x, y.y);
-            }
+        for (int c = 0; c < CH; ++c) {
+          const float2 y = make_float2(acc[c][nt][x] * inv, acc[c][nt][2 + x] * inv);
+          if (!whole) *reinterpret_cast<float2*>(part_o + 16 * c) = y;
+          else if (16 * c + 2 * rg < v.d) {
+            if constexpr (sizeof(T) == 4) *reinterpret_cast<float2*>(out + 16 * c) = y;
+            else *reinterpret_cast<__nv_bfloat162*>(out + 16 * c) = __floats2bfloat162_rn(y.x, y.y);
           }
-          if (!whole && rg == 0) a.part_ml[part * RT + r] = make_float2(m_run[nt][x], l);
         }
-      __syncthreads();
-    } else {
-      // ---- the four warps' results of a row
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-          if (rg == 0) s_ml[warp * RT + 8 * nt + 2 * rc + x] = make_float2(m_run[nt][x], l_run[nt][x]);
-      __syncthreads();
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int x = 0; x < 2; ++x) {
-          const int r = 8 * nt + 2 * rc + x;
-          float m = -CUDART_INF_F;
-#pragma unroll
-          for (int w = 0; w < WARPS; ++w) m = fmaxf(m, s_ml[w * RT + r].x);
-          const float f = m_run[nt][x] == -CUDART_INF_F ? 0.f : ex2(m_run[nt][x] - m) * r_inv;
-#pragma unroll
-          for (int c = 0; c < CH; ++c) { acc[c][nt][x] *= f; acc[c][nt][2 + x] *= f; }
-        }
-    constexpr int SUB = C::SUB, MP = C::MP;
-    const int o_sub = tid / (RT * 4), o_row = tid / 4 % RT, o_c = 4 * (tid % 4), f = du.f0 + o_row;
-    float m_all = -CUDART_INF_F, l_all = 0.f;
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) m_all = fmaxf(m_all, s_ml[w * RT + o_row].x);
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-      const float2 x = s_ml[w * RT + o_row];
-      l_all += x.y * (x.x == -CUDART_INF_F ? 0.f : ex2(x.x - m_all));       // a sum that is not a number stays one
-    }
-    const float inv = l_all == 0.f ? 0.f : 1.f / l_all;      // nothing seen: zero
-    T* out = reinterpret_cast<T*>(a.out) + ((long long)(du.r0 + f / G) * v.H + d_head * G + f % G) * v.d;
-    float* part_o = a.part_o + ((long long)part * RT + o_row) * P;
-#pragma unroll
-    for (int c0 = 0; c0 < CH; c0 += SUB) {
-#pragma unroll
-      for (int sub = 0; sub < SUB; ++sub) {
-        if (c0 + sub >= CH) break;
-        const int cc = c0 + sub < CH ? c0 + sub : 0;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int x = 0; x < 2; ++x)
-            *reinterpret_cast<float2*>(s_merge + ((sub * WARPS + warp) * RT + 8 * nt + 2 * rc + x) * MP + 2 * rg) = make_float2(acc[cc][nt][x], acc[cc][nt][2 + x]);
+        if (!whole && rg == 0) a.part_ml[part * RT + r] = make_float2(m_run[nt][x], l);
       }
-      __syncthreads();
-      const int c = 16 * (c0 + o_sub) + o_c;
-      if (o_sub < SUB && f < du.nf && c < P) {
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-        for (int w = 0; w < WARPS; ++w) {
-          const float4 y = *reinterpret_cast<const float4*>(s_merge + ((o_sub * WARPS + w) * RT + o_row) * MP + o_c);
-          x = make_float4(x.x + y.x, x.y + y.y, x.z + y.z, x.w + y.w);
-        }
-        if (!whole) store4(part_o + c, x);
-        else if (c < v.d) store4(out + c, scaled(x, inv));
-      }
-      __syncthreads();
+    if (begun && lane == 0 && (RS == 1 || warp == 0)) {      // a unit to merge: in any order, each by itself
+      const int n = last - worker + 1;
+      const bool many = n > MANY;
+      const int i = atomicAdd(a.n_cuts + (many ? 1 : 0), 1);
+      a.cuts[many ? a.max_cuts - 1 - i : i] = {du.r0, du.f0, du.nf, d_head, worker, n};
     }
-    if (!whole && f < du.nf && tid % 4 == 0 && o_sub == 0) a.part_ml[part * RT + o_row] = make_float2(m_all, l_all);
-    }
-    if (begun && goes_on && tid == 0)                        // the CTAs that have its blocks: this one and the next ones
-      a.cuts[blockIdx.x] = {du.r0, du.f0, du.nf, d_head, (u_begin + du.tiles - 1) / share - (int)blockIdx.x + 1};
     if (!more) break;
   }
 }
 
-// Parts of the units that were cut, in the order of their CTAs: a warp per row.  grid (CTAs of the attention, row groups), block 128
+// Parts of the units that were cut, in the order of their shares: a warp for a row, or, with many parts, a CTA.  The last CTA empties
+// the lists.
 template <typename T, int P>
-__global__ void __launch_bounds__(THREADS) qkv_merge_kernel(QkvAttnArgs a, int RT) {
-  constexpr int Y = P > 128 ? 2 : 1, IN = Y > 1 ? 8 : 16;    // parts asked for at a time
+__global__ void __launch_bounds__(32 * MERGE_WARPS) qkv_merge_kernel(QkvAttnArgs a, int RT) {
+  constexpr int Y = P > 128 ? 2 : 1, IN = Y > 1 ? 8 : 16;         // parts asked for at a time
+  __shared__ float4 s_sum[MERGE_WARPS][32 * Y];
+  __shared__ float s_l[MERGE_WARPS];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, G = a.v.H / a.v.KH, groups = (RT + MERGE_WARPS - 1) / MERGE_WARPS;
   pdl_wait();
-  const QkvCut o = a.cuts[blockIdx.x];
-  const int lane = threadIdx.x & 31, rows = min(RT, o.nf - o.f0), G = a.v.H / a.v.KH;
-  for (int r = blockIdx.y * WARPS + (threadIdx.x >> 5); o.n > 0 && r < rows; r += gridDim.y * WARPS) {
-    auto at = [&](int j) { return (long long)(2 * (blockIdx.x + j) + (j == 0 ? 1 : 0)) * RT + r; };
-    float m = -CUDART_INF_F, l = 0.f;
-    for (int j = lane; j < o.n; j += 32) m = fmaxf(m, a.part_ml[at(j)].x);
+  QkvCut o = a.cuts[blockIdx.x / groups];                    // asked for together with the lists' lengths
+  const int n_few = a.n_cuts[0] * groups, n_all = n_few + a.n_cuts[1] * RT;
+  for (int item = blockIdx.x; item < n_all; item += gridDim.x) {
+    const bool many = item >= n_few;
+    const int x0 = item - n_few;
+    if (many) o = a.cuts[a.max_cuts - 1 - x0 / RT];
+    else if (item != blockIdx.x) o = a.cuts[item / groups];
+    const int rows = min(RT, o.nf - o.f0), r = many ? x0 % RT : item % groups * MERGE_WARPS + warp;
+    if (r >= rows) continue;                                 // many: the same for all warps
+    const int step = many ? MERGE_WARPS : 1, own = many ? warp : 0;          // this warp's parts: own, own + step, ..
+    auto at = [&](int j) { return (long long)(2 * (o.first + j) + (j == 0 ? 1 : 0)) * RT + r; };
+    auto ask = [&](int j0, float4 (&x)[IN][Y]) {
+#pragma unroll
+      for (int j = 0; j < IN; ++j)
+#pragma unroll
+        for (int y = 0; y < Y; ++y) {
+          const int c = 4 * lane + 128 * y;
+          x[j][y] = c < P ? *reinterpret_cast<const float4*>(a.part_o + at(min(j0 + j * step, o.n - 1)) * P + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+    };
+    float4 x[IN][Y];
+    ask(own, x);
+    float2 ml = make_float2(-CUDART_INF_F, 0.f);
+    if (own + lane * step < o.n) ml = a.part_ml[at(own + lane * step)];
+    float m = ml.x, l = 0.f;
+    if (many)
+      for (int j = lane; j < o.n; j += 32) m = fmaxf(m, a.part_ml[at(j)].x);
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
     float4 sum[Y];
 #pragma unroll
     for (int y = 0; y < Y; ++y) sum[y] = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int j0 = 0; j0 < o.n; j0 += 32) {
-      float w = 0.f;
-      if (j0 + lane < o.n) {
-        const float2 ml = a.part_ml[at(j0 + lane)];
-        // nothing seen: no weight; a sum without a maximum is no number
-        w = ml.x == -CUDART_INF_F ? (ml.y == 0.f ? 0.f : CUDART_NAN_F) : ex2(ml.x - m);
-        l += ml.y * w;
+    for (int j0 = own; j0 < o.n; j0 += 32 * step) {
+      if (j0 != own) {
+        ml = make_float2(-CUDART_INF_F, 0.f);
+        if (j0 + lane * step < o.n) ml = a.part_ml[at(j0 + lane * step)];
       }
+      // nothing seen: no weight; a sum without a maximum is no number
+      const float w = ml.x == -CUDART_INF_F ? (ml.y == 0.f ? 0.f : CUDART_NAN_F) : ex2(ml.x - m);
+      l += ml.y * w;
 #pragma unroll 1
-      for (int j1 = 0; j1 < 32 && j0 + j1 < o.n; j1 += IN) {
-        float4 x[IN][Y];
-#pragma unroll
-        for (int j = 0; j < IN; ++j)
-#pragma unroll
-          for (int y = 0; y < Y; ++y) {
-            const int c = 4 * lane + 128 * y;
-            x[j][y] = c < P ? *reinterpret_cast<const float4*>(a.part_o + at(min(j0 + j1 + j, o.n - 1)) * P + c) : make_float4(0.f, 0.f, 0.f, 0.f);
-          }
+      for (int j1 = 0; j1 < 32 && j0 + j1 * step < o.n; j1 += IN) {
+        if (j0 != own || j1) ask(j0 + j1 * step, x);
 #pragma unroll
         for (int j = 0; j < IN; ++j) {
           const float f = __shfl_sync(0xffffffffu, w, j1 + j);
@@ -663,12 +575,34 @@ __global__ void __launch_bounds__(THREADS) qkv_merge_kernel(QkvAttnArgs a, int R
       }
     }
     l = warp_sum(l);
+    if (many) {
+#pragma unroll
+      for (int y = 0; y < Y; ++y) s_sum[warp][lane + 32 * y] = sum[y];
+      if (lane == 0) s_l[warp] = l;
+      __syncthreads();
+      l = 0.f;
+#pragma unroll
+      for (int y = 0; y < Y; ++y) sum[y] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < MERGE_WARPS; ++w) {
+        l += s_l[w];
+#pragma unroll
+        for (int y = 0; y < Y; ++y) {
+          const float4 x = s_sum[w][lane + 32 * y];
+          sum[y] = make_float4(sum[y].x + x.x, sum[y].y + x.y, sum[y].z + x.z, sum[y].w + x.w);
+        }
+      }
+      __syncthreads();
+      if (warp) continue;
+    }
     const int f = o.f0 + r;
     T* out = reinterpret_cast<T*>(a.out) + ((long long)(o.r0 + f / G) * a.v.H + o.head * G + f % G) * a.v.d;
 #pragma unroll
     for (int y = 0; y < Y; ++y)
       if (4 * lane + 128 * y < a.v.d) store4(out + 4 * lane + 128 * y, scaled(sum[y], l == 0.f ? 0.f : 1.f / l));
   }
+  __syncthreads();
+  if (threadIdx.x == 0 && atomicAdd(a.n_cuts + 2, 1) == (int)gridDim.x - 1) { a.n_cuts[0] = 0; a.n_cuts[1] = 0; a.n_cuts[2] = 0; }
 }
 
 template <typename T, int SCHEME, int P, int NT, int RS>
@@ -683,6 +617,9 @@ int32_t launch(vn_qkv* c, const QkvAttnArgs& a) {
     int n = 0;
     VN_CUDA(ctx, cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, kernel, THREADS, C::SMEM));
     VN_REQUIRE(ctx, n > 0, "qkv_attn_kernel does not fit an SM");
+    // the same division of the SMs' memory for both, so that neither has to wait for another one
+    VN_CUDA(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
+    VN_CUDA(ctx, cudaFuncSetAttribute(qkv_merge_kernel<T, P>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
     occ = min(n, C::CTAS);
   }
   const long long rts = ceil_div((long long)a.step.T * (a.v.H / a.v.KH), (long long)C::RT);
@@ -691,9 +628,9 @@ int32_t launch(vn_qkv* c, const QkvAttnArgs& a) {
   // units of a few blocks stay whole: cutting them saves less than the merge costs
   const bool split = tiles > UNCUT;
   // no more CTAs than there can be shares
-  const unsigned grid = (unsigned)min((long long)occ * ctx->sm_count, split ? ceil_div(blocks * tiles, (long long)MIN_SHARE) : blocks);
-  VN_LAUNCH_NAMED(ctx, "qkv_attn_kernel", kernel, grid, THREADS, C::SMEM, a, (int)rts, split);
-  if (split) VN_LAUNCH_PDL_LEVEL(ctx, 1, "qkv_merge_kernel", (qkv_merge_kernel<T, P>), dim3(grid, min(C::RT / WARPS, 16)), THREADS, 0, a, C::RT);
+  const unsigned grid = (unsigned)min((long long)occ * ctx->sm_count, ceil_div(split ? ceil_div(blocks * tiles, (long long)MIN_SHARE) : blocks, (long long)C::RINGS));
+  VN_LAUNCH_PDL_LEVEL(ctx, 1, "qkv_attn_kernel", kernel, grid, THREADS, C::SMEM, a, (int)rts, split);
+  if (split) VN_LAUNCH_PDL_LEVEL(ctx, 1, "qkv_merge_kernel", (qkv_merge_kernel<T, P>), dim3((unsigned)ctx->sm_count * 2), 32 * MERGE_WARPS, 0, a, C::RT);
   return VN_OK;
 }
 
