@@ -514,92 +514,102 @@ __global__ void __launch_bounds__(THREADS, (AttnCfg<T, P, NT, RS>::CTAS)) qkv_at
 }
 
 // Parts of the units that were cut, in the order of their shares: a warp for a row, or, with many parts, a CTA.  The last CTA empties
-// the lists.
+// the lists.  The kernel begins while the shares end; it goes through the motions once before it waits for them, so that its
+// instructions are there (without that a row took 3 us, most of it fetching them).  rmax: rows of a unit at most
 template <typename T, int P>
-__global__ void __launch_bounds__(32 * MERGE_WARPS) qkv_merge_kernel(QkvAttnArgs a, int RT) {
-  constexpr int Y = P > 128 ? 2 : 1, IN = Y > 1 ? 8 : 16;         // parts asked for at a time
+__global__ void __launch_bounds__(32 * MERGE_WARPS) qkv_merge_kernel(QkvAttnArgs a, int RT, int rmax) {
+  constexpr int Y = P > 128 ? 2 : 1, IN = Y > 1 ? 8 : 16;    // parts asked for at a time
   __shared__ float4 s_sum[MERGE_WARPS][32 * Y];
   __shared__ float s_l[MERGE_WARPS];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, G = a.v.H / a.v.KH, groups = (RT + MERGE_WARPS - 1) / MERGE_WARPS;
-  pdl_wait();
-  QkvCut o = a.cuts[blockIdx.x / groups];                    // asked for together with the lists' lengths
-  const int n_few = a.n_cuts[0] * groups, n_all = n_few + a.n_cuts[1] * RT;
-  for (int item = blockIdx.x; item < n_all; item += gridDim.x) {
-    const bool many = item >= n_few;
-    const int x0 = item - n_few;
-    if (many) o = a.cuts[a.max_cuts - 1 - x0 / RT];
-    else if (item != blockIdx.x) o = a.cuts[item / groups];
-    const int rows = min(RT, o.nf - o.f0), r = many ? x0 % RT : item % groups * MERGE_WARPS + warp;
-    if (r >= rows) continue;                                 // many: the same for all warps
-    const int step = many ? MERGE_WARPS : 1, own = many ? warp : 0;          // this warp's parts: own, own + step, ..
-    auto at = [&](int j) { return (long long)(2 * (o.first + j) + (j == 0 ? 1 : 0)) * RT + r; };
-    auto ask = [&](int j0, float4 (&x)[IN][Y]) {
-#pragma unroll
-      for (int j = 0; j < IN; ++j)
-#pragma unroll
-        for (int y = 0; y < Y; ++y) {
-          const int c = 4 * lane + 128 * y;
-          x[j][y] = c < P ? *reinterpret_cast<const float4*>(a.part_o + at(min(j0 + j * step, o.n - 1)) * P + c) : make_float4(0.f, 0.f, 0.f, 0.f);
-        }
-    };
-    float4 x[IN][Y];
-    ask(own, x);
-    float2 ml = make_float2(-CUDART_INF_F, 0.f);
-    if (own + lane * step < o.n) ml = a.part_ml[at(own + lane * step)];
-    float m = ml.x, l = 0.f;
-    if (many)
-      for (int j = lane; j < o.n; j += 32) m = fmaxf(m, a.part_ml[at(j)].x);
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
-    float4 sum[Y];
-#pragma unroll
-    for (int y = 0; y < Y; ++y) sum[y] = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int j0 = own; j0 < o.n; j0 += 32 * step) {
-      if (j0 != own) {
-        ml = make_float2(-CUDART_INF_F, 0.f);
-        if (j0 + lane * step < o.n) ml = a.part_ml[at(j0 + lane * step)];
-      }
-      // nothing seen: no weight; a sum without a maximum is no number
-      const float w = ml.x == -CUDART_INF_F ? (ml.y == 0.f ? 0.f : CUDART_NAN_F) : ex2(ml.x - m);
-      l += ml.y * w;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, G = a.v.H / a.v.KH;
 #pragma unroll 1
-      for (int j1 = 0; j1 < 32 && j0 + j1 * step < o.n; j1 += IN) {
-        if (j0 != own || j1) ask(j0 + j1 * step, x);
+  for (int pass = 0; pass < 2; ++pass) {
+    int n_few = 1, n_all = 1;
+    QkvCut o = {0, 0, rmax, 0, 0, 1};
+    if (pass) {
+      pdl_wait();
+      o = a.cuts[min((blockIdx.x * MERGE_WARPS + warp) / rmax, a.max_cuts - 1)];       // asked for together with the lists' lengths
+      n_few = a.n_cuts[0] * rmax;
+      n_all = (n_few + MERGE_WARPS - 1) / MERGE_WARPS + a.n_cuts[1] * rmax;
+    }
+#pragma unroll 1
+    for (int item = pass ? blockIdx.x : 0; item < n_all; item += gridDim.x) {
+      const int few = item * MERGE_WARPS + warp, x0 = item - (n_few + MERGE_WARPS - 1) / MERGE_WARPS;
+      const bool many = x0 >= 0;
+      if (!many && few >= n_few) continue;
+      if (many) o = a.cuts[a.max_cuts - 1 - x0 / rmax];
+      else if (item != blockIdx.x) o = a.cuts[few / rmax];
+      const int r = many ? x0 % rmax : few % rmax;
+      if (r >= min(RT, o.nf - o.f0)) continue;               // many: the same for all warps
+      const int step = many ? MERGE_WARPS : 1, own = many ? warp : 0;        // this warp's parts: own, own + step, ..
+      auto at = [&](int j) { return (long long)(2 * (o.first + j) + (j == 0 ? 1 : 0)) * RT + r; };
+      float4 sum[Y];
+      float m = -CUDART_INF_F, l = 0.f;
+#pragma unroll
+      for (int y = 0; y < Y; ++y) sum[y] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (many)
+        for (int j0 = lane; j0 < o.n; j0 += 256) {
+          float x[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) x[e] = a.part_ml[at(min(j0 + 32 * e, o.n - 1))].x;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) m = fmaxf(m, x[e]);
+        }
+#pragma unroll 1
+      for (int j0 = own; j0 < o.n; j0 += IN * step) {
+        float4 x[IN][Y];
+#pragma unroll
+        for (int j = 0; j < IN; ++j)
+#pragma unroll
+          for (int y = 0; y < Y; ++y) {
+            const int c = 4 * lane + 128 * y;
+            x[j][y] = c < P ? *reinterpret_cast<const float4*>(a.part_o + at(min(j0 + j * step, o.n - 1)) * P + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+          }
+        float2 ml = make_float2(-CUDART_INF_F, 0.f);
+        if (lane < IN && j0 + lane * step < o.n) ml = a.part_ml[at(j0 + lane * step)];
+        if (j0 == own) {
+          m = fmaxf(m, ml.x);
+#pragma unroll
+          for (int d = 16; d > 0; d >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, d));
+        }
+        // nothing seen: no weight; a sum without a maximum is no number
+        const float w = ml.x == -CUDART_INF_F ? (ml.y == 0.f ? 0.f : CUDART_NAN_F) : ex2(ml.x - m);
+        l += ml.y * w;
 #pragma unroll
         for (int j = 0; j < IN; ++j) {
-          const float f = __shfl_sync(0xffffffffu, w, j1 + j);
+          const float f = __shfl_sync(0xffffffffu, w, j);
 #pragma unroll
           for (int y = 0; y < Y; ++y)
             sum[y] = make_float4(fmaf(x[j][y].x, f, sum[y].x), fmaf(x[j][y].y, f, sum[y].y), fmaf(x[j][y].z, f, sum[y].z), fmaf(x[j][y].w, f, sum[y].w));
         }
       }
-    }
-    l = warp_sum(l);
-    if (many) {
+      l = warp_sum(l);
+      if (many) {
 #pragma unroll
-      for (int y = 0; y < Y; ++y) s_sum[warp][lane + 32 * y] = sum[y];
-      if (lane == 0) s_l[warp] = l;
-      __syncthreads();
-      l = 0.f;
+        for (int y = 0; y < Y; ++y) s_sum[warp][lane + 32 * y] = sum[y];
+        if (lane == 0) s_l[warp] = l;
+        __syncthreads();
+        l = 0.f;
 #pragma unroll
-      for (int y = 0; y < Y; ++y) sum[y] = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int y = 0; y < Y; ++y) sum[y] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-      for (int w = 0; w < MERGE_WARPS; ++w) {
-        l += s_l[w];
+        for (int w = 0; w < MERGE_WARPS; ++w) {
+          l += s_l[w];
 #pragma unroll
-        for (int y = 0; y < Y; ++y) {
-          const float4 x = s_sum[w][lane + 32 * y];
-          sum[y] = make_float4(sum[y].x + x.x, sum[y].y + x.y, sum[y].z + x.z, sum[y].w + x.w);
+          for (int y = 0; y < Y; ++y) {
+            const float4 x = s_sum[w][lane + 32 * y];
+            sum[y] = make_float4(sum[y].x + x.x, sum[y].y + x.y, sum[y].z + x.z, sum[y].w + x.w);
+          }
         }
+        __syncthreads();
       }
-      __syncthreads();
-      if (warp) continue;
-    }
-    const int f = o.f0 + r;
-    T* out = reinterpret_cast<T*>(a.out) + ((long long)(o.r0 + f / G) * a.v.H + o.head * G + f % G) * a.v.d;
+      if ((many && warp) || !pass) continue;
+      const int f = o.f0 + r;
+      T* out = reinterpret_cast<T*>(a.out) + ((long long)(o.r0 + f / G) * a.v.H + o.head * G + f % G) * a.v.d;
 #pragma unroll
-    for (int y = 0; y < Y; ++y)
-      if (4 * lane + 128 * y < a.v.d) store4(out + 4 * lane + 128 * y, scaled(sum[y], l == 0.f ? 0.f : 1.f / l));
+      for (int y = 0; y < Y; ++y)
+        if (4 * lane + 128 * y < a.v.d) store4(out + 4 * lane + 128 * y, scaled(sum[y], l == 0.f ? 0.f : 1.f / l));
+    }
   }
   __syncthreads();
   if (threadIdx.x == 0 && atomicAdd(a.n_cuts + 2, 1) == (int)gridDim.x - 1) { a.n_cuts[0] = 0; a.n_cuts[1] = 0; a.n_cuts[2] = 0; }
@@ -630,7 +640,7 @@ int32_t launch(vn_qkv* c, const QkvAttnArgs& a) {
   // no more CTAs than there can be shares
   const unsigned grid = (unsigned)min((long long)occ * ctx->sm_count, ceil_div(split ? ceil_div(blocks * tiles, (long long)MIN_SHARE) : blocks, (long long)C::RINGS));
   VN_LAUNCH_PDL_LEVEL(ctx, 1, "qkv_attn_kernel", kernel, grid, THREADS, C::SMEM, a, (int)rts, split);
-  if (split) VN_LAUNCH_PDL_LEVEL(ctx, 1, "qkv_merge_kernel", (qkv_merge_kernel<T, P>), dim3((unsigned)ctx->sm_count * 2), 32 * MERGE_WARPS, 0, a, C::RT);
+  if (split) VN_LAUNCH_PDL_LEVEL(ctx, 1, "qkv_merge_kernel", (qkv_merge_kernel<T, P>), dim3((unsigned)ctx->sm_count * 2), 32 * MERGE_WARPS, 0, a, C::RT, (int)min((long long)C::RT, (long long)a.step.T * (a.v.H / a.v.KH)));
   return VN_OK;
 }
 
