@@ -19,7 +19,8 @@ struct AppendArgs {
   int off = 0, H = 0;                  // H = 0: the rows hold no queries
   const float *qn = nullptr, *kn = nullptr, *cs = nullptr, *sn = nullptr;
   float eps = 0.f;
-  int pairs = 0, interleaved = 0, rope_rows = 0, vec = 0;
+  int pairs = 0, interleaved = 0, rope_rows = 0;
+  int vec = 0, vec_norm = 0, vec_rope = 0;            // rows, norms' weights, rotation in whole quads
 };
 
 template <typename T> __device__ __forceinline__ float4 quad_of(const T* p, bool vec) {
@@ -38,105 +39,228 @@ __device__ __forceinline__ unsigned char code_of(float y, int scheme) {
   return (unsigned char)r;
 }
 
-// One warp per (row, head); a lane takes quads lane, lane + 32 of the head, which is staged in shared memory for the rotation.
-// grid ceil(M units / 8), block (32, 8)
-template <typename T>
-__global__ void __launch_bounds__(256) qkv_append_kernel(AppendArgs a) {
-  __shared__ __align__(16) float s_head[8][256];
-  const int units = a.H + 2 * a.v.KH, lane = threadIdx.x;
-  const long long task = (long long)blockIdx.x * 8 + threadIdx.y;
-  const int unit = (int)(task % units);
-  if (task / units >= a.step.M) return;
-  const int row = (int)(task / units);
+__device__ __forceinline__ float4 quad_at(const float* p, bool vec) { return vec ? load4(p) : make_float4(p[0], p[1], p[2], p[3]); }
+
+// A warp takes `per` tasks of a row, four asked for at a time: a task is 32 / L neighbouring heads, whose L lanes hold Y quads of channels
+// each (lane, lane + 32).  Heads pass through shared memory only for half-split rotation, where a quad meets the one pairs further on.
+// What bounds it: the rows' bytes for many rows; for few, the chain entry, length, page, store (the row's values are asked for first).
+// grid ceil(M ceil(tasks / per) / 8), block 256
+template <typename T, int L, int Y>
+__global__ void __launch_bounds__(256) qkv_append_kernel(AppendArgs a, int tasks, int per) {
+  constexpr int HPW = 32 / L, IN = Y > 1 ? 2 : 4;
+  __shared__ __align__(16) float s_head[8][HPW][4 * L * Y];
+  const int lane = threadIdx.x & 31, l = lane % L, sub = lane / L, warp = threadIdx.x >> 5;
+  const int units = a.H + 2 * a.v.KH, d = a.v.d, P = a.v.P, slices = (tasks + per - 1) / per;
+  const unsigned item = blockIdx.x * 8u + warp;
+  pdl_wait();
+  const int row = (int)(item / (unsigned)slices), first = (int)(item % (unsigned)slices) * per, last = min(tasks, first + per);
+  if (row >= a.step.M) return;
+  const T* xr = reinterpret_cast<const T*>(a.x) + row * a.ld;
+  float4 x[IN][Y];
+  auto ask = [&](int task) {
+#pragma unroll
+    for (int k = 0; k < IN; ++k)
+#pragma unroll
+      for (int y = 0; y < Y; ++y) {
+        const int unit = (task + k) * HPW + sub, c = 4 * l + 128 * y;
+        x[k][y] = task + k < last && unit < units && c < d ? quad_of(xr + (long long)unit * d + c, a.vec) : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+  };
+  ask(first);
   int slot, i, n;
   if (!a.step.row(a.v, row, &slot, &i, &n)) return;
-  const bool is_q = unit < a.H, is_v = unit >= a.H + a.v.KH;
-  const int len = a.v.len(slot), pos = len + a.off + i, d = a.v.d;
-  const int turn = len + a.off + a.tree.away(row, i);
-  float* s = s_head[threadIdx.y];
-  const T* x = reinterpret_cast<const T*>(a.x) + row * a.ld + (long long)unit * d;
-  const float* w = is_v ? nullptr : is_q ? a.qn : a.kn;
-  float ss = 0.f;
-  for (int c = 4 * lane; c < d; c += 128) {
-    const float4 v = quad_of(x + c, a.vec);
-    *reinterpret_cast<float4*>(s + c) = v;
-    ss += v.x * v.x + v.y * v.y + v.z * v.z + v.w * v.w;
-  }
-  const float r = w ? sqrtf(warp_sum(ss) / (float)d + a.eps) : 1.f;
-  __syncwarp();
-  if (w) {
-    for (int c = lane; c < d; c += 32) s[c] = s[c] / r * w[c];
-    __syncwarp();
-  }
-  if (!is_v && a.pairs) {
-    const long long at = (long long)min(max(turn, 0), a.rope_rows - 1) * a.pairs;
-    for (int p = lane; p < a.pairs; p += 32) {
-      const int cu = a.interleaved ? 2 * p : p, cv = a.interleaved ? 2 * p + 1 : p + a.pairs;
-      const float u = s[cu], v = s[cv], cs = a.cs[at + p], sn = a.sn[at + p];
-      s[cu] = u * cs - v * sn;
-      s[cv] = v * cs + u * sn;
-    }
-    __syncwarp();
-  }
-  if (is_q) {
-    T* o = reinterpret_cast<T*>(a.q) + ((long long)row * a.H + unit) * d;
-    for (int c = 4 * lane; c < d; c += 128) put_quad(o + c, *reinterpret_cast<const float4*>(s + c), a.vec);
-    return;
-  }
-  const int head = unit - a.H - (is_v ? a.v.KH : 0);
-  const int page = pos >= 0 && pos < a.v.capacity() ? a.v.page(slot, pos / KV_PAGE) : -1;
-  if (page < 0) { if (lane == 0) a.v.status[0] = 1; return; }
-  float top = 0.f;
-  bool bad = false;
-  for (int c = lane; c < d; c += 32) { top = fmaxf(top, fabsf(s[c])); bad |= !isfinite(s[c]); }
+  const int len = a.v.len(slot), pos = len + a.off + i;
+  const int turn = min(max(len + a.off + a.tree.away(row, i), 0), a.rope_rows - 1);
+  const int page = pos >= 0 && pos < a.v.capacity() ? a.v.page(slot, pos / KV_PAGE) : -1, at = pos % QKV_BLOCK;
+  // what a quad is turned by: half-split, quads of the two halves by the same angles
+  float4 cs[Y], sn[Y];
+  bool turned[Y];
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  bad = __any_sync(0xffffffffu, bad);
-  const float scale = fmaxf((top > 0.f ? top : 1.f) / (a.v.scheme == QKV_I8 ? 127.f : 448.f), QKV_SCALE_MIN);
-  unsigned char* b = a.v.block(page, head, pos % KV_PAGE / QKV_BLOCK);
-  const int at = pos % QKV_BLOCK, P = a.v.P, t = qkv_turn(P / 16, at);
-  unsigned char* codes = b + (is_v ? QKV_BLOCK * P : 0) + at * P;
-  for (int c = 4 * lane; c < P; c += 128) {
-    const unsigned char none = a.v.scheme == QKV_I8 ? 128 : 0;
-    uchar4 k = make_uchar4(none, none, none, none);
-    if (c < d && !bad) {
-      const float4 v = *reinterpret_cast<const float4*>(s + c);
-      k = make_uchar4(code_of(v.x / scale, a.v.scheme), code_of(v.y / scale, a.v.scheme), code_of(v.z / scale, a.v.scheme), code_of(v.w / scale, a.v.scheme));
+  for (int y = 0; y < Y; ++y) {
+    const int c = 4 * l + 128 * y, np = a.pairs;
+    turned[y] = np && c < 2 * np;
+    cs[y] = make_float4(1.f, 1.f, 1.f, 1.f);
+    sn[y] = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (!turned[y]) continue;
+    const float *pc = a.cs + (long long)turn * np, *ps = a.sn + (long long)turn * np;
+    if (a.interleaved) {
+      const bool two = c + 2 < 2 * np;
+      cs[y].x = cs[y].y = pc[c / 2]; sn[y].x = sn[y].y = ps[c / 2];
+      if (two) { cs[y].z = cs[y].w = pc[c / 2 + 1]; sn[y].z = sn[y].w = ps[c / 2 + 1]; }
+    } else if (a.vec_rope) {
+      cs[y] = load4(pc + (c < np ? c : c - np)); sn[y] = load4(ps + (c < np ? c : c - np));
+    } else {
+      auto angle = [&](int e, float& u, float& w) {
+        if (c + e < 2 * np) { const int p = c + e < np ? c + e : c + e - np; u = pc[p]; w = ps[p]; }
+      };
+      angle(0, cs[y].x, sn[y].x); angle(1, cs[y].y, sn[y].y); angle(2, cs[y].z, sn[y].z); angle(3, cs[y].w, sn[y].w);
     }
-    *reinterpret_cast<uchar4*>(codes + (((c >> 4) ^ t) << 4) + (c & 15)) = k;
   }
-  if (lane == 0) reinterpret_cast<float*>(b + 2 * QKV_BLOCK * P)[(is_v ? QKV_BLOCK : 0) + at] = bad ? CUDART_NAN_F : scale;
+  float* s = s_head[warp][sub];
+#pragma unroll 1
+  for (int task = first; task < last; task += IN) {
+    if (task != first) ask(task);
+#pragma unroll
+    for (int k = 0; k < IN; ++k) {
+      if (task + k >= last) break;
+      const int unit = (task + k) * HPW + sub;
+      const bool live = unit < units, is_q = unit < a.H, is_v = unit >= a.H + a.v.KH;
+      float4 v[Y];
+#pragma unroll
+      for (int y = 0; y < Y; ++y) v[y] = x[k][y];
+      const float* w = is_v || !live ? nullptr : is_q ? a.qn : a.kn;
+      if (__any_sync(0xffffffffu, w != nullptr)) {           // a warp's heads may be of two kinds
+        float ss = 0.f;
+#pragma unroll
+        for (int y = 0; y < Y; ++y) ss += v[y].x * v[y].x + v[y].y * v[y].y + v[y].z * v[y].z + v[y].w * v[y].w;
+#pragma unroll
+        for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+        if (w) {
+          const float r = sqrtf(ss / (float)d + a.eps);
+#pragma unroll
+          for (int y = 0; y < Y; ++y) {
+            const int c = 4 * l + 128 * y;
+            if (c >= d) break;
+            const float4 g = quad_at(w + c, a.vec_norm);
+            v[y] = make_float4(v[y].x / r * g.x, v[y].y / r * g.y, v[y].z / r * g.z, v[y].w / r * g.w);
+          }
+        }
+      }
+      if (a.pairs && a.interleaved) {
+        if (!is_v)
+#pragma unroll
+          for (int y = 0; y < Y; ++y)
+            v[y] = make_float4(v[y].x * cs[y].x - v[y].y * sn[y].x, v[y].y * cs[y].x + v[y].x * sn[y].x, v[y].z * cs[y].z - v[y].w * sn[y].z, v[y].w * cs[y].z + v[y].z * sn[y].z);
+      } else if (a.pairs) {
+        __syncwarp();
+#pragma unroll
+        for (int y = 0; y < Y; ++y) *reinterpret_cast<float4*>(s + 4 * l + 128 * y) = v[y];
+        __syncwarp();
+#pragma unroll
+        for (int y = 0; y < Y; ++y) {
+          const int c = 4 * l + 128 * y, np = a.pairs;
+          if (is_v || !turned[y]) continue;
+          // the other half's values, with the sign that they enter with
+          auto other = [&](int e) { return c + e < np ? -s[c + e + np] : c + e < 2 * np ? s[c + e - np] : 0.f; };
+          float4 t;
+          if (a.vec_rope) {
+            t = *reinterpret_cast<const float4*>(s + (c < np ? c + np : c - np));
+            if (c < np) t = make_float4(-t.x, -t.y, -t.z, -t.w);
+          } else {
+            t = make_float4(other(0), other(1), other(2), other(3));
+          }
+          v[y] = make_float4(v[y].x * cs[y].x + t.x * sn[y].x, v[y].y * cs[y].y + t.y * sn[y].y, v[y].z * cs[y].z + t.z * sn[y].z, v[y].w * cs[y].w + t.w * sn[y].w);
+        }
+      }
+      if (live && is_q) {
+        T* o = reinterpret_cast<T*>(a.q) + ((long long)row * a.H + unit) * d;
+#pragma unroll
+        for (int y = 0; y < Y; ++y)
+          if (4 * l + 128 * y < d) put_quad(o + 4 * l + 128 * y, v[y], a.vec);
+      }
+      if (__all_sync(0xffffffffu, !live || is_q)) continue;
+      // ---- a head of the cache
+      unsigned top = 0;                                      // magnitudes as bits: what is not finite is above all others
+#pragma unroll
+      for (int y = 0; y < Y; ++y)
+        top = max(top, max(max(__float_as_uint(v[y].x) & 0x7fffffffu, __float_as_uint(v[y].y) & 0x7fffffffu),
+                           max(__float_as_uint(v[y].z) & 0x7fffffffu, __float_as_uint(v[y].w) & 0x7fffffffu)));
+#pragma unroll
+      for (int o = L / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      if (!live || is_q) continue;
+      if (page < 0) { if (l == 0) a.v.status[0] = 1; continue; }
+      const bool bad = top >= 0x7f800000u;
+      const float scale = fmaxf((top ? __uint_as_float(top) : 1.f) / (a.v.scheme == QKV_I8 ? 127.f : 448.f), QKV_SCALE_MIN);
+      const int head = unit - a.H - (is_v ? a.v.KH : 0), t = qkv_turn(P / 16, at);
+      unsigned char* b = a.v.block(page, head, pos % KV_PAGE / QKV_BLOCK);
+      unsigned char* codes = b + (is_v ? QKV_BLOCK * P : 0) + at * P;
+#pragma unroll
+      for (int y = 0; y < Y; ++y) {
+        const int c = 4 * l + 128 * y;
+        if (c >= P) break;
+        const unsigned char none = a.v.scheme == QKV_I8 ? 128 : 0;
+        uchar4 q = make_uchar4(none, none, none, none);
+        if (c < d && !bad) q = make_uchar4(code_of(v[y].x / scale, a.v.scheme), code_of(v[y].y / scale, a.v.scheme), code_of(v[y].z / scale, a.v.scheme), code_of(v[y].w / scale, a.v.scheme));
+        *reinterpret_cast<uchar4*>(codes + (((c >> 4) ^ t) << 4) + (c & 15)) = q;
+      }
+      if (l == 0) reinterpret_cast<float*>(b + 2 * QKV_BLOCK * P)[(is_v ? QKV_BLOCK : 0) + at] = bad ? CUDART_NAN_F : scale;
+    }
+  }
 }
 
-// One thread per 8 channels of a head at a position.  grid (ceil(M KH d / 8 / 256), 2)
-template <typename O, int SCHEME>
+// A thread takes 16 bytes of results (C channels of a head) of RB neighbouring rows, all asked for before any is converted; the rows'
+// blocks are found by the first threads.  Bound by the bytes of codes and results.
+// grid (ceil(M / RB), ceil(KH d / C / 256), 2), block 256
+template <typename O, int SCHEME, int RB>
 __global__ void __launch_bounds__(256) qkv_read_kernel(QkvView v, QkvStep step, int start, int off, O* __restrict__ k, O* __restrict__ vals, int vec) {
-  const long long t = (long long)blockIdx.x * 256 + threadIdx.x;
-  const int per = v.d / 8, c = (int)(t % per) * 8;
-  const long long rh = t / per;
-  const int head = (int)(rh % v.KH);
-  const long long row = rh / v.KH;
-  if (row >= step.M) return;
-  int slot, i, n;
-  if (!step.row(v, (int)row, &slot, &i, &n)) return;
-  const int pos = (start >= 0 ? start : v.len(slot) + off - (start == -2 ? n : 0)) + i;
-  const int page = pos >= 0 && pos < v.capacity() ? v.page(slot, pos / KV_PAGE) : -1;
-  float x[8];
-  if (page < 0) {
-    v.status[0] = 1;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = 0.f;
-  } else {
-    const unsigned char* b = v.block(page, head, pos % KV_PAGE / QKV_BLOCK);
-    const int at = pos % QKV_BLOCK;
-    const float scale = reinterpret_cast<const float*>(b + 2 * QKV_BLOCK * v.P)[blockIdx.y * QKV_BLOCK + at];
-    const uint2 u = *reinterpret_cast<const uint2*>(b + blockIdx.y * QKV_BLOCK * v.P + at * v.P + (((c >> 4) ^ qkv_turn(v.P / 16, at)) << 4) + (c & 15));
-#pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = qkv_value<SCHEME>((unsigned char)((e < 4 ? u.x : u.y) >> (8 * (e & 3)))) * scale;
+  constexpr int C = 16 / sizeof(O);
+  __shared__ long long s_block[RB];                          // of head 0, -1: none
+  __shared__ int s_at[RB];                                   // place in the block, -1: no row
+  const int row0 = blockIdx.x * RB, per = v.d / C, it = blockIdx.y * 256 + threadIdx.x;
+  pdl_wait();
+  if (threadIdx.x < RB) {
+    const int row = row0 + threadIdx.x;
+    int slot, i, n, at = -1;
+    long long block = -1;
+    if (row < step.M && step.row(v, row, &slot, &i, &n)) {
+      const int pos = (start >= 0 ? start : v.len(slot) + off - (start == -2 ? n : 0)) + i;
+      const int page = pos >= 0 && pos < v.capacity() ? v.page(slot, pos / KV_PAGE) : -1;
+      at = page < 0 ? 0 : pos % QKV_BLOCK;
+      if (page < 0) v.status[0] = 1;
+      else block = ((long long)page * v.KH * 2 + pos % KV_PAGE / QKV_BLOCK) * v.block_bytes();
+    }
+    s_block[threadIdx.x] = block;
+    s_at[threadIdx.x] = at;
   }
-  O* o = (blockIdx.y ? vals : k) + rh * v.d + c;
-  put_quad(o, make_float4(x[0], x[1], x[2], x[3]), vec);
-  put_quad(o + 4, make_float4(x[4], x[5], x[6], x[7]), vec);
+  __syncthreads();
+  if (it >= v.KH * per) return;
+  const int head = it / per, c = it % per * C;
+  const unsigned char* pool = v.pool + (long long)head * 2 * v.block_bytes();
+  uint2 u[RB];
+  float sc[RB];
+#pragma unroll
+  for (int r = 0; r < RB; ++r) {
+    const long long block = s_block[r];
+    const int at = s_at[r];
+    u[r] = make_uint2(SCHEME == QKV_I8 ? 0x80808080u : 0u, SCHEME == QKV_I8 ? 0x80808080u : 0u);
+    sc[r] = 0.f;
+    if (block < 0) continue;
+    const unsigned char* b = pool + block;
+    const unsigned char* p = b + (blockIdx.z * QKV_BLOCK + at) * v.P + (((c >> 4) ^ qkv_turn(v.P / 16, at)) << 4) + (c & 15);
+    if (C == 8) u[r] = *reinterpret_cast<const uint2*>(p);
+    else u[r].x = *reinterpret_cast<const unsigned*>(p);
+    sc[r] = reinterpret_cast<const float*>(b + 2 * QKV_BLOCK * v.P)[blockIdx.z * QKV_BLOCK + at];
+  }
+#pragma unroll
+  for (int r = 0; r < RB; ++r) {
+    if (s_at[r] < 0) continue;
+    O* o = (blockIdx.z ? vals : k) + ((long long)(row0 + r) * v.KH + head) * v.d + c;
+    float4 y[2];
+#pragma unroll
+    for (int h = 0; h < C / 4; ++h) {
+      const unsigned w = h ? u[r].y : u[r].x;
+      float4 x;
+      if (SCHEME == QKV_I8) {                                // a byte under the exponent of 2^23, less 2^23 + 128
+        const float off8 = 8388736.f;
+        x = make_float4(__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440)) - off8, __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7441)) - off8,
+                        __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7442)) - off8, __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7443)) - off8);
+      } else {
+        unsigned lo, hi;
+        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(lo) : "h"((unsigned short)w));
+        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(hi) : "h"((unsigned short)(w >> 16)));
+        const float2 p0 = __half22float2(*reinterpret_cast<const __half2*>(&lo)), p1 = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+        x = make_float4(p0.x, p0.y, p1.x, p1.y);
+      }
+      y[h] = scaled(x, sc[r]);
+    }
+    if (C == 8 && vec) {                                     // 16 bytes in one piece
+      const __nv_bfloat162 p[4] = {__floats2bfloat162_rn(y[0].x, y[0].y), __floats2bfloat162_rn(y[0].z, y[0].w), __floats2bfloat162_rn(y[1].x, y[1].y), __floats2bfloat162_rn(y[1].z, y[1].w)};
+      *reinterpret_cast<uint4*>(o) = *reinterpret_cast<const uint4*>(p);
+    } else {
+#pragma unroll
+      for (int h = 0; h < C / 4; ++h) put_quad(o + 4 * h, y[h], vec);
+    }
+  }
 }
 
 // A block per (sequence, head): the kept positions are read whole before any is written, so that they may overlap in any
@@ -146,6 +270,7 @@ __global__ void __launch_bounds__(256) qkv_commit_kernel(QkvView v, int n_new, c
   __shared__ __align__(16) unsigned char s_codes[QKV_MAX_DRAFT][2][256];
   __shared__ float s_scale[QKV_MAX_DRAFT][2];
   const int head = blockIdx.x, slot = blockIdx.y, tid = threadIdx.x, P = v.P, CH = P / 16;
+  pdl_wait();
   const int len = v.len(slot);
   int n = n_keep[slot] + keep_add;
   if (n < 0 || n > n_new || len + n > v.capacity()) {
@@ -192,6 +317,7 @@ __global__ void __launch_bounds__(256) qkv_commit_kernel(QkvView v, int n_new, c
 
 __global__ void set_lengths_kernel(int* __restrict__ lens, const int* __restrict__ from, int n) {
   const int i = blockIdx.x * 256 + threadIdx.x;
+  pdl_wait();
   if (i < n) lens[i] = from[i];
 }
 
@@ -312,7 +438,7 @@ int32_t vn_qkv_set_lengths(vn_qkv* c, const int32_t* lens, int32_t on_device) {
   VN_CHECK_QKV(c);
   VN_REQUIRE(c->ctx, lens, "lens is null");
   if (on_device) {
-    VN_LAUNCH(c->ctx, set_lengths_kernel, ceil_div(c->v.max_batch, 256), 256, 0, c->v.lens, lens, c->v.max_batch);
+    VN_LAUNCH_PDL_LEVEL(c->ctx, 1, "set_lengths_kernel", set_lengths_kernel, ceil_div(c->v.max_batch, 256), 256, 0, c->v.lens, lens, c->v.max_batch);
     return VN_OK;
   }
   for (int i = 0; i < c->v.max_batch; ++i)
@@ -358,11 +484,19 @@ int32_t vn_qkv_append(vn_qkv* c, const void* rows, int64_t ld, int32_t queries, 
   a.qn = q_norm; a.kn = k_norm; a.eps = eps;
   a.cs = cos_; a.sn = sin_; a.pairs = pairs; a.interleaved = interleaved; a.rope_rows = rope_rows;
   a.vec = aligned(rows, 4 * es) && aligned(q_out, 4 * es) && ld % 4 == 0;
-  const long long tasks = (long long)M * (a.H + 2 * c->v.KH);
-  VN_REQUIRE(c->ctx, tasks < (1ll << 33), "%d rows are too many for one call", M);
-  const dim3 grid((unsigned)ceil_div(tasks, 8ll)), block(32, 8);
-  if (es == 4) VN_LAUNCH_NAMED(c->ctx, "qkv_append_kernel", qkv_append_kernel<float>, grid, block, 0, a);
-  else VN_LAUNCH_NAMED(c->ctx, "qkv_append_kernel", qkv_append_kernel<bf16>, grid, block, 0, a);
+  a.vec_norm = aligned(q_norm, 16) && aligned(k_norm, 16);
+  a.vec_rope = pairs % 4 == 0 && aligned(cos_, 16) && aligned(sin_, 16);
+  const int units = a.H + 2 * c->v.KH, L = c->v.P <= 32 ? 8 : c->v.P <= 64 ? 16 : 32, tasks = ceil_div(units, 32 / L);
+  // a warp takes one task where there are few, so that all SMs have some; more, for fewer looks at lengths and angles, where there are many
+  int per = 1;
+  while (per < tasks && per < 16 && (long long)M * ceil_div(tasks, 2 * per) >= 128ll * c->ctx->sm_count) per *= 2;
+  const long long items = (long long)M * ceil_div(tasks, per);
+  VN_REQUIRE(c->ctx, items < (1ll << 32), "%d rows are too many for one call", M);
+  const unsigned grid = (unsigned)ceil_div(items, 8ll);
+#define APPEND(L, Y) do { if (es == 4) VN_LAUNCH_PDL_LEVEL(c->ctx, 1, "qkv_append_kernel", (qkv_append_kernel<float, L, Y>), grid, 256, 0, a, tasks, per); \
+                          else VN_LAUNCH_PDL_LEVEL(c->ctx, 1, "qkv_append_kernel", (qkv_append_kernel<bf16, L, Y>), grid, 256, 0, a, tasks, per); } while (0)
+  if (L == 8) APPEND(8, 1); else if (L == 16) APPEND(16, 1); else if (c->v.P <= 128) APPEND(32, 1); else APPEND(32, 2);
+#undef APPEND
   return VN_OK;
 }
 
@@ -377,14 +511,18 @@ int32_t vn_qkv_read(vn_qkv* c, int32_t n_ent, const int32_t* ents, const int32_t
   VN_REQUIRE(c->ctx, k_out && v_out, "null output");
   const int es = dtype == VN_F32 ? 4 : 2;
   VN_REQUIRE(c->ctx, aligned(k_out, es) && aligned(v_out, es), "outputs are not aligned to their values");
-  const int vec = aligned(k_out, 4 * es) && aligned(v_out, 4 * es);
-  const long long items = (long long)M * c->v.KH * (c->v.d / 8);
-  VN_REQUIRE(c->ctx, items < (1ll << 38), "%d rows are too many for one call", M);
-  const dim3 grid((unsigned)ceil_div(items, 256ll), 2);
-#define READ(O, S) VN_LAUNCH_NAMED(c->ctx, "qkv_read_kernel", (qkv_read_kernel<O, S>), grid, 256, 0, c->v, s, start, offset, (O*)k_out, (O*)v_out, vec)
+  const int vec = aligned(k_out, 16) && aligned(v_out, 16);
+  // rows of a CTA: more of them in flight for each thread where there are CTAs enough
+  const int y = ceil_div(c->v.KH * c->v.d * es / 16, 256);
+  const bool many = (long long)ceil_div(M, 8) * y >= 4ll * c->ctx->sm_count;
+  VN_REQUIRE(c->ctx, y <= 65535, "%d heads of %d", c->v.KH, c->v.d);
+  const dim3 grid(ceil_div(M, many ? 8 : 2), y, 2);
+#define READ2(O, S, RB) VN_LAUNCH_PDL_LEVEL(c->ctx, 1, "qkv_read_kernel", (qkv_read_kernel<O, S, RB>), grid, 256, 0, c->v, s, start, offset, (O*)k_out, (O*)v_out, vec)
+#define READ(O, S) do { if (many) READ2(O, S, 8); else READ2(O, S, 2); } while (0)
   if (c->v.scheme == QKV_I8) { if (es == 4) READ(float, QKV_I8); else READ(bf16, QKV_I8); }
   else { if (es == 4) READ(float, QKV_E4M3); else READ(bf16, QKV_E4M3); }
 #undef READ
+#undef READ2
   return VN_OK;
 }
 
@@ -393,7 +531,7 @@ int32_t vn_qkv_commit(vn_qkv* c, int32_t n_new, const int32_t* keep_idx, int32_t
   VN_REQUIRE(c->ctx, n_keep, "n_keep is null");
   VN_REQUIRE(c->ctx, n_new >= 0, "n_new %d", n_new);
   VN_REQUIRE(c->ctx, !keep_idx || (n_new <= QKV_MAX_DRAFT && stride >= 0), "rows are picked from at most %d, not %d", QKV_MAX_DRAFT, n_new);
-  VN_LAUNCH(c->ctx, qkv_commit_kernel, dim3(keep_idx ? c->v.KH : 1, c->v.max_batch), 256, 0, c->v, n_new, keep_idx, stride, n_keep, keep_add, c->tickets);
+  VN_LAUNCH_PDL_LEVEL(c->ctx, 1, "qkv_commit_kernel", qkv_commit_kernel, dim3(keep_idx ? c->v.KH : 1, c->v.max_batch), 256, 0, c->v, n_new, keep_idx, stride, n_keep, keep_add, c->tickets);
   return VN_OK;
 }
 

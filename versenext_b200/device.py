@@ -193,7 +193,7 @@ class DeviceArray:
     def __init__(self, ctx: Context, ptr: int, shape, dtype, owner=False, base=None):
         self.ctx = ctx
         self.ptr = int(ptr) if ptr else 0
-        self.shape = tuple(int(s) for s in shape)
+        self.shape = tuple(map(int, shape))
         self.dtype = np.dtype(dtype)
         self._owner = owner
         self._base = base  # keeps the owning buffer alive for views

@@ -12,6 +12,7 @@ bf16 rows are `np.uint16` arrays, the upper halves of float32 (a torch tensor's 
 from __future__ import annotations
 
 import ctypes as C
+import math
 from typing import Optional
 
 import numpy as np
@@ -37,7 +38,7 @@ def from_bf16(x) -> np.ndarray:
 
 
 def _ptr(a):
-    return a.ptr or None if a is not None else None
+    return None if a is None else a.ptr
 
 
 class Step:
@@ -108,6 +109,7 @@ class QuantKVCache:
         self.ctx, self.scheme, self.dtype = ctx, scheme, dtype
         self.max_batch, self.n_head, self.n_kv_head, self.head_dim = int(max_batch), int(n_head), int(n_kv_head), int(head_dim)
         self._code, self._np = _DTYPES[dtype]
+        self._lib, self._scale = ctx.lib, self.head_dim ** -0.5
         h = C.c_void_p()
         ctx._check(ctx.lib.vn_qkv_create(ctx.handle, self.max_batch, int(max_seq), self.n_head, self.n_kv_head, self.head_dim, scheme.encode(), self._code, int(pages),
                                          C.byref(h)))
@@ -168,17 +170,16 @@ class QuantKVCache:
 
     def _rows(self, shape, tail, step):
         """(entries, ents, row_ent, T, M) of rows of this shape, whose last axes are `tail`."""
-        lead = shape[:len(shape) - len(tail)]
-        if tuple(shape[len(lead):]) != tuple(tail):
+        k = len(shape) - len(tail)
+        lead = shape[:k]
+        if shape[k:] != tail or k < 0:
             raise ValueError(f"rows of shape {tuple(shape)} do not end in {tuple(tail)}")
         if step is not None:
-            m = 1
-            for n in lead:
-                m *= n
+            m = math.prod(lead)
             if m < step.rows:
                 raise ValueError(f"{m} rows for a step of {step.rows}")
             return step.entries, step.ents, step.row_ent, step.T, step.rows
-        if len(lead) != 2 or lead[0] > self.max_batch:
+        if k != 2 or lead[0] > self.max_batch:
             raise ValueError(f"rows of shape (sequences, rows, ..) with at most {self.max_batch} sequences, or a step, are needed")
         return lead[0], None, None, lead[1], lead[0] * lead[1]
 
@@ -207,12 +208,15 @@ class QuantKVCache:
     def _out(self, out, shape, dtype):
         if out is None:
             return self.ctx.empty(shape, dtype)
-        n = 1
-        for s in shape:
-            n *= s
-        if not isinstance(out, DeviceArray) or out.dtype != dtype or out.size < n:
+        if not isinstance(out, DeviceArray) or out.dtype != dtype or out.size < math.prod(shape):
             raise ValueError(f"out must be a device array of {np.dtype(dtype)} with room for {tuple(shape)}")
         return out
+
+    def _weight(self, a, name):
+        a = as_device(self.ctx, a, np.float32)
+        if a.shape != (self.head_dim,):
+            raise ValueError(f"{name} must have shape ({self.head_dim},)")
+        return a
 
     def append(self, rows, step: Optional[Step] = None, tree: Optional[Tree] = None, offset: int = 0, queries: bool = True, q_norm=None, k_norm=None, eps: float = 1e-6,
                rope=None, interleaved: bool = False, out: Optional[DeviceArray] = None) -> Optional[DeviceArray]:
@@ -223,32 +227,28 @@ class QuantKVCache:
         query / key head; rope: (cos, sin) tables (positions, pairs) for rotating the first 2 * pairs dimensions of queries and keys
         (half-split, or neighbours when `interleaved`).  Lengths stay: `commit` moves them."""
         x = self._in(rows)
-        H = self.n_head if queries else 0
-        width = (H + 2 * self.n_kv_head) * self.head_dim
+        H, d = self.n_head if queries else 0, self.head_dim
+        width = (H + 2 * self.n_kv_head) * d
         E, ents, row_ent, T, M = self._rows(x.shape, (width,), step)
         _, depth, per_row = self._tree(tree, step, T, M)
-        f32 = lambda a, name: self._table(a, (self.head_dim,), name)  # noqa: E731
-        qn = f32(q_norm, "q_norm") if q_norm is not None else None
-        kn = f32(k_norm, "k_norm") if k_norm is not None else None
+        qn = self._weight(q_norm, "q_norm") if q_norm is not None else None
+        kn = self._weight(k_norm, "k_norm") if k_norm is not None else None
         cs = sn = None
         pairs = rope_rows = 0
         if rope is not None:
-            cs, sn = (as_device(self.ctx, t, np.float32) for t in rope)
-            if cs.ndim != 2 or cs.shape != sn.shape or 2 * cs.shape[1] > self.head_dim:
-                raise ValueError(f"rope: two tables (positions, pairs) with at most {self.head_dim // 2} pairs are needed")
+            cs, sn = rope
+            cs, sn = as_device(self.ctx, cs, np.float32), as_device(self.ctx, sn, np.float32)
+            if cs.ndim != 2 or cs.shape != sn.shape or 2 * cs.shape[1] > d:
+                raise ValueError(f"rope: two tables (positions, pairs) with at most {d // 2} pairs are needed")
             rope_rows, pairs = cs.shape
             if pairs and rope_rows < self.max_seq:
                 raise ValueError(f"rope: tables of {rope_rows} positions for a cache of {self.max_seq}")
-        q = self._out(out, x.shape[:-1] + (H, self.head_dim), self._np) if queries else None
-        self.ctx._check(self.ctx.lib.vn_qkv_append(self.handle, _ptr(x), width, int(bool(queries)), E, ents, row_ent, T, M, int(offset), depth, per_row, _ptr(qn), _ptr(kn),
-                                                   float(eps), _ptr(cs), _ptr(sn), rope_rows, pairs, int(bool(interleaved)), _ptr(q)))
+        q = self._out(out, x.shape[:-1] + (H, d), self._np) if queries else None
+        st = self._lib.vn_qkv_append(self.handle, x.ptr, width, queries, E, ents, row_ent, T, M, offset, depth, per_row, _ptr(qn), _ptr(kn), eps, _ptr(cs), _ptr(sn),
+                                     rope_rows, pairs, interleaved, _ptr(q))
+        if st:
+            self.ctx._check(st)
         return q
-
-    def _table(self, a, shape, name):
-        a = as_device(self.ctx, a, np.float32)
-        if a.shape != shape:
-            raise ValueError(f"{name} must have shape {shape}")
-        return a
 
     def attention(self, q, step: Optional[Step] = None, tree: Optional[Tree] = None, window: int = 0, scale: Optional[float] = None, out: Optional[DeviceArray] = None) -> DeviceArray:
         """softmax(scale q k^T) v of a step's queries (.., n_head, head_dim) over the committed positions and the step's own rows, which
@@ -258,8 +258,9 @@ class QuantKVCache:
         E, ents, row_ent, T, M = self._rows(q.shape, (self.n_head, self.head_dim), step)
         seen, depth, per_row = self._tree(tree, step, T, M)
         out = self._out(out, q.shape, self._np)
-        self.ctx._check(self.ctx.lib.vn_qkv_attention(self.handle, _ptr(q), E, ents, row_ent, T, M, seen, depth, per_row, int(window),
-                                                      self.head_dim ** -0.5 if scale is None else float(scale), _ptr(out)))
+        st = self._lib.vn_qkv_attention(self.handle, q.ptr, E, ents, row_ent, T, M, seen, depth, per_row, window, self._scale if scale is None else scale, out.ptr)
+        if st:
+            self.ctx._check(st)
         return out
 
     def commit(self, n_new: int, n_keep, keep_idx=None, keep_add: int = 0):
@@ -274,7 +275,9 @@ class QuantKVCache:
             if ki.ndim != 2 or ki.shape[0] < self.max_batch or ki.shape[1] < n_new:
                 raise ValueError(f"keep_idx must have shape ({self.max_batch}, {n_new})")
             stride = ki.shape[-1]
-        self.ctx._check(self.ctx.lib.vn_qkv_commit(self.handle, int(n_new), _ptr(ki), stride, _ptr(nk), int(keep_add)))
+        st = self._lib.vn_qkv_commit(self.handle, n_new, _ptr(ki), stride, nk.ptr, keep_add)
+        if st:
+            self.ctx._check(st)
 
     def read(self, step, start: Optional[int] = None, offset: int = 0, back: bool = False, dtype: Optional[str] = None, out=None):
         """(k, v) values (rows, n_kv_head, head_dim) of a step's positions, as `dtype` (the cache's unless given): positions start .. of every
@@ -290,12 +293,15 @@ class QuantKVCache:
             ents, row_ent, M, lead = None, None, E * T, (E, T)
         if start is not None and (back or start < 0):
             raise ValueError("start is a position, and excludes `back`")
-        if (dtype or self.dtype) not in _DTYPES:
+        if dtype is not None and dtype not in _DTYPES:
             raise ValueError(f"unknown dtype {dtype!r}, expected one of {tuple(_DTYPES)}")
         code, kind = _DTYPES[dtype or self.dtype]
         shape = lead + (self.n_kv_head, self.head_dim)
-        k, v = (self._out(o, shape, kind) for o in (out if out is not None else (None, None)))
-        self.ctx._check(self.ctx.lib.vn_qkv_read(self.handle, E, ents, row_ent, T, M, -2 if back else -1 if start is None else int(start), int(offset), code, _ptr(k), _ptr(v)))
+        k, v = out if out is not None else (None, None)
+        k, v = self._out(k, shape, kind), self._out(v, shape, kind)
+        st = self._lib.vn_qkv_read(self.handle, E, ents, row_ent, T, M, -2 if back else -1 if start is None else start, offset, code, k.ptr, v.ptr)
+        if st:
+            self.ctx._check(st)
         return k, v
 
     def get(self, seq_idx: int = 0, n_positions: Optional[int] = None):
