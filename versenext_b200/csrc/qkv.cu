@@ -1,6 +1,7 @@
 // The paged 8-bit cache's entry points and the kernels that write, read and keep positions; attention is in qkv_attn.cuh.
 #include <string.h>
 
+#include <algorithm>
 #include <new>
 
 #include "qkv.cuh"
@@ -23,48 +24,108 @@ struct AppendArgs {
   int vec = 0, vec_norm = 0, vec_rope = 0;            // rows, norms' weights, rotation in whole quads
 };
 
-template <typename T> __device__ __forceinline__ float4 quad_of(const T* p, bool vec) {
-  if (vec) return load4(p);
-  return make_float4(to_f<T>(p[0]), to_f<T>(p[1]), to_f<T>(p[2]), to_f<T>(p[3]));
-}
 template <typename T> __device__ __forceinline__ void put_quad(T* p, float4 v, bool vec) {
   if (vec) { store4(p, v); return; }
   p[0] = from_f<T>(v.x); p[1] = from_f<T>(v.y); p[2] = from_f<T>(v.z); p[3] = from_f<T>(v.w);
 }
 
-__device__ __forceinline__ unsigned char code_of(float y, int scheme) {
-  if (scheme == QKV_I8) return (unsigned char)(max(-127, min(127, __float2int_rn(y))) + 128);
-  unsigned short r;
-  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(0.f), "f"(y));
-  return (unsigned char)r;
+// x / s to nearest: Markstein's correction (IBM J. Res. Dev. 34, 1990) of the product with 1 / s by its remainder, which is exact while it is
+// a normal number; so small heads are made larger by a power of two first
+struct Quotient {
+  float up, s, r;
+  __device__ __forceinline__ explicit Quotient(float scale) : up(scale < 1e-24f ? 1.8446744e19f : 1.f), s(scale * up), r(1.f / s) {}
+  __device__ __forceinline__ float of(float x) const {
+    const float v = x * up, y = v * r;
+    return fmaf(fmaf(-y, s, v), r, y);
+  }
+};
+
+// four codes of a head, x / scale to nearest even
+template <int SCHEME> __device__ __forceinline__ unsigned codes_of(float4 x, const Quotient& q) {
+  const float4 y = make_float4(q.of(x.x), q.of(x.y), q.of(x.z), q.of(x.w));
+  if (SCHEME == QKV_I8) {
+    // |y| is below 127.5: the sum with 1.5 2^23 is rounded to a whole number, whose low byte, plus 128, is the code
+    auto c = [](float v) { return __float_as_uint(fminf(fmaxf(v, -127.f), 127.f) + 12582912.f); };
+    return __byte_perm(__byte_perm(c(y.x), c(y.y), 0x0040), __byte_perm(c(y.z), c(y.w), 0x0040), 0x5410) ^ 0x80808080u;
+  }
+  unsigned short lo, hi;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(y.y), "f"(y.x));
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(y.w), "f"(y.z));
+  return (unsigned)hi << 16 | lo;
 }
 
-__device__ __forceinline__ float4 quad_at(const float* p, bool vec) { return vec ? load4(p) : make_float4(p[0], p[1], p[2], p[3]); }
+// eight neighbouring channels of a row, as they stand in memory; whole: in 16-byte pieces
+template <typename T> struct Eight;
+template <> struct Eight<float> {
+  float v[8];
+  __device__ __forceinline__ void load(const float* p, bool whole) {
+    if (whole) {
+      const float4 x = load4(p), y = load4(p + 4);
+      v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w; v[4] = y.x; v[5] = y.y; v[6] = y.z; v[7] = y.w;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = p[e];
+    }
+  }
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = 0.f;
+  }
+  __device__ __forceinline__ void get(float (&x)[8]) const {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = v[e];
+  }
+};
+template <> struct Eight<bf16> {
+  uint4 u;
+  __device__ __forceinline__ void load(const bf16* p, bool whole) {
+    if (whole) { u = *reinterpret_cast<const uint4*>(p); return; }
+    const unsigned short* h = reinterpret_cast<const unsigned short*>(p);
+    u = make_uint4(h[0] | (unsigned)h[1] << 16, h[2] | (unsigned)h[3] << 16, h[4] | (unsigned)h[5] << 16, h[6] | (unsigned)h[7] << 16);
+  }
+  __device__ __forceinline__ void zero() { u = make_uint4(0u, 0u, 0u, 0u); }
+  __device__ __forceinline__ void get(float (&x)[8]) const {
+    const unsigned w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) { x[2 * e] = __uint_as_float(w[e] << 16); x[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u); }
+  }
+};
+__device__ __forceinline__ void put_eight(float* p, const float (&x)[8], bool whole) {
+  put_quad(p, make_float4(x[0], x[1], x[2], x[3]), whole);
+  put_quad(p + 4, make_float4(x[4], x[5], x[6], x[7]), whole);
+}
+__device__ __forceinline__ void put_eight(bf16* p, const float (&x)[8], bool whole) {
+  if (!whole) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) p[e] = __float2bfloat16_rn(x[e]);
+    return;
+  }
+  const __nv_bfloat162 h[4] = {__floats2bfloat162_rn(x[0], x[1]), __floats2bfloat162_rn(x[2], x[3]), __floats2bfloat162_rn(x[4], x[5]), __floats2bfloat162_rn(x[6], x[7])};
+  *reinterpret_cast<uint4*>(p) = *reinterpret_cast<const uint4*>(h);
+}
 
-// A warp takes `per` tasks of a row, four asked for at a time: a task is 32 / L neighbouring heads, whose L lanes hold Y quads of channels
-// each (lane, lane + 32).  Heads pass through shared memory only for half-split rotation, where a quad meets the one pairs further on.
-// What bounds it: the rows' bytes for many rows; for few, the chain entry, length, page, store (the row's values are asked for first).
-// grid ceil(M ceil(tasks / per) / 8), block 256
-template <typename T, int L, int Y>
-__global__ void __launch_bounds__(256) qkv_append_kernel(AppendArgs a, int tasks, int per) {
-  constexpr int HPW = 32 / L, IN = Y > 1 ? 2 : 4;
-  __shared__ __align__(16) float s_head[8][HPW][4 * L * Y];
-  const int lane = threadIdx.x & 31, l = lane % L, sub = lane / L, warp = threadIdx.x >> 5;
+// A warp takes `per` tasks of a row, four asked for at a time: a task is 32 / L neighbouring heads, whose lanes hold eight channels each.
+// Heads pass through shared memory only for half-split rotation, where a channel meets the one `pairs` further on.  Bound by
+// instructions for many rows (with four channels a lane a prompt of 8000 rows of 2048 values took 48 us, twice as long); for few, the
+// chain entry, length, page, store (the row's values are asked for first).  grid ceil(M ceil(tasks / per) / 8), block 256
+template <typename T, int SCHEME, int L>
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2) qkv_append_kernel(AppendArgs a, int tasks, int per) {
+  constexpr int HPW = 32 / L, IN = 4;
+  __shared__ __align__(16) float s_head[8][HPW][8 * L];
+  const int lane = threadIdx.x & 31, c = lane % L * 8, sub = lane / L, warp = threadIdx.x >> 5;
   const int units = a.H + 2 * a.v.KH, d = a.v.d, P = a.v.P, slices = (tasks + per - 1) / per;
   const unsigned item = blockIdx.x * 8u + warp;
   pdl_wait();
   const int row = (int)(item / (unsigned)slices), first = (int)(item % (unsigned)slices) * per, last = min(tasks, first + per);
   if (row >= a.step.M) return;
   const T* xr = reinterpret_cast<const T*>(a.x) + row * a.ld;
-  float4 x[IN][Y];
+  Eight<T> x[IN];
   auto ask = [&](int task) {
 #pragma unroll
-    for (int k = 0; k < IN; ++k)
-#pragma unroll
-      for (int y = 0; y < Y; ++y) {
-        const int unit = (task + k) * HPW + sub, c = 4 * l + 128 * y;
-        x[k][y] = task + k < last && unit < units && c < d ? quad_of(xr + (long long)unit * d + c, a.vec) : make_float4(0.f, 0.f, 0.f, 0.f);
-      }
+    for (int k = 0; k < IN; ++k) {
+      const int unit = (task + k) * HPW + sub;
+      if (task + k < last && unit < units && c < d) x[k].load(xr + unit * d + c, a.vec); else x[k].zero();
+    }
   };
   ask(first);
   int slot, i, n;
@@ -72,29 +133,30 @@ __global__ void __launch_bounds__(256) qkv_append_kernel(AppendArgs a, int tasks
   const int len = a.v.len(slot), pos = len + a.off + i;
   const int turn = min(max(len + a.off + a.tree.away(row, i), 0), a.rope_rows - 1);
   const int page = pos >= 0 && pos < a.v.capacity() ? a.v.page(slot, pos / KV_PAGE) : -1, at = pos % QKV_BLOCK;
-  // what a quad is turned by: half-split, quads of the two halves by the same angles
-  float4 cs[Y], sn[Y];
-  bool turned[Y];
-#pragma unroll
-  for (int y = 0; y < Y; ++y) {
-    const int c = 4 * l + 128 * y, np = a.pairs;
-    turned[y] = np && c < 2 * np;
-    cs[y] = make_float4(1.f, 1.f, 1.f, 1.f);
-    sn[y] = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (!turned[y]) continue;
+  unsigned char* base = a.v.block(max(page, 0), 0, pos % KV_PAGE / QKV_BLOCK);
+  const int to = at * P + (((c >> 4) ^ qkv_turn(P / 16, at)) << 4) + (c & 15), head_bytes = 2 * a.v.block_bytes(), np = a.pairs;
+  // what the channels are turned by: half-split, those of the two halves by the same angles
+  float cs[8], sn[8];
+  const bool turned = c < 2 * np;
+  if (turned) {
     const float *pc = a.cs + (long long)turn * np, *ps = a.sn + (long long)turn * np;
-    if (a.interleaved) {
-      const bool two = c + 2 < 2 * np;
-      cs[y].x = cs[y].y = pc[c / 2]; sn[y].x = sn[y].y = ps[c / 2];
-      if (two) { cs[y].z = cs[y].w = pc[c / 2 + 1]; sn[y].z = sn[y].w = ps[c / 2 + 1]; }
-    } else if (a.vec_rope) {
-      cs[y] = load4(pc + (c < np ? c : c - np)); sn[y] = load4(ps + (c < np ? c : c - np));
+    if (a.vec_rope && !a.interleaved) {
+      const int p = c < np ? c : c - np;
+      const float4 u = load4(pc + p), v = load4(pc + p + 4), w = load4(ps + p), y = load4(ps + p + 4);
+      cs[0] = u.x; cs[1] = u.y; cs[2] = u.z; cs[3] = u.w; cs[4] = v.x; cs[5] = v.y; cs[6] = v.z; cs[7] = v.w;
+      sn[0] = w.x; sn[1] = w.y; sn[2] = w.z; sn[3] = w.w; sn[4] = y.x; sn[5] = y.y; sn[6] = y.z; sn[7] = y.w;
     } else {
-      auto angle = [&](int e, float& u, float& w) {
-        if (c + e < 2 * np) { const int p = c + e < np ? c + e : c + e - np; u = pc[p]; w = ps[p]; }
-      };
-      angle(0, cs[y].x, sn[y].x); angle(1, cs[y].y, sn[y].y); angle(2, cs[y].z, sn[y].z); angle(3, cs[y].w, sn[y].w);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const bool in = c + e < 2 * np;
+        const int p = !in ? 0 : a.interleaved ? (c + e) / 2 : c + e < np ? c + e : c + e - np;
+        cs[e] = in ? pc[p] : 1.f;
+        sn[e] = in ? ps[p] : 0.f;
+      }
     }
+    if (!a.interleaved)                                      // the sign that the other half's values enter with
+#pragma unroll
+      for (int e = 0; e < 8; ++e) sn[e] = c + e < np ? -sn[e] : sn[e];
   }
   float* s = s_head[warp][sub];
 #pragma unroll 1
@@ -105,160 +167,142 @@ __global__ void __launch_bounds__(256) qkv_append_kernel(AppendArgs a, int tasks
       if (task + k >= last) break;
       const int unit = (task + k) * HPW + sub;
       const bool live = unit < units, is_q = unit < a.H, is_v = unit >= a.H + a.v.KH;
-      float4 v[Y];
-#pragma unroll
-      for (int y = 0; y < Y; ++y) v[y] = x[k][y];
-      const float* w = is_v || !live ? nullptr : is_q ? a.qn : a.kn;
-      if (__any_sync(0xffffffffu, w != nullptr)) {           // a warp's heads may be of two kinds
+      float v[8];
+      x[k].get(v);
+      if (a.qn || a.kn) {
+        const float* w = is_v || !live ? nullptr : is_q ? a.qn : a.kn;
         float ss = 0.f;
 #pragma unroll
-        for (int y = 0; y < Y; ++y) ss += v[y].x * v[y].x + v[y].y * v[y].y + v[y].z * v[y].z + v[y].w * v[y].w;
+        for (int e = 0; e < 8; ++e) ss = fmaf(v[e], v[e], ss);
 #pragma unroll
         for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-        if (w) {
-          const float r = sqrtf(ss / (float)d + a.eps);
+        if (w && c < d) {
+          const float r = 1.f / sqrtf(ss / (float)d + a.eps);
+          Eight<float> g;
+          g.load(w + c, a.vec_norm);
 #pragma unroll
-          for (int y = 0; y < Y; ++y) {
-            const int c = 4 * l + 128 * y;
-            if (c >= d) break;
-            const float4 g = quad_at(w + c, a.vec_norm);
-            v[y] = make_float4(v[y].x / r * g.x, v[y].y / r * g.y, v[y].z / r * g.z, v[y].w / r * g.w);
-          }
+          for (int e = 0; e < 8; ++e) v[e] = v[e] * r * g.v[e];
         }
       }
-      if (a.pairs && a.interleaved) {
-        if (!is_v)
+      if (np && a.interleaved) {
+        if (!is_v && turned)
 #pragma unroll
-          for (int y = 0; y < Y; ++y)
-            v[y] = make_float4(v[y].x * cs[y].x - v[y].y * sn[y].x, v[y].y * cs[y].x + v[y].x * sn[y].x, v[y].z * cs[y].z - v[y].w * sn[y].z, v[y].w * cs[y].z + v[y].z * sn[y].z);
-      } else if (a.pairs) {
+          for (int e = 0; e < 8; e += 2) {
+            const float y = v[e] * cs[e] - v[e + 1] * sn[e], z = v[e + 1] * cs[e] + v[e] * sn[e];
+            v[e] = y; v[e + 1] = z;
+          }
+      } else if (np && (task + k) * HPW < a.H + a.v.KH) {    // a task with queries or keys
         __syncwarp();
-#pragma unroll
-        for (int y = 0; y < Y; ++y) *reinterpret_cast<float4*>(s + 4 * l + 128 * y) = v[y];
+        put_eight(s + c, v, true);
         __syncwarp();
-#pragma unroll
-        for (int y = 0; y < Y; ++y) {
-          const int c = 4 * l + 128 * y, np = a.pairs;
-          if (is_v || !turned[y]) continue;
-          // the other half's values, with the sign that they enter with
-          auto other = [&](int e) { return c + e < np ? -s[c + e + np] : c + e < 2 * np ? s[c + e - np] : 0.f; };
-          float4 t;
+        if (!is_v && turned) {
+          float t[8];
           if (a.vec_rope) {
-            t = *reinterpret_cast<const float4*>(s + (c < np ? c + np : c - np));
-            if (c < np) t = make_float4(-t.x, -t.y, -t.z, -t.w);
+            Eight<float> g;
+            g.load(s + (c < np ? c + np : c - np), true);
+            g.get(t);
           } else {
-            t = make_float4(other(0), other(1), other(2), other(3));
+#pragma unroll
+            for (int e = 0; e < 8; ++e) t[e] = c + e < np ? s[c + e + np] : c + e < 2 * np ? s[c + e - np] : 0.f;
           }
-          v[y] = make_float4(v[y].x * cs[y].x + t.x * sn[y].x, v[y].y * cs[y].y + t.y * sn[y].y, v[y].z * cs[y].z + t.z * sn[y].z, v[y].w * cs[y].w + t.w * sn[y].w);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] = v[e] * cs[e] + t[e] * sn[e];
         }
       }
-      if (live && is_q) {
-        T* o = reinterpret_cast<T*>(a.q) + ((long long)row * a.H + unit) * d;
-#pragma unroll
-        for (int y = 0; y < Y; ++y)
-          if (4 * l + 128 * y < d) put_quad(o + 4 * l + 128 * y, v[y], a.vec);
-      }
-      if (__all_sync(0xffffffffu, !live || is_q)) continue;
+      if (live && is_q && c < d) put_eight(reinterpret_cast<T*>(a.q) + ((long long)row * a.H + unit) * d + c, v, a.vec);
+      if ((task + k + 1) * HPW <= a.H) continue;             // queries only
       // ---- a head of the cache
       unsigned top = 0;                                      // magnitudes as bits: what is not finite is above all others
 #pragma unroll
-      for (int y = 0; y < Y; ++y)
-        top = max(top, max(max(__float_as_uint(v[y].x) & 0x7fffffffu, __float_as_uint(v[y].y) & 0x7fffffffu),
-                           max(__float_as_uint(v[y].z) & 0x7fffffffu, __float_as_uint(v[y].w) & 0x7fffffffu)));
+      for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(v[e]) & 0x7fffffffu);
 #pragma unroll
       for (int o = L / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
       if (!live || is_q) continue;
-      if (page < 0) { if (l == 0) a.v.status[0] = 1; continue; }
+      if (page < 0) { a.v.status[0] = 1; continue; }
       const bool bad = top >= 0x7f800000u;
-      const float scale = fmaxf((top ? __uint_as_float(top) : 1.f) / (a.v.scheme == QKV_I8 ? 127.f : 448.f), QKV_SCALE_MIN);
-      const int head = unit - a.H - (is_v ? a.v.KH : 0), t = qkv_turn(P / 16, at);
-      unsigned char* b = a.v.block(page, head, pos % KV_PAGE / QKV_BLOCK);
-      unsigned char* codes = b + (is_v ? QKV_BLOCK * P : 0) + at * P;
-#pragma unroll
-      for (int y = 0; y < Y; ++y) {
-        const int c = 4 * l + 128 * y;
-        if (c >= P) break;
-        const unsigned char none = a.v.scheme == QKV_I8 ? 128 : 0;
-        uchar4 q = make_uchar4(none, none, none, none);
-        if (c < d && !bad) q = make_uchar4(code_of(v[y].x / scale, a.v.scheme), code_of(v[y].y / scale, a.v.scheme), code_of(v[y].z / scale, a.v.scheme), code_of(v[y].w / scale, a.v.scheme));
-        *reinterpret_cast<uchar4*>(codes + (((c >> 4) ^ t) << 4) + (c & 15)) = q;
+      const float scale = fmaxf((top ? __uint_as_float(top) : 1.f) / (SCHEME == QKV_I8 ? 127.f : 448.f), QKV_SCALE_MIN);
+      const Quotient by(scale);
+      unsigned char* b = base + (long long)(unit - a.H - (is_v ? a.v.KH : 0)) * head_bytes;
+      if (c < P) {
+        uint2 q = make_uint2(SCHEME == QKV_I8 ? 0x80808080u : 0u, SCHEME == QKV_I8 ? 0x80808080u : 0u);
+        if (c < d && !bad) q = make_uint2(codes_of<SCHEME>(make_float4(v[0], v[1], v[2], v[3]), by), codes_of<SCHEME>(make_float4(v[4], v[5], v[6], v[7]), by));
+        *reinterpret_cast<uint2*>(b + (is_v ? QKV_BLOCK * P : 0) + to) = q;
       }
-      if (l == 0) reinterpret_cast<float*>(b + 2 * QKV_BLOCK * P)[(is_v ? QKV_BLOCK : 0) + at] = bad ? CUDART_NAN_F : scale;
+      if (c == 0) reinterpret_cast<float*>(b + 2 * QKV_BLOCK * P)[(is_v ? QKV_BLOCK : 0) + at] = bad ? CUDART_NAN_F : scale;
     }
   }
 }
 
-// A thread takes 16 bytes of results (C channels of a head) of RB neighbouring rows, all asked for before any is converted; the rows'
-// blocks are found by the first threads.  Bound by the bytes of codes and results.
-// grid (ceil(M / RB), ceil(KH d / C / 256), 2), block 256
+// A warp takes RB neighbouring rows of 32 pieces of 16 bytes of results (C channels of a head), keys and values, all asked for before any is
+// converted; its first lanes find the rows' blocks (entry, length, page: three loads one after another, which other warps fill).
+// Bound by the bytes of codes and results.  grid ceil(ceil(M / RB) slices / 8), block 256
 template <typename O, int SCHEME, int RB>
-__global__ void __launch_bounds__(256) qkv_read_kernel(QkvView v, QkvStep step, int start, int off, O* __restrict__ k, O* __restrict__ vals, int vec) {
+__global__ void __launch_bounds__(256) qkv_read_kernel(QkvView v, QkvStep step, int start, int off, O* __restrict__ k, O* __restrict__ vals, int vec, int slices) {
   constexpr int C = 16 / sizeof(O);
-  __shared__ long long s_block[RB];                          // of head 0, -1: none
-  __shared__ int s_at[RB];                                   // place in the block, -1: no row
-  const int row0 = blockIdx.x * RB, per = v.d / C, it = blockIdx.y * 256 + threadIdx.x;
+  const unsigned item = blockIdx.x * 8u + (threadIdx.x >> 5);
+  const int lane = threadIdx.x & 31, per = v.d / C, row0 = (int)(item / (unsigned)slices) * RB, it = (int)(item % (unsigned)slices) * 32 + lane;
+  if (row0 >= step.M) return;
   pdl_wait();
-  if (threadIdx.x < RB) {
-    const int row = row0 + threadIdx.x;
-    int slot, i, n, at = -1;
-    long long block = -1;
-    if (row < step.M && step.row(v, row, &slot, &i, &n)) {
+  int own_at = -1;                                           // of row row0 + lane: place in its block, -1: no row
+  long long own_block = -1;                                  // of head 0, -1: none
+  if (lane < RB && row0 + lane < step.M) {
+    int slot, i, n;
+    if (step.row(v, row0 + lane, &slot, &i, &n)) {
       const int pos = (start >= 0 ? start : v.len(slot) + off - (start == -2 ? n : 0)) + i;
       const int page = pos >= 0 && pos < v.capacity() ? v.page(slot, pos / KV_PAGE) : -1;
-      at = page < 0 ? 0 : pos % QKV_BLOCK;
+      own_at = page < 0 ? 0 : pos % QKV_BLOCK;
       if (page < 0) v.status[0] = 1;
-      else block = ((long long)page * v.KH * 2 + pos % KV_PAGE / QKV_BLOCK) * v.block_bytes();
+      else own_block = ((long long)page * v.KH * 2 + pos % KV_PAGE / QKV_BLOCK) * v.block_bytes();
     }
-    s_block[threadIdx.x] = block;
-    s_at[threadIdx.x] = at;
   }
-  __syncthreads();
-  if (it >= v.KH * per) return;
-  const int head = it / per, c = it % per * C;
+  const int head = it / per, c = it % per * C, CH = v.P / 16, scales = 2 * QKV_BLOCK * v.P;
+  const bool reads = it < v.KH * per;
   const unsigned char* pool = v.pool + (long long)head * 2 * v.block_bytes();
-  uint2 u[RB];
-  float sc[RB];
+  uint2 u[RB][2];
+  float sc[RB][2];
 #pragma unroll
   for (int r = 0; r < RB; ++r) {
-    const long long block = s_block[r];
-    const int at = s_at[r];
-    u[r] = make_uint2(SCHEME == QKV_I8 ? 0x80808080u : 0u, SCHEME == QKV_I8 ? 0x80808080u : 0u);
-    sc[r] = 0.f;
-    if (block < 0) continue;
+    const long long block = __shfl_sync(0xffffffffu, own_block, r);
+    const int at = __shfl_sync(0xffffffffu, own_at, r);
+#pragma unroll
+    for (int w = 0; w < 2; ++w) { u[r][w] = make_uint2(0u, 0u); sc[r][w] = 0.f; }          // no page: zeros
+    if (!reads || block < 0) continue;
     const unsigned char* b = pool + block;
-    const unsigned char* p = b + (blockIdx.z * QKV_BLOCK + at) * v.P + (((c >> 4) ^ qkv_turn(v.P / 16, at)) << 4) + (c & 15);
-    if (C == 8) u[r] = *reinterpret_cast<const uint2*>(p);
-    else u[r].x = *reinterpret_cast<const unsigned*>(p);
-    sc[r] = reinterpret_cast<const float*>(b + 2 * QKV_BLOCK * v.P)[blockIdx.z * QKV_BLOCK + at];
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      const unsigned char* p = b + (w * QKV_BLOCK + at) * v.P + (((c >> 4) ^ qkv_turn(CH, at)) << 4) + (c & 15);
+      if (C == 8) u[r][w] = __ldcs(reinterpret_cast<const uint2*>(p));
+      else u[r][w].x = __ldcs(reinterpret_cast<const unsigned*>(p));
+      sc[r][w] = reinterpret_cast<const float*>(b + scales)[w * QKV_BLOCK + at];
+    }
   }
 #pragma unroll
   for (int r = 0; r < RB; ++r) {
-    if (s_at[r] < 0) continue;
-    O* o = (blockIdx.z ? vals : k) + ((long long)(row0 + r) * v.KH + head) * v.d + c;
-    float4 y[2];
+    if (__shfl_sync(0xffffffffu, own_at, r) < 0 || !reads) continue;
 #pragma unroll
-    for (int h = 0; h < C / 4; ++h) {
-      const unsigned w = h ? u[r].y : u[r].x;
-      float4 x;
-      if (SCHEME == QKV_I8) {                                // a byte under the exponent of 2^23, less 2^23 + 128
-        const float off8 = 8388736.f;
-        x = make_float4(__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440)) - off8, __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7441)) - off8,
-                        __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7442)) - off8, __uint_as_float(__byte_perm(w, 0x4b000000u, 0x7443)) - off8);
-      } else {
-        unsigned lo, hi;
-        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(lo) : "h"((unsigned short)w));
-        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(hi) : "h"((unsigned short)(w >> 16)));
-        const float2 p0 = __half22float2(*reinterpret_cast<const __half2*>(&lo)), p1 = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-        x = make_float4(p0.x, p0.y, p1.x, p1.y);
+    for (int w = 0; w < 2; ++w) {
+      O* out = (w ? vals : k) + ((long long)(row0 + r) * v.KH + head) * v.d + c;
+      float y[8];
+#pragma unroll
+      for (int h = 0; h < C / 4; ++h) {
+        const unsigned q = h ? u[r][w].y : u[r][w].x;
+        float4 x;
+        if (SCHEME == QKV_I8) {                              // a byte under the exponent of 2^23, less 2^23 + 128
+          const float over = 8388736.f;
+          x = make_float4(__uint_as_float(__byte_perm(q, 0x4b000000u, 0x7440)) - over, __uint_as_float(__byte_perm(q, 0x4b000000u, 0x7441)) - over,
+                          __uint_as_float(__byte_perm(q, 0x4b000000u, 0x7442)) - over, __uint_as_float(__byte_perm(q, 0x4b000000u, 0x7443)) - over);
+        } else {
+          unsigned lo, hi;
+          asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(lo) : "h"((unsigned short)q));
+          asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(hi) : "h"((unsigned short)(q >> 16)));
+          const float2 p0 = __half22float2(*reinterpret_cast<const __half2*>(&lo)), p1 = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+          x = make_float4(p0.x, p0.y, p1.x, p1.y);
+        }
+        x = scaled(x, sc[r][w]);
+        y[4 * h] = x.x; y[4 * h + 1] = x.y; y[4 * h + 2] = x.z; y[4 * h + 3] = x.w;
       }
-      y[h] = scaled(x, sc[r]);
-    }
-    if (C == 8 && vec) {                                     // 16 bytes in one piece
-      const __nv_bfloat162 p[4] = {__floats2bfloat162_rn(y[0].x, y[0].y), __floats2bfloat162_rn(y[0].z, y[0].w), __floats2bfloat162_rn(y[1].x, y[1].y), __floats2bfloat162_rn(y[1].z, y[1].w)};
-      *reinterpret_cast<uint4*>(o) = *reinterpret_cast<const uint4*>(p);
-    } else {
-#pragma unroll
-      for (int h = 0; h < C / 4; ++h) put_quad(o + 4 * h, y[h], vec);
+      if constexpr (C == 8) put_eight(out, y, vec);
+      else put_quad(out, make_float4(y[0], y[1], y[2], y[3]), vec);
     }
   }
 }
@@ -483,19 +527,21 @@ int32_t vn_qkv_append(vn_qkv* c, const void* rows, int64_t ld, int32_t queries, 
   a.x = rows; a.q = q_out; a.ld = ld; a.off = offset;
   a.qn = q_norm; a.kn = k_norm; a.eps = eps;
   a.cs = cos_; a.sn = sin_; a.pairs = pairs; a.interleaved = interleaved; a.rope_rows = rope_rows;
-  a.vec = aligned(rows, 4 * es) && aligned(q_out, 4 * es) && ld % 4 == 0;
+  a.vec = aligned(rows, 16) && aligned(q_out, 16) && ld * es % 16 == 0;
   a.vec_norm = aligned(q_norm, 16) && aligned(k_norm, 16);
-  a.vec_rope = pairs % 4 == 0 && aligned(cos_, 16) && aligned(sin_, 16);
-  const int units = a.H + 2 * c->v.KH, L = c->v.P <= 32 ? 8 : c->v.P <= 64 ? 16 : 32, tasks = ceil_div(units, 32 / L);
+  a.vec_rope = pairs % 8 == 0 && aligned(cos_, 16) && aligned(sin_, 16);
+  const int units = a.H + 2 * c->v.KH, L = c->v.P <= 32 ? 4 : c->v.P <= 64 ? 8 : c->v.P <= 128 ? 16 : 32, tasks = ceil_div(units, 32 / L);
   // a warp takes one task where there are few, so that all SMs have some; more, for fewer looks at lengths and angles, where there are many
   int per = 1;
   while (per < tasks && per < 16 && (long long)M * ceil_div(tasks, 2 * per) >= 128ll * c->ctx->sm_count) per *= 2;
   const long long items = (long long)M * ceil_div(tasks, per);
   VN_REQUIRE(c->ctx, items < (1ll << 32), "%d rows are too many for one call", M);
   const unsigned grid = (unsigned)ceil_div(items, 8ll);
-#define APPEND(L, Y) do { if (es == 4) VN_LAUNCH_PDL_LEVEL(c->ctx, 1, "qkv_append_kernel", (qkv_append_kernel<float, L, Y>), grid, 256, 0, a, tasks, per); \
-                          else VN_LAUNCH_PDL_LEVEL(c->ctx, 1, "qkv_append_kernel", (qkv_append_kernel<bf16, L, Y>), grid, 256, 0, a, tasks, per); } while (0)
-  if (L == 8) APPEND(8, 1); else if (L == 16) APPEND(16, 1); else if (c->v.P <= 128) APPEND(32, 1); else APPEND(32, 2);
+#define APPEND(S, L) do { if (es == 4) VN_LAUNCH_PDL_LEVEL(c->ctx, 1, "qkv_append_kernel", (qkv_append_kernel<float, S, L>), grid, 256, 0, a, tasks, per); \
+                          else VN_LAUNCH_PDL_LEVEL(c->ctx, 1, "qkv_append_kernel", (qkv_append_kernel<bf16, S, L>), grid, 256, 0, a, tasks, per); } while (0)
+#define APPEND_ALL(S) do { if (L == 4) APPEND(S, 4); else if (L == 8) APPEND(S, 8); else if (L == 16) APPEND(S, 16); else APPEND(S, 32); } while (0)
+  if (c->v.scheme == QKV_I8) APPEND_ALL(QKV_I8); else APPEND_ALL(QKV_E4M3);
+#undef APPEND_ALL
 #undef APPEND
   return VN_OK;
 }
@@ -512,13 +558,14 @@ int32_t vn_qkv_read(vn_qkv* c, int32_t n_ent, const int32_t* ents, const int32_t
   const int es = dtype == VN_F32 ? 4 : 2;
   VN_REQUIRE(c->ctx, aligned(k_out, es) && aligned(v_out, es), "outputs are not aligned to their values");
   const int vec = aligned(k_out, 16) && aligned(v_out, 16);
-  // rows of a CTA: more of them in flight for each thread where there are CTAs enough
-  const int y = ceil_div(c->v.KH * c->v.d * es / 16, 256);
-  const bool many = (long long)ceil_div(M, 8) * y >= 4ll * c->ctx->sm_count;
-  VN_REQUIRE(c->ctx, y <= 65535, "%d heads of %d", c->v.KH, c->v.d);
-  const dim3 grid(ceil_div(M, many ? 8 : 2), y, 2);
-#define READ2(O, S, RB) VN_LAUNCH_PDL_LEVEL(c->ctx, 1, "qkv_read_kernel", (qkv_read_kernel<O, S, RB>), grid, 256, 0, c->v, s, start, offset, (O*)k_out, (O*)v_out, vec)
-#define READ(O, S) do { if (many) READ2(O, S, 8); else READ2(O, S, 2); } while (0)
+  // rows of a warp: four where there are warps enough for all SMs, else one
+  const int slices = ceil_div(c->v.KH * c->v.d * es / 16, 32);
+  const bool many = (long long)ceil_div(M, 4) * slices >= 64ll * c->ctx->sm_count;
+  const long long items = (long long)ceil_div(M, many ? 4 : 1) * slices;
+  VN_REQUIRE(c->ctx, items < (1ll << 32), "%d rows are too many for one call", M);
+  const unsigned grid = (unsigned)ceil_div(items, 8ll);
+#define READ2(O, S, RB) VN_LAUNCH_PDL_LEVEL(c->ctx, 1, "qkv_read_kernel", (qkv_read_kernel<O, S, RB>), grid, 256, 0, c->v, s, start, offset, (O*)k_out, (O*)v_out, vec, slices)
+#define READ(O, S) do { if (many) READ2(O, S, 4); else READ2(O, S, 1); } while (0)
   if (c->v.scheme == QKV_I8) { if (es == 4) READ(float, QKV_I8); else READ(bf16, QKV_I8); }
   else { if (es == 4) READ(float, QKV_E4M3); else READ(bf16, QKV_E4M3); }
 #undef READ
