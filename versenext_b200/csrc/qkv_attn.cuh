@@ -59,7 +59,7 @@ __device__ __forceinline__ void fetch_block(unsigned dst, const void* src, unsig
 }
 
 __device__ __forceinline__ void mma_f16(float (&c)[4], const unsigned (&a)[4], unsigned b0, unsigned b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};\n"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ unsigned pack_f16(float lo, float hi) {
@@ -107,10 +107,11 @@ template <int SCHEME, bool EVERY_OTHER, bool BIAS> __device__ __forceinline__ vo
 struct Unit {
   int slot, r0, n, len, f0, nf;              // rows f0 .. of nf = tokens x heads of the group
   int lo, hi, full_lo, full_hi;              // positions any row sees; positions all rows see
-  int tile0, tiles;                          // blocks of 32 positions
+  int tile0, tiles;                          // the tiles of positions that hold them
 };
 
-template <int RT>
+// BLK: positions of a tile
+template <int RT, int BLK>
 __device__ __forceinline__ bool unit_of(const QkvAttnArgs& a, int rts, int z, Unit& u) {
   const int e = rts == 1 ? z : z / rts, rt = rts == 1 ? 0 : z - e * rts, G = a.v.H / a.v.KH;
   u.tiles = 0;
@@ -129,9 +130,59 @@ __device__ __forceinline__ bool unit_of(const QkvAttnArgs& a, int rts, int z, Un
     u.full_lo = max(0, u.len + (tree ? QKV_MAX_DRAFT - 1 : t1) - a.window + 1);
     if (tree) u.lo = min(u.lo, u.len);
   }
-  u.tile0 = u.lo / QKV_BLOCK;
-  u.tiles = (u.hi + QKV_BLOCK - 1) / QKV_BLOCK - u.tile0;
+  u.tile0 = u.lo / BLK;
+  u.tiles = (u.hi + BLK - 1) / BLK - u.tile0;
   if (u.tiles <= 0) { u.tile0 = 0; u.tiles = 1; }            // rows that see nothing still get their zeros
+  return true;
+}
+
+// The line of tiles of all (entry, rows, head) units (or of the units, where they are not cut) and what of it a worker has: tiles at .. end,
+// the first of them tile `tile` of unit (z, head).  False: nothing.  Called by all threads of a CTA; s_plan: THREADS + 8 ints
+struct Share { int z, head, tile, at, end, share; };
+template <int RT, int BLK>
+__device__ __forceinline__ bool find_share(const QkvAttnArgs& a, int rts, bool split, int least, int worker, int workers, int* s_plan, Unit& u, Share& s) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, KH = a.v.KH, Z = a.step.n_ent * rts, zc = (Z + THREADS - 1) / THREADS;
+  auto weight = [&]() { return (split ? u.tiles : min(u.tiles, 1)) * KH; };
+  int up = 0;
+  if (tid < THREADS) {
+    for (int z = tid * zc; z < min(Z, (tid + 1) * zc); ++z) {
+      unit_of<RT, BLK>(a, rts, z, u);
+      up += weight();
+    }
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int t = __shfl_up_sync(0xffffffffu, up, o);
+      if (lane >= o) up += t;
+    }
+    if (lane == 31) s_plan[THREADS + 1 + warp] = up;
+  }
+  __syncthreads();
+  if (tid < THREADS) {
+#pragma unroll
+    for (int w = 0; w < WARPS - 1; ++w) up += w < warp ? s_plan[THREADS + 1 + w] : 0;
+    s_plan[tid + 1] = up;
+    if (tid == 0) s_plan[0] = 0;
+  }
+  __syncthreads();
+  const int W = s_plan[THREADS];
+  s.share = max((W + workers - 1) / workers, split ? least : 1);
+  s.at = (int)min((long long)worker * s.share, (long long)W);
+  s.end = (int)min((long long)s.at + s.share, (long long)W);
+  if (s.at >= s.end) return false;
+  int j = 0;
+#pragma unroll
+  for (int o = THREADS / 2; o > 0; o >>= 1)
+    if (s_plan[j + o] <= s.at) j += o;
+  s.z = j * zc;
+  int rem = s.at - s_plan[j];
+  for (;; ++s.z) {
+    unit_of<RT, BLK>(a, rts, s.z, u);
+    const int n = weight();
+    if (rem < n) break;
+    rem -= n;
+  }
+  s.head = split ? rem / u.tiles : rem;
+  s.tile = split ? rem - s.head * u.tiles : 0;
   return true;
 }
 
@@ -154,54 +205,12 @@ __global__ void __launch_bounds__(THREADS, (AttnCfg<T, P, NT, RS>::CTAS)) qkv_at
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   pdl_wait();
 
-  // ---- the line of blocks (or of units, where they are not cut) and the share of this warp or CTA
-  const int Z = a.step.n_ent * rts, zc = (Z + THREADS - 1) / THREADS;
   const int worker = RS > 1 ? blockIdx.x : blockIdx.x * WARPS + warp, workers = RS > 1 ? gridDim.x : gridDim.x * WARPS;
   Unit u;
-  auto weight = [&]() { return (split ? u.tiles : min(u.tiles, 1)) * v.KH; };
-  {
-    int sum = 0;
-    for (int z = tid * zc; z < min(Z, (tid + 1) * zc); ++z) {
-      unit_of<RT>(a, rts, z, u);
-      sum += weight();
-    }
-    int up = sum;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int t = __shfl_up_sync(0xffffffffu, up, o);
-      if (lane >= o) up += t;
-    }
-    int* s_tot = s_plan + THREADS + 1;
-    if (lane == 31) s_tot[warp] = up;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < WARPS - 1; ++w) up += w < warp ? s_tot[w] : 0;
-    s_plan[tid + 1] = up;
-    if (tid == 0) s_plan[0] = 0;
-    __syncthreads();
-  }
-  const int W = s_plan[THREADS];
-  const int share = max((W + workers - 1) / workers, split ? MIN_SHARE : 1);
-  int at = (int)min((long long)worker * share, (long long)W);
-  const int end = (int)min((long long)at + share, (long long)W);
-  if (at >= end) return;
-  int z, head, tile;                                         // where the share begins
-  {
-    int j = 0;
-#pragma unroll
-    for (int o = THREADS / 2; o > 0; o >>= 1)
-      if (s_plan[j + o] <= at) j += o;
-    z = j * zc;
-    int rem = at - s_plan[j];
-    for (;; ++z) {
-      unit_of<RT>(a, rts, z, u);
-      const int n = weight();
-      if (rem < n) break;
-      rem -= n;
-    }
-    head = split ? rem / u.tiles : rem;
-    tile = split ? rem - head * u.tiles : 0;
-  }
+  Share sh;
+  if (!find_share<RT, QKV_BLOCK>(a, rts, split, MIN_SHARE, worker, workers, s_plan, u, sh)) return;
+  int z = sh.z, head = sh.head, tile = sh.tile, at = sh.at;
+  const int end = sh.end, share = sh.share;
 
   unsigned it = 0, put = 0;                                  // blocks taken and asked for
   bool dead = false;                                         // a copy did not come: nothing is computed any more
@@ -469,7 +478,7 @@ __global__ void __launch_bounds__(THREADS, (AttnCfg<T, P, NT, RS>::CTAS)) qkv_at
       tile = 0;
       if (++head == v.KH) {
         head = 0;
-        do { ++z; unit_of<RT>(a, rts, z, u); } while (u.tiles == 0);
+        do { ++z; unit_of<RT, QKV_BLOCK>(a, rts, z, u); } while (u.tiles == 0);
       }
       begin_segment();
     }
@@ -615,6 +624,29 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) qkv_merge_kernel(QkvAttnArgs
   if (threadIdx.x == 0 && atomicAdd(a.n_cuts + 2, 1) == (int)gridDim.x - 1) { a.n_cuts[0] = 0; a.n_cuts[1] = 0; a.n_cuts[2] = 0; }
 }
 
+// row blocks of an entry, and whether units are cut: those of a few tiles stay whole, as cutting them saves less than the merge costs
+struct Launch {
+  long long rts = 0, units = 0, tiles = 0;
+  bool split = false;
+  int32_t of(vn_qkv* c, const QkvAttnArgs& a, int RT, int blk, int uncut) {
+    rts = ceil_div((long long)a.step.T * (a.v.H / a.v.KH), (long long)RT);
+    units = rts * a.step.n_ent * a.v.KH;
+    tiles = a.v.capacity() / blk;
+    split = tiles > uncut;
+    VN_REQUIRE(c->ctx, rts < (1ll << 31) && units < (1ll << 31) / tiles - THREADS, "%d rows over %d positions are too many for one call: bring them in portions", a.step.M, a.v.capacity());
+    return VN_OK;
+  }
+  // shares that there can be
+  long long most(int least) const { return split ? ceil_div(units * tiles, (long long)least) : units; }
+};
+
+template <typename T, int P>
+int32_t merge(vn_qkv* c, const QkvAttnArgs& a, int RT) {
+  VN_LAUNCH_PDL_LEVEL(c->ctx, 1, "qkv_merge_kernel", (qkv_merge_kernel<T, P>), dim3((unsigned)c->ctx->sm_count * 2), 32 * MERGE_WARPS, 0, a, RT,
+                      (int)min((long long)RT, (long long)a.step.T * (a.v.H / a.v.KH)));
+  return VN_OK;
+}
+
 template <typename T, int SCHEME, int P, int NT, int RS>
 int32_t launch(vn_qkv* c, const QkvAttnArgs& a) {
   using C = AttnCfg<T, P, NT, RS>;
@@ -632,22 +664,20 @@ int32_t launch(vn_qkv* c, const QkvAttnArgs& a) {
     VN_CUDA(ctx, cudaFuncSetAttribute(qkv_merge_kernel<T, P>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
     occ = min(n, C::CTAS);
   }
-  const long long rts = ceil_div((long long)a.step.T * (a.v.H / a.v.KH), (long long)C::RT);
-  const long long blocks = rts * a.step.n_ent * a.v.KH, tiles = a.v.capacity() / QKV_BLOCK;
-  VN_REQUIRE(ctx, rts < (1ll << 31) && blocks < (1ll << 31) / tiles - THREADS, "%d rows over %d positions are too many for one call: bring them in portions", a.step.M, a.v.capacity());
-  // units of a few blocks stay whole: cutting them saves less than the merge costs
-  const bool split = tiles > UNCUT;
-  // no more CTAs than there can be shares
-  const unsigned grid = (unsigned)min((long long)occ * ctx->sm_count, ceil_div(split ? ceil_div(blocks * tiles, (long long)MIN_SHARE) : blocks, (long long)C::RINGS));
-  VN_LAUNCH_PDL_LEVEL(ctx, 1, "qkv_attn_kernel", kernel, grid, THREADS, C::SMEM, a, (int)rts, split);
-  if (split) VN_LAUNCH_PDL_LEVEL(ctx, 1, "qkv_merge_kernel", (qkv_merge_kernel<T, P>), dim3((unsigned)ctx->sm_count * 2), 32 * MERGE_WARPS, 0, a, C::RT, (int)min((long long)C::RT, (long long)a.step.T * (a.v.H / a.v.KH)));
-  return VN_OK;
+  Launch l;
+  if (int32_t st = l.of(c, a, C::RT, QKV_BLOCK, UNCUT)) return st;
+  const unsigned grid = (unsigned)min((long long)occ * ctx->sm_count, ceil_div(l.most(MIN_SHARE), (long long)C::RINGS));
+  VN_LAUNCH_PDL_LEVEL(ctx, 1, "qkv_attn_kernel", kernel, grid, THREADS, C::SMEM, a, (int)l.rts, l.split);
+  return l.split ? merge<T, P>(c, a, C::RT) : VN_OK;
 }
+
+template <int SCHEME, int P> int32_t launch_tc(vn_qkv* c, const QkvAttnArgs& a);      // qkv_attn_tc.cuh
 
 template <int SCHEME>
 int32_t pick(vn_qkv* c, const QkvAttnArgs& a) {
   // as few columns as hold the rows of an entry; from 17 rows on the warps split the rows
   const long long rows = (long long)a.step.T * (a.v.H / a.v.KH);
+  if (c->dtype == VN_BF16 && rows > 16 && (a.v.P == 64 || a.v.P == 128)) return a.v.P == 64 ? launch_tc<SCHEME, 64>(c, a) : launch_tc<SCHEME, 128>(c, a);
 #define GO(P, NT, RS) return c->dtype == VN_F32 ? launch<float, SCHEME, P, NT, RS>(c, a) : launch<bf16, SCHEME, P, NT, RS>(c, a)
 #define GO2(P) do { if (rows <= 8) GO(P, 1, 1); else if (rows <= 16) GO(P, 2, 1); else GO(P, 2, 4); } while (0)
 #define GO4(P) do { if (rows <= 8) GO(P, 1, 1); else if (rows <= 16) GO(P, 2, 1); else if (rows <= 64) GO(P, 2, 4); else GO(P, 4, 4); } while (0)

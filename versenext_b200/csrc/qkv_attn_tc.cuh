@@ -1,0 +1,456 @@
+// Attention over the 8-bit cache for many rows (prompts, trees): 128 rows of a unit on tcgen05.
+//
+// A CTA has nine warps.  Four convert: a page (64 positions) of codes, brought in by one bulk copy, becomes 16-bit floats in shared memory, keys
+// and values alike with 128-byte rows of 64 channels and the 128-byte swizzle -- the layout of a K-major operand for the keys
+// (S = Q K^T) and of an MN-major one for the values (O += P V).  One warp issues the products.  Four do the soft-max, a thread for a row: S
+// from TMEM, weights back to TMEM as the second product's A operand, results in TMEM.  S of the next page is computed while the weights of
+// this one are, and two CTAs share an SM.
+//
+// A row's reference maximum is moved only when a page's is more than 2^4 above it, so that the results in TMEM are seldom rescaled; weights
+// are at most 2^4 then, and taken relative to R (at least the largest scale of values, with room of 2^2) times 2^11: a half holds them down
+// to 2^-33 of the largest.
+#pragma once
+#include "qkv_attn.cuh"
+
+namespace qkv_detail {
+
+constexpr int TC_ROWS = 128, TC_KEYS = KV_PAGE, TC_THREADS = 288, TC_CTAS = 2;
+constexpr int TC_MIN_SHARE = 2, TC_UNCUT = 4;       // pages of a share at least; of a unit that is never cut
+
+template <int P>
+struct TcCfg {
+  static constexpr int PANELS = P / 64, PAGE = 2 * QKV_BLOCK * (2 * P + 8), STAGES = P > 64 ? 2 : 3;
+  static constexpr int Q = 0, K = Q + PANELS * TC_ROWS * 128, V = K + PANELS * TC_KEYS * 128, RAW = V + PANELS * TC_KEYS * 128, SCALES = RAW + STAGES * PAGE,
+                       WEIGHTS = SCALES + 2 * 2 * TC_KEYS * 4, META = WEIGHTS + 4 * TC_KEYS * 4, BARS = META + 32, SLOT = BARS + 16 * 8, PLAN = SLOT + 16,
+                       SMEM = PLAN + (THREADS + 8) * 4 + 1024;        // the first 1024: the swizzle's alignment
+  static constexpr unsigned S_COL = 0, P_COL = 64, O_COL = 128;
+  static_assert(P % 64 == 0 && O_COL + P <= 256, "256 columns of TMEM for each of two CTAs");
+  static_assert(TC_CTAS * TC_ROWS * P <= QKV_PART, "parts fit their place");
+};
+
+__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void fence_to_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+__device__ __forceinline__ void tc_commit(unsigned bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
+}
+// both operands in shared memory
+__device__ __forceinline__ void tc_mma_ss(unsigned d, unsigned long long a, unsigned long long b, unsigned idesc, bool add) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((unsigned)add) : "memory");
+}
+// A in TMEM: two neighbouring k of a row in every column
+__device__ __forceinline__ void tc_mma_ts(unsigned d, unsigned a, unsigned long long b, unsigned idesc, bool add) {
+  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"((unsigned)add) : "memory");
+}
+// 128-byte swizzle, groups of eight 128-byte rows 1024 bytes apart; panels: bytes between panels of 64 along M or N (MN-major operands)
+__device__ __forceinline__ unsigned long long tc_desc(unsigned addr, unsigned panels) {
+  return (unsigned long long)((addr & 0x3ffffu) >> 4) | (unsigned long long)(panels >> 4) << 16 | 64ull << 32 | 1ull << 46 | 2ull << 61;
+}
+#define QKV_R32(x) "=r"((x)[0]), "=r"((x)[1]), "=r"((x)[2]), "=r"((x)[3]), "=r"((x)[4]), "=r"((x)[5]), "=r"((x)[6]), "=r"((x)[7]), "=r"((x)[8]), "=r"((x)[9]), "=r"((x)[10]), \
+  "=r"((x)[11]), "=r"((x)[12]), "=r"((x)[13]), "=r"((x)[14]), "=r"((x)[15]), "=r"((x)[16]), "=r"((x)[17]), "=r"((x)[18]), "=r"((x)[19]), "=r"((x)[20]), "=r"((x)[21]), \
+  "=r"((x)[22]), "=r"((x)[23]), "=r"((x)[24]), "=r"((x)[25]), "=r"((x)[26]), "=r"((x)[27]), "=r"((x)[28]), "=r"((x)[29]), "=r"((x)[30]), "=r"((x)[31])
+#define QKV_I32(x) "r"((x)[0]), "r"((x)[1]), "r"((x)[2]), "r"((x)[3]), "r"((x)[4]), "r"((x)[5]), "r"((x)[6]), "r"((x)[7]), "r"((x)[8]), "r"((x)[9]), "r"((x)[10]), \
+  "r"((x)[11]), "r"((x)[12]), "r"((x)[13]), "r"((x)[14]), "r"((x)[15]), "r"((x)[16]), "r"((x)[17]), "r"((x)[18]), "r"((x)[19]), "r"((x)[20]), "r"((x)[21]), \
+  "r"((x)[22]), "r"((x)[23]), "r"((x)[24]), "r"((x)[25]), "r"((x)[26]), "r"((x)[27]), "r"((x)[28]), "r"((x)[29]), "r"((x)[30]), "r"((x)[31])
+// 32 columns of the warp's 32 rows
+__device__ __forceinline__ void tc_ld(unsigned at, unsigned* x) {
+  asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+               "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];" : QKV_R32(x) : "r"(at));
+}
+__device__ __forceinline__ void tc_st(unsigned at, const unsigned* x) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+               "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::QKV_I32(x), "r"(at) : "memory");
+}
+#undef QKV_R32
+#undef QKV_I32
+__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// 16 codes to 16-bit floats in two chunks of a panel's row; none: zeros
+template <int SCHEME>
+__device__ __forceinline__ void convert16(const unsigned char* from, unsigned char* row, int chunk, int turn, bool none) {
+  uint4 u = *reinterpret_cast<const uint4*>(from);
+  if (none) u = SCHEME == QKV_I8 ? make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u) : make_uint4(0u, 0u, 0u, 0u);
+  uint4 x, y;
+  halves_of<SCHEME, false, false>(u.x, x.x, x.y);
+  halves_of<SCHEME, false, false>(u.y, x.z, x.w);
+  halves_of<SCHEME, false, false>(u.z, y.x, y.y);
+  halves_of<SCHEME, false, false>(u.w, y.z, y.w);
+  *reinterpret_cast<uint4*>(row + ((chunk ^ turn) << 4)) = x;
+  *reinterpret_cast<uint4*>(row + (((chunk + 1) ^ turn) << 4)) = y;
+}
+
+template <int SCHEME, int P>
+__global__ void __launch_bounds__(TC_THREADS, TC_CTAS) qkv_attn_tc_kernel(QkvAttnArgs a, int rts, bool split) {
+  pdl_trigger();
+  using C = TcCfg<P>;
+  constexpr int ST = C::STAGES, PANELS = C::PANELS, BLOCK = QKV_BLOCK * (2 * P + 8);
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = smem_raw + ((1024u - ((unsigned)__cvta_generic_to_shared(smem_raw) & 1023u)) & 1023u);
+  const unsigned s_base = (unsigned)__cvta_generic_to_shared(smem);
+  const QkvView& v = a.v;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = v.H / v.KH;
+  enum { RAW_FULL = 0, K_READY = 4, V_READY, Q_READY, S_FULL, S_FREE, P_FULL, PV_DONE };
+  auto bar = [&](int i) { return s_base + C::BARS + 8 * i; };
+  float* s_scales = reinterpret_cast<float*>(smem + C::SCALES);            // [2][keys | values][64]
+  int* s_meta = reinterpret_cast<int*>(smem + C::META);                    // [2]: page there, largest exponent of values' scales of either half
+  if (tid == 0) {
+    for (int i = 0; i < ST; ++i) mbar_init(bar(RAW_FULL + i), 1);
+    for (int i : {(int)K_READY, (int)V_READY, (int)Q_READY, (int)S_FREE, (int)P_FULL}) mbar_init(bar(i), 4);
+    mbar_init(bar(S_FULL), 1);
+    mbar_init(bar(PV_DONE), 1);
+  }
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  pdl_wait();
+  Unit u;
+  Share sh;
+  if (!find_share<TC_ROWS, TC_KEYS>(a, rts, split, TC_MIN_SHARE, blockIdx.x, gridDim.x, reinterpret_cast<int*>(smem + C::PLAN), u, sh)) return;
+  unsigned* s_slot = reinterpret_cast<unsigned*>(smem + C::SLOT);
+  if (warp == 8) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s_base + C::SLOT), "r"(256u) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const unsigned tmem = *s_slot;
+  bool dead = false;                                         // a wait ran out: the results are no good, but everybody comes to the end
+  auto wait = [&](int b, unsigned parity) {
+    if (!mbar_try1(bar(b), parity) && !mbar_wait_long(bar(b), parity, dead ? 1000000ull : WAIT_CYCLES)) { dead = true; v.status[2] = 1; }
+  };
+  unsigned n = 0;                                            // pages gone through, the same count for all roles
+  int seg_a, seg_n, segs = 0;
+  auto begin = [&]() {
+    seg_a = u.tile0 + sh.tile;
+    seg_n = split ? min(u.tiles - sh.tile, sh.end - sh.at) : u.tiles;
+  };
+  auto advance = [&]() {                                     // to the next segment; false: none
+    sh.at += split ? seg_n : 1;
+    if (sh.at >= sh.end) return false;
+    sh.tile = 0;
+    if (++sh.head == v.KH) {
+      sh.head = 0;
+      do { ++sh.z; unit_of<TC_ROWS, TC_KEYS>(a, rts, sh.z, u); } while (u.tiles == 0);
+    }
+    ++segs;
+    return true;
+  };
+  auto page_of = [&](int i) { return v.page(u.slot, seg_a + i); };
+
+  if (warp == 8) {
+    // ---- products: S of page i + 1 before O of page i
+    if (lane == 0) {
+      const unsigned idesc_s = 1u << 4 | (unsigned)(TC_KEYS >> 3) << 17 | (unsigned)(TC_ROWS >> 4) << 24;
+      const unsigned idesc_o = 1u << 4 | 1u << 16 | (unsigned)(P >> 3) << 17 | (unsigned)(TC_ROWS >> 4) << 24;
+      auto scores = [&](unsigned t) {
+        wait(K_READY, t & 1);
+        if (t) wait(S_FREE, (t - 1) & 1);
+        tc_fence_after();
+#pragma unroll
+        for (int p = 0; p < PANELS; ++p) {
+          const unsigned long long da = tc_desc(s_base + C::Q + p * TC_ROWS * 128, 16), db = tc_desc(s_base + C::K + p * TC_KEYS * 128, 16);
+#pragma unroll
+          for (int k = 0; k < 4; ++k) tc_mma_ss(tmem + C::S_COL, da + 2 * k, db + 2 * k, idesc_s, p || k);
+        }
+        tc_commit(bar(S_FULL));
+      };
+      auto results = [&](unsigned t, bool add) {
+        wait(V_READY, t & 1);
+        wait(P_FULL, t & 1);
+        tc_fence_after();
+        const unsigned long long db = tc_desc(s_base + C::V, TC_KEYS * 128);
+#pragma unroll
+        for (int k = 0; k < TC_KEYS / 16; ++k) tc_mma_ts(tmem + C::O_COL, tmem + C::P_COL + 8 * k, db + 128 * k, idesc_o, add || k);
+        tc_commit(bar(PV_DONE));
+      };
+      do {
+        begin();
+        wait(Q_READY, segs & 1);
+        scores(n);
+        for (int i = 1; i < seg_n; ++i) {
+          scores(n + i);
+          results(n + i - 1, i > 1);
+        }
+        results(n + seg_n - 1, seg_n > 1);
+        n += seg_n;
+      } while (advance());
+    }
+  } else if (warp >= 4) {
+    // ---- codes to halves
+    const int ct = tid - 128;
+    auto ask = [&](int i) {                                  // page i of the segment, which is page n + i of all
+      const unsigned s = (n + i) % ST;
+      const int page = page_of(i);
+      if (page >= 0 && !dead) fetch_block(s_base + C::RAW + s * C::PAGE, v.block(page, sh.head, 0), C::PAGE, bar(RAW_FULL + s));
+      else mbar_arrive1(bar(RAW_FULL + s));
+    };
+    do {
+      begin();
+      if (ct == 0)
+        for (int i = 0; i < min(ST, seg_n); ++i) ask(i);
+      for (int i = 0; i < seg_n; ++i) {
+        const unsigned t = n + i, s = t % ST;
+        const unsigned char* raw = smem + C::RAW + s * C::PAGE;
+        const bool none = page_of(i) < 0;
+        float* sc = s_scales + (t & 1) * 2 * TC_KEYS;
+        auto convert = [&](int which) {
+#pragma unroll
+          for (int x = ct; x < TC_KEYS * (P / 16); x += 128) {
+            const int r = x / (P / 16), c = x % (P / 16);
+            const unsigned char* from = raw + (r / QKV_BLOCK) * BLOCK + (which * QKV_BLOCK + r % QKV_BLOCK) * P + ((c ^ qkv_turn(P / 16, r % QKV_BLOCK)) << 4);
+            convert16<SCHEME>(from, smem + (which ? C::V : C::K) + (c / 4) * TC_KEYS * 128 + r * 128, c % 4 * 2, r & 7, none);
+          }
+        };
+        if (t) wait(S_FULL, (t - 1) & 1);                    // the keys before these have been multiplied
+        wait(RAW_FULL + s, (t / ST) & 1);
+        convert(0);
+        // scales, and the largest exponent of those of values that count: 32 positions for each of two warps
+        if (ct < TC_KEYS) {
+          const float* from = reinterpret_cast<const float*>(raw + (ct / QKV_BLOCK) * BLOCK + 2 * QKV_BLOCK * P) + ct % QKV_BLOCK;
+          const int key = (seg_a + i) * TC_KEYS + ct;
+          const float vs = none ? 0.f : from[QKV_BLOCK];
+          sc[ct] = none ? 0.f : from[0];
+          sc[TC_KEYS + ct] = vs;
+          const unsigned b = __float_as_uint(vs);
+          const unsigned top = __reduce_max_sync(0xffffffffu, key >= u.lo && key < u.hi && b < 0x7f800000u ? b : 0u);
+          if (lane == 0) s_meta[(t & 1) * 4 + 1 + ct / 32] = (int)(top >> 23);
+          if (ct == 0) s_meta[(t & 1) * 4] = !none;
+        }
+        fence_to_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive1(bar(K_READY));
+        if (t) wait(PV_DONE, (t - 1) & 1);                   // and the values before these
+        convert(1);
+        fence_to_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive1(bar(V_READY));
+        asm volatile("bar.sync 1, 128;" ::: "memory");       // nobody reads the stage any more
+        if (ct == 0 && i + ST < seg_n) ask(i + ST);
+        if (none && ct == 0) v.status[0] = 1;
+      }
+      n += seg_n;
+    } while (advance());
+  } else {
+    // ---- soft-max: thread = row
+    const unsigned lanes = tmem + ((unsigned)(warp * 32) << 16);
+    float* s_w = reinterpret_cast<float*>(smem + C::WEIGHTS) + warp * TC_KEYS;             // the page's scales of values, relative to R
+    do {
+      begin();
+      const int f = u.f0 + tid, tok = f < u.nf ? f / G : -1;
+      // queries of the warp's rows, eight at a time: a lane takes P / 32 channels
+      float rf = 0.f;
+      const int away = tok < 0 ? 0 : a.tree.away(u.r0 + tok, tok);
+      const unsigned long long seen = a.tree.seen && tok >= 0 ? a.tree.seen[a.tree.per_row ? u.r0 + tok : tok] : 0;
+#pragma unroll 1
+      for (int rb = 0; rb < 32; rb += 8) {
+        constexpr int W = P / 32;                            // 2 or 4 channels
+        float x[8][W];
+        unsigned top[8];
+#pragma unroll
+        for (int b = 0; b < 8; ++b) {
+          const int rt = __shfl_sync(0xffffffffu, tok, rb + b), rf_ = u.f0 + warp * 32 + rb + b;
+          const bf16* q = reinterpret_cast<const bf16*>(a.q) + ((long long)(u.r0 + max(rt, 0)) * v.H + sh.head * G + (rt < 0 ? 0 : rf_ - rt * G)) * v.d + W * lane;
+          uint2 w = make_uint2(0u, 0u);
+          if (rt >= 0 && W * lane < v.d) {
+            if (W == 4) w = *reinterpret_cast<const uint2*>(q); else w.x = *reinterpret_cast<const unsigned*>(q);
+          }
+          x[b][0] = __uint_as_float(w.x << 16); x[b][1] = __uint_as_float(w.x & 0xffff0000u);
+          if (W == 4) { x[b][W - 2] = __uint_as_float(w.y << 16); x[b][W - 1] = __uint_as_float(w.y & 0xffff0000u); }
+        }
+#pragma unroll
+        for (int b = 0; b < 8; ++b) {
+          top[b] = 0;
+#pragma unroll
+          for (int e = 0; e < W; ++e) top[b] = max(top[b], __float_as_uint(x[b][e]) & 0x7fffffffu);
+        }
+#pragma unroll
+        for (int b = 0; b < 8; ++b) top[b] = __reduce_max_sync(0xffffffffu, top[b]);
+#pragma unroll
+        for (int b = 0; b < 8; ++b) {
+          const int e = top[b] >= 0x7f800000u ? 140 : min(max((int)(top[b] >> 23), 27), 254), r = warp * 32 + rb + b, c = W * lane;   // not finite: left as it is
+          const float up = pow2(267 - e);
+          unsigned char* to = smem + C::Q + (c / 64) * TC_ROWS * 128 + r * 128 + (((c % 64 / 8) ^ (r & 7)) << 4) + (c % 8) * 2;
+          if (W == 4) *reinterpret_cast<uint2*>(to) = make_uint2(pack_f16(x[b][0] * up, x[b][1] * up), pack_f16(x[b][W - 2] * up, x[b][W - 1] * up));
+          else *reinterpret_cast<unsigned*>(to) = pack_f16(x[b][0] * up, x[b][1] * up);
+          if (lane == rb + b) rf = fmaxf(a.scale * 1.4426950408889634f * pow2(e - 13), 1.17549435e-38f);
+        }
+      }
+      fence_to_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive1(bar(Q_READY));
+      float m = -CUDART_INF_F, l = 0.f;
+      int R = 16;
+#pragma unroll 1
+      for (int i = 0; i < seg_n; ++i) {
+        const unsigned t = n + i;
+        const float* sc = s_scales + (t & 1) * 2 * TC_KEYS;
+        const int* meta = s_meta + (t & 1) * 4;
+        wait(S_FULL, t & 1);                                 // and with it the scales, written before the product was issued
+        __syncwarp();
+        tc_fence_after();
+        float x[TC_KEYS];
+        tc_ld(lanes + C::S_COL, reinterpret_cast<unsigned*>(x));
+        tc_ld(lanes + C::S_COL + 32, reinterpret_cast<unsigned*>(x) + 32);
+        tc_wait_ld();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive1(bar(S_FREE));
+        const int e = max(meta[1], meta[2]);
+        float f_r = 1.f;
+        if (e > R) {
+          const int to = min(e + 2, 254);
+          f_r = pow2(127 + R - to);
+          R = to;
+        }
+        const float rs = pow2(264 - R);
+        s_w[lane] = sc[TC_KEYS + lane] * rs;
+        s_w[lane + 32] = sc[TC_KEYS + lane + 32] * rs;
+#pragma unroll
+        for (int c = 0; c < TC_KEYS; c += 4) {
+          const float4 k = *reinterpret_cast<const float4*>(sc + c);
+          x[c] *= k.x; x[c + 1] *= k.y; x[c + 2] *= k.z; x[c + 3] *= k.w;
+        }
+        const int k0 = (seg_a + i) * TC_KEYS;
+        const bool full = meta[0] && k0 >= u.full_lo && k0 + TC_KEYS <= u.full_hi;
+        if (!full) {
+          // which of the page's positions the row sees, as bits
+          auto range = [&](int lo, int hi) {                 // positions lo .. hi - 1
+            const int p = min(max(lo - k0, 0), 64), q = min(max(hi - k0, 0), 64);
+            return p >= q ? 0ull : (~0ull >> (64 - (q - p))) << p;
+          };
+          unsigned long long see = 0;
+          if (tok >= 0 && meta[0]) {
+            const int from = a.window > 0 ? max(0, u.len + away - a.window + 1) : 0;
+            if (a.tree.seen) {
+              const int off = u.len - k0;                    // where the new rows begin in the page
+              const unsigned long long rows = u.n >= 64 ? seen : seen & ((1ull << u.n) - 1);
+              see = range(from, u.len) | (off >= 64 || off <= -64 ? 0ull : off >= 0 ? rows << off : rows >> -off);
+            } else {
+              see = range(from, u.len + tok + 1);
+            }
+            see &= range(0, u.hi);
+          }
+          const unsigned lo = (unsigned)see, hi = (unsigned)(see >> 32);
+#pragma unroll
+          for (int c = 0; c < 32; ++c) {
+            if (!((lo >> c) & 1)) x[c] = -CUDART_INF_F;
+            if (!((hi >> c) & 1)) x[c + 32] = -CUDART_INF_F;
+          }
+        }
+        float mx[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+        for (int c = 4; c < TC_KEYS; ++c) mx[c & 3] = fmaxf(mx[c & 3], x[c]);
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * rf;
+        float f_m = 1.f;
+        if (top > m + 4.f || (m == -CUDART_INF_F && top > m)) {
+          f_m = ex2(m - top);                                // from nothing: zero
+          m = top;
+          l *= f_m;
+        }
+        const float base = m == -CUDART_INF_F ? 0.f : m;     // nothing seen yet: every weight becomes exp2(-inf) = 0
+        unsigned pk[TC_KEYS / 2];
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        __syncwarp();                                        // s_w
+#pragma unroll
+        for (int c = 0; c < TC_KEYS; c += 4) {
+          const float4 w = *reinterpret_cast<const float4*>(s_w + c);
+          float p[4], g[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+          for (int y = 0; y < 4; ++y) {
+            p[y] = ex2(fmaf(x[c + y], rf, -base));
+            sum[y] += p[y];
+            g[y] *= p[y];
+            if (!full && x[c + y] == -CUDART_INF_F) g[y] = 0.f;                            // unseen: any scale, NaN too
+          }
+          pk[c / 2] = pack_f16(g[0], g[1]);
+          pk[c / 2 + 1] = pack_f16(g[2], g[3]);
+        }
+        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        if (t) wait(PV_DONE, (t - 1) & 1);
+        __syncwarp();
+        tc_fence_after();
+        const float f_o = f_m * f_r;
+        if (i && __any_sync(0xffffffffu, f_o != 1.f)) {
+#pragma unroll 1
+          for (int c = 0; c < P; c += 32) {
+            unsigned o[32];
+            tc_ld(lanes + C::O_COL + c, o);
+            tc_wait_ld();
+#pragma unroll
+            for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(__uint_as_float(o[y]) * f_o);
+            tc_st(lanes + C::O_COL + c, o);
+          }
+        }
+        tc_st(lanes + C::P_COL, pk);
+        tc_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive1(bar(P_FULL));
+      }
+      n += seg_n;
+      // ---- a row's results
+      wait(PV_DONE, (n - 1) & 1);
+      __syncwarp();
+      tc_fence_after();
+      const int u_begin = sh.at - sh.tile;
+      const bool whole = !split || seg_n == u.tiles, begun = !whole && sh.tile == 0;
+      const int last = whole ? 0 : (u_begin + u.tiles - 1) / sh.share, part = 2 * blockIdx.x + (begun ? 1 : 0);
+      const float r_inv = pow2(R - 10), inv = whole ? (l == 0.f ? 0.f : r_inv / l) : r_inv;
+      bf16* out = reinterpret_cast<bf16*>(a.out) + ((long long)(u.r0 + max(tok, 0)) * v.H + sh.head * G + (f - max(tok, 0) * G)) * v.d;
+      float* part_o = a.part_o + ((long long)part * TC_ROWS + tid) * P;
+#pragma unroll 1
+      for (int c = 0; c < P; c += 32) {
+        unsigned o[32];
+        __syncwarp();
+        tc_ld(lanes + C::O_COL + c, o);
+        tc_wait_ld();
+#pragma unroll
+        for (int y = 0; y < 32; y += 8) {
+          if (tok < 0) break;
+          float r[8];
+#pragma unroll
+          for (int x = 0; x < 8; ++x) r[x] = l == 0.f ? 0.f : __uint_as_float(o[y + x]) * inv;       // nothing seen: zero
+          if (!whole) {
+            store4(part_o + c + y, make_float4(r[0], r[1], r[2], r[3]));
+            store4(part_o + c + y + 4, make_float4(r[4], r[5], r[6], r[7]));
+          } else if (c + y < v.d) {
+            const __nv_bfloat162 h[4] = {__floats2bfloat162_rn(r[0], r[1]), __floats2bfloat162_rn(r[2], r[3]), __floats2bfloat162_rn(r[4], r[5]), __floats2bfloat162_rn(r[6], r[7])};
+            *reinterpret_cast<uint4*>(out + c + y) = *reinterpret_cast<const uint4*>(h);
+          }
+        }
+      }
+      if (!whole && tok >= 0) a.part_ml[part * TC_ROWS + tid] = make_float2(m, l);
+      if (begun && tid == 0) {                               // a unit to merge: in any order, each by itself
+        const int cnt = last - (int)blockIdx.x + 1;
+        const bool many = cnt > MANY;
+        const int at = atomicAdd(a.n_cuts + (many ? 1 : 0), 1);
+        a.cuts[many ? a.max_cuts - 1 - at : at] = {u.r0, u.f0, u.nf, sh.head, (int)blockIdx.x, cnt};
+      }
+    } while (advance());
+  }
+  tc_fence_before();
+  __syncthreads();
+  __syncwarp();
+  if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256u) : "memory");
+}
+
+template <int SCHEME, int P>
+int32_t launch_tc(vn_qkv* c, const QkvAttnArgs& a) {
+  using C = TcCfg<P>;
+  vn_ctx* ctx = c->ctx;
+  auto kernel = qkv_attn_tc_kernel<SCHEME, P>;
+  static bool ready[64] = {};
+  if (!ready[ctx->device & 63]) {
+    VN_CUDA(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    VN_CUDA(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
+    VN_CUDA(ctx, cudaFuncSetAttribute(qkv_merge_kernel<bf16, P>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
+    ready[ctx->device & 63] = true;
+  }
+  Launch l;
+  if (int32_t st = l.of(c, a, TC_ROWS, TC_KEYS, TC_UNCUT)) return st;
+  const unsigned grid = (unsigned)min((long long)TC_CTAS * ctx->sm_count, l.most(TC_MIN_SHARE));
+  VN_LAUNCH_PDL_LEVEL(ctx, 1, "qkv_attn_tc_kernel", kernel, grid, TC_THREADS, C::SMEM, a, (int)l.rts, l.split);
+  return l.split ? merge<bf16, P>(c, a, TC_ROWS) : VN_OK;
+}
+
+}  // namespace qkv_detail
