@@ -21,7 +21,7 @@ template <int P>
 struct TcCfg {
   static constexpr int PANELS = P / 64, PAGE = 2 * QKV_BLOCK * (2 * P + 8), STAGES = P > 64 ? 2 : 3;
   static constexpr int Q = 0, K = Q + PANELS * TC_ROWS * 128, V = K + PANELS * TC_KEYS * 128, RAW = V + PANELS * TC_KEYS * 128, SCALES = RAW + STAGES * PAGE,
-                       WEIGHTS = SCALES + 2 * 2 * TC_KEYS * 4, META = WEIGHTS + 4 * TC_KEYS * 4, BARS = META + 32, SLOT = BARS + 16 * 8, PLAN = SLOT + 16,
+                       WEIGHTS = SCALES + 3 * 2 * TC_KEYS * 4, META = WEIGHTS + 4 * TC_KEYS * 4, FACTORS = META + 64, BARS = FACTORS + 2 * TC_ROWS * 4, SLOT = BARS + 16 * 8, PLAN = SLOT + 16,
                        SMEM = PLAN + (THREADS + 8) * 4 + 1024;        // the first 1024: the swizzle's alignment
   static constexpr unsigned S_COL = 0, P_COL = 64, O_COL = 128;
   static_assert(P % 64 == 0 && O_COL + P <= 256, "256 columns of TMEM for each of two CTAs");
@@ -92,8 +92,9 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) qkv_attn_tc_kernel(QkvAtt
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = v.H / v.KH;
   enum { RAW_FULL = 0, K_READY = 4, V_READY, Q_READY, S_FULL, S_FREE, P_FULL, PV_DONE };
   auto bar = [&](int i) { return s_base + C::BARS + 8 * i; };
-  float* s_scales = reinterpret_cast<float*>(smem + C::SCALES);            // [2][keys | values][64]
-  int* s_meta = reinterpret_cast<int*>(smem + C::META);                    // [2]: page there, largest exponent of values' scales of either half
+  float* s_scales = reinterpret_cast<float*>(smem + C::SCALES);            // [3][keys | values][64]: page t + 1's are written while t - 1's may still be read
+  float* s_rf = reinterpret_cast<float*>(smem + C::FACTORS);               // [2][rows] r of a segment's rows
+  int* s_meta = reinterpret_cast<int*>(smem + C::META);                    // [3][4]: page there, largest exponent of values' scales of either half
   if (tid == 0) {
     for (int i = 0; i < ST; ++i) mbar_init(bar(RAW_FULL + i), 1);
     for (int i : {(int)K_READY, (int)V_READY, (int)Q_READY, (int)S_FREE, (int)P_FULL}) mbar_init(bar(i), 4);
@@ -135,7 +136,6 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) qkv_attn_tc_kernel(QkvAtt
     ++segs;
     return true;
   };
-  auto page_of = [&](int i) { return v.page(u.slot, seg_a + i); };
 
   if (warp == 8) {
     // ---- products: S of page i + 1 before O of page i
@@ -176,57 +176,102 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) qkv_attn_tc_kernel(QkvAtt
       } while (advance());
     }
   } else if (warp >= 4) {
-    // ---- codes to halves
-    const int ct = tid - 128;
-    auto ask = [&](int i) {                                  // page i of the segment, which is page n + i of all
-      const unsigned s = (n + i) % ST;
-      const int page = page_of(i);
-      if (page >= 0 && !dead) fetch_block(s_base + C::RAW + s * C::PAGE, v.block(page, sh.head, 0), C::PAGE, bar(RAW_FULL + s));
-      else mbar_arrive1(bar(RAW_FULL + s));
-    };
+    // ---- queries and codes to halves: the keys of page i + 1 before the values of page i
+    const int ct = tid - 128, rg = lane >> 2, rc = lane & 3;
+    unsigned asked = 0;                                      // pages asked for in all
     do {
       begin();
-      if (ct == 0)
+      // pages of the segment, 32 at a time: lane j has that of page first + j
+      int pages = -1, next_pages = -1, first = 0;
+      auto pages_of = [&](int i0) { return i0 + lane < seg_n ? v.page(u.slot, seg_a + i0 + lane) : -1; };
+      pages = pages_of(0);
+      next_pages = pages_of(32);
+      auto page = [&](int i) { return __shfl_sync(0xffffffffu, i - first < 32 ? pages : next_pages, (i - first) & 31); };
+      auto ask = [&](int i) {                                // by one warp: nobody reads the stage any more
+        const int pg = page(i);
+        const unsigned s = asked++ % ST;
+        if (lane) return;
+        if (pg >= 0 && !dead) fetch_block(s_base + C::RAW + s * C::PAGE, v.block(pg, sh.head, 0), C::PAGE, bar(RAW_FULL + s));
+        else mbar_arrive1(bar(RAW_FULL + s));
+      };
+      if (warp == 4)
         for (int i = 0; i < min(ST, seg_n); ++i) ask(i);
-      for (int i = 0; i < seg_n; ++i) {
-        const unsigned t = n + i, s = t % ST;
-        const unsigned char* raw = smem + C::RAW + s * C::PAGE;
-        const bool none = page_of(i) < 0;
-        float* sc = s_scales + (t & 1) * 2 * TC_KEYS;
-        auto convert = [&](int which) {
+      if (n) wait(S_FULL, (n - 1) & 1);                      // the queries and keys before these have been multiplied
+      // a warp's 32 rows, eight at a time: four lanes a row, channels 16 k + 4 rc .. + 3 each
+#pragma unroll 1
+      for (int rb = 0; rb < 32; rb += 8) {
+        const int r = (warp - 4) * 32 + rb + rg, f = u.f0 + r, t = f / G;
+        const bool ok = f < u.nf;
+        const bf16* q = reinterpret_cast<const bf16*>(a.q) + ((long long)(u.r0 + (ok ? t : 0)) * v.H + sh.head * G + (ok ? f - t * G : 0)) * v.d + 4 * rc;
+        uint2 x[P / 16];
 #pragma unroll
-          for (int x = ct; x < TC_KEYS * (P / 16); x += 128) {
-            const int r = x / (P / 16), c = x % (P / 16);
-            const unsigned char* from = raw + (r / QKV_BLOCK) * BLOCK + (which * QKV_BLOCK + r % QKV_BLOCK) * P + ((c ^ qkv_turn(P / 16, r % QKV_BLOCK)) << 4);
-            convert16<SCHEME>(from, smem + (which ? C::V : C::K) + (c / 4) * TC_KEYS * 128 + r * 128, c % 4 * 2, r & 7, none);
-          }
-        };
-        if (t) wait(S_FULL, (t - 1) & 1);                    // the keys before these have been multiplied
-        wait(RAW_FULL + s, (t / ST) & 1);
-        convert(0);
-        // scales, and the largest exponent of those of values that count: 32 positions for each of two warps
-        if (ct < TC_KEYS) {
-          const float* from = reinterpret_cast<const float*>(raw + (ct / QKV_BLOCK) * BLOCK + 2 * QKV_BLOCK * P) + ct % QKV_BLOCK;
-          const int key = (seg_a + i) * TC_KEYS + ct;
-          const float vs = none ? 0.f : from[QKV_BLOCK];
-          sc[ct] = none ? 0.f : from[0];
-          sc[TC_KEYS + ct] = vs;
-          const unsigned b = __float_as_uint(vs);
-          const unsigned top = __reduce_max_sync(0xffffffffu, key >= u.lo && key < u.hi && b < 0x7f800000u ? b : 0u);
-          if (lane == 0) s_meta[(t & 1) * 4 + 1 + ct / 32] = (int)(top >> 23);
-          if (ct == 0) s_meta[(t & 1) * 4] = !none;
+        for (int k = 0; k < P / 16; ++k) x[k] = ok && 16 * k + 4 * rc < v.d ? *reinterpret_cast<const uint2*>(q + 16 * k) : make_uint2(0u, 0u);
+        unsigned top = 0;                                    // of the magnitudes' upper halves: all of a bf16
+#pragma unroll
+        for (int k = 0; k < P / 16; ++k) top = __vmaxu2(top, __vmaxu2(x[k].x & 0x7fff7fffu, x[k].y & 0x7fff7fffu));
+        top = max(top >> 16, top & 0xffffu);
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        const int e = top >= 0x7f80u ? 140 : min(max((int)(top >> 7), 27), 254);           // a row that is not finite is left as it is
+        const float up = pow2(267 - e);
+#pragma unroll
+        for (int k = 0; k < P / 16; ++k) {
+          auto two = [&](unsigned w) { return pack_f16(__uint_as_float(w << 16) * up, __uint_as_float(w & 0xffff0000u) * up); };
+          const int c = 16 * k + 4 * rc;
+          *reinterpret_cast<uint2*>(smem + C::Q + (c / 64) * TC_ROWS * 128 + r * 128 + (((c % 64 / 8) ^ (r & 7)) << 4) + (c % 8) * 2) = make_uint2(two(x[k].x), two(x[k].y));
+        }
+        if (rc == 0) s_rf[(segs & 1) * TC_ROWS + r] = fmaxf(a.scale * 1.4426950408889634f * pow2(e - 13), 1.17549435e-38f);
+      }
+      fence_to_async();
+      __syncwarp();
+      if (lane == 0) mbar_arrive1(bar(Q_READY));
+      auto convert = [&](int which, const unsigned char* raw, bool none) {
+#pragma unroll
+        for (int x = ct; x < TC_KEYS * (P / 16); x += 128) {
+          const int r = x / (P / 16), c = x % (P / 16);
+          const unsigned char* from = raw + (r / QKV_BLOCK) * BLOCK + (which * QKV_BLOCK + r % QKV_BLOCK) * P + ((c ^ qkv_turn(P / 16, r % QKV_BLOCK)) << 4);
+          convert16<SCHEME>(from, smem + (which ? C::V : C::K) + (c / 4) * TC_KEYS * 128 + r * 128, c % 4 * 2, r & 7, none);
         }
         fence_to_async();
         __syncwarp();
-        if (lane == 0) mbar_arrive1(bar(K_READY));
-        if (t) wait(PV_DONE, (t - 1) & 1);                   // and the values before these
-        convert(1);
-        fence_to_async();
-        __syncwarp();
-        if (lane == 0) mbar_arrive1(bar(V_READY));
-        asm volatile("bar.sync 1, 128;" ::: "memory");       // nobody reads the stage any more
-        if (ct == 0 && i + ST < seg_n) ask(i + ST);
-        if (none && ct == 0) v.status[0] = 1;
+        if (lane == 0) mbar_arrive1(bar(which ? V_READY : K_READY));
+      };
+      bool none = false;
+#pragma unroll 1
+      for (int i = 0; i <= seg_n; ++i) {
+        const unsigned t = n + i;
+        const bool none_before = none;
+        if (i - first == 32) { first = i; pages = next_pages; next_pages = pages_of(i + 32); }
+        if (i < seg_n) {                                     // keys of page i
+          none = page(i) < 0;
+          const unsigned char* raw = smem + C::RAW + t % ST * C::PAGE;
+          if (i) wait(S_FULL, (t - 1) & 1);
+          wait(RAW_FULL + t % ST, (t / ST) & 1);
+          // scales, and the largest exponent of those of values that count: 32 positions for each of two warps
+          if (ct < TC_KEYS) {
+            const float* from = reinterpret_cast<const float*>(raw + (ct / QKV_BLOCK) * BLOCK + 2 * QKV_BLOCK * P) + ct % QKV_BLOCK;
+            float* sc = s_scales + t % 3 * 2 * TC_KEYS;
+            const int key = (seg_a + i) * TC_KEYS + ct;
+            const float vs = none ? 0.f : from[QKV_BLOCK];
+            sc[ct] = none ? 0.f : from[0];
+            sc[TC_KEYS + ct] = vs;
+            const unsigned b = __float_as_uint(vs);
+            const unsigned top = __reduce_max_sync(0xffffffffu, key >= u.lo && key < u.hi && b < 0x7f800000u ? b : 0u);
+            if (lane == 0) s_meta[t % 3 * 4 + 1 + ct / 32] = (int)(top >> 23);
+            if (ct == 0) {
+              s_meta[t % 3 * 4] = !none;
+              if (none) v.status[0] = 1;
+            }
+          }
+          convert(0, raw, none);
+        }
+        if (i) {                                             // values of the page before
+          const unsigned t1 = t - 1;
+          if (t1) wait(PV_DONE, (t1 - 1) & 1);
+          convert(1, smem + C::RAW + t1 % ST * C::PAGE, none_before);
+          asm volatile("bar.sync 1, 128;" ::: "memory");     // nobody reads the stage any more
+          if (warp == 4 && i - 1 + ST < seg_n) ask(i - 1 + ST);
+        }
       }
       n += seg_n;
     } while (advance());
@@ -237,57 +282,20 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) qkv_attn_tc_kernel(QkvAtt
     do {
       begin();
       const int f = u.f0 + tid, tok = f < u.nf ? f / G : -1;
-      // queries of the warp's rows, eight at a time: a lane takes P / 32 channels
-      float rf = 0.f;
       const int away = tok < 0 ? 0 : a.tree.away(u.r0 + tok, tok);
       const unsigned long long seen = a.tree.seen && tok >= 0 ? a.tree.seen[a.tree.per_row ? u.r0 + tok : tok] : 0;
-#pragma unroll 1
-      for (int rb = 0; rb < 32; rb += 8) {
-        constexpr int W = P / 32;                            // 2 or 4 channels
-        float x[8][W];
-        unsigned top[8];
-#pragma unroll
-        for (int b = 0; b < 8; ++b) {
-          const int rt = __shfl_sync(0xffffffffu, tok, rb + b), rf_ = u.f0 + warp * 32 + rb + b;
-          const bf16* q = reinterpret_cast<const bf16*>(a.q) + ((long long)(u.r0 + max(rt, 0)) * v.H + sh.head * G + (rt < 0 ? 0 : rf_ - rt * G)) * v.d + W * lane;
-          uint2 w = make_uint2(0u, 0u);
-          if (rt >= 0 && W * lane < v.d) {
-            if (W == 4) w = *reinterpret_cast<const uint2*>(q); else w.x = *reinterpret_cast<const unsigned*>(q);
-          }
-          x[b][0] = __uint_as_float(w.x << 16); x[b][1] = __uint_as_float(w.x & 0xffff0000u);
-          if (W == 4) { x[b][W - 2] = __uint_as_float(w.y << 16); x[b][W - 1] = __uint_as_float(w.y & 0xffff0000u); }
-        }
-#pragma unroll
-        for (int b = 0; b < 8; ++b) {
-          top[b] = 0;
-#pragma unroll
-          for (int e = 0; e < W; ++e) top[b] = max(top[b], __float_as_uint(x[b][e]) & 0x7fffffffu);
-        }
-#pragma unroll
-        for (int b = 0; b < 8; ++b) top[b] = __reduce_max_sync(0xffffffffu, top[b]);
-#pragma unroll
-        for (int b = 0; b < 8; ++b) {
-          const int e = top[b] >= 0x7f800000u ? 140 : min(max((int)(top[b] >> 23), 27), 254), r = warp * 32 + rb + b, c = W * lane;   // not finite: left as it is
-          const float up = pow2(267 - e);
-          unsigned char* to = smem + C::Q + (c / 64) * TC_ROWS * 128 + r * 128 + (((c % 64 / 8) ^ (r & 7)) << 4) + (c % 8) * 2;
-          if (W == 4) *reinterpret_cast<uint2*>(to) = make_uint2(pack_f16(x[b][0] * up, x[b][1] * up), pack_f16(x[b][W - 2] * up, x[b][W - 1] * up));
-          else *reinterpret_cast<unsigned*>(to) = pack_f16(x[b][0] * up, x[b][1] * up);
-          if (lane == rb + b) rf = fmaxf(a.scale * 1.4426950408889634f * pow2(e - 13), 1.17549435e-38f);
-        }
-      }
-      fence_to_async();
-      __syncwarp();
-      if (lane == 0) mbar_arrive1(bar(Q_READY));
+      float rf = 0.f;
       float m = -CUDART_INF_F, l = 0.f;
       int R = 16;
 #pragma unroll 1
       for (int i = 0; i < seg_n; ++i) {
         const unsigned t = n + i;
-        const float* sc = s_scales + (t & 1) * 2 * TC_KEYS;
-        const int* meta = s_meta + (t & 1) * 4;
+        const float* sc = s_scales + t % 3 * 2 * TC_KEYS;
+        const int* meta = s_meta + t % 3 * 4;
         wait(S_FULL, t & 1);                                 // and with it the scales, written before the product was issued
         __syncwarp();
         tc_fence_after();
+        if (i == 0) rf = s_rf[(segs & 1) * TC_ROWS + tid];
         float x[TC_KEYS];
         tc_ld(lanes + C::S_COL, reinterpret_cast<unsigned*>(x));
         tc_ld(lanes + C::S_COL + 32, reinterpret_cast<unsigned*>(x) + 32);
