@@ -63,6 +63,10 @@ __device__ __forceinline__ void tc_st(unsigned at, const unsigned* x) {
 }
 #undef QKV_R32
 #undef QKV_I32
+// 32 bytes, a whole sector, of a row
+__device__ __forceinline__ void store32(void* p, const unsigned* x) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7]) : "memory");
+}
 __device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -197,30 +201,37 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) qkv_attn_tc_kernel(QkvAtt
       if (warp == 4)
         for (int i = 0; i < min(ST, seg_n); ++i) ask(i);
       if (n) wait(S_FULL, (n - 1) & 1);                      // the queries and keys before these have been multiplied
-      // a warp's 32 rows, eight at a time: four lanes a row, channels 16 k + 4 rc .. + 3 each
+      // a warp's 32 rows, 16 asked for at a time: four lanes a row, channels 16 k + 4 rc .. + 3 each
 #pragma unroll 1
-      for (int rb = 0; rb < 32; rb += 8) {
-        const int r = (warp - 4) * 32 + rb + rg, f = u.f0 + r, t = f / G;
-        const bool ok = f < u.nf;
-        const bf16* q = reinterpret_cast<const bf16*>(a.q) + ((long long)(u.r0 + (ok ? t : 0)) * v.H + sh.head * G + (ok ? f - t * G : 0)) * v.d + 4 * rc;
-        uint2 x[P / 16];
+      for (int rb = 0; rb < 32; rb += 16) {
+        uint2 x[2][P / 16];
 #pragma unroll
-        for (int k = 0; k < P / 16; ++k) x[k] = ok && 16 * k + 4 * rc < v.d ? *reinterpret_cast<const uint2*>(q + 16 * k) : make_uint2(0u, 0u);
-        unsigned top = 0;                                    // of the magnitudes' upper halves: all of a bf16
+        for (int h = 0; h < 2; ++h) {
+          const int f = u.f0 + (warp - 4) * 32 + rb + 8 * h + rg, t = f / G;
+          const bool ok = f < u.nf;
+          const bf16* q = reinterpret_cast<const bf16*>(a.q) + ((long long)(u.r0 + (ok ? t : 0)) * v.H + sh.head * G + (ok ? f - t * G : 0)) * v.d + 4 * rc;
 #pragma unroll
-        for (int k = 0; k < P / 16; ++k) top = __vmaxu2(top, __vmaxu2(x[k].x & 0x7fff7fffu, x[k].y & 0x7fff7fffu));
-        top = max(top >> 16, top & 0xffffu);
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        const int e = top >= 0x7f80u ? 140 : min(max((int)(top >> 7), 27), 254);           // a row that is not finite is left as it is
-        const float up = pow2(267 - e);
-#pragma unroll
-        for (int k = 0; k < P / 16; ++k) {
-          auto two = [&](unsigned w) { return pack_f16(__uint_as_float(w << 16) * up, __uint_as_float(w & 0xffff0000u) * up); };
-          const int c = 16 * k + 4 * rc;
-          *reinterpret_cast<uint2*>(smem + C::Q + (c / 64) * TC_ROWS * 128 + r * 128 + (((c % 64 / 8) ^ (r & 7)) << 4) + (c % 8) * 2) = make_uint2(two(x[k].x), two(x[k].y));
+          for (int k = 0; k < P / 16; ++k) x[h][k] = ok && 16 * k + 4 * rc < v.d ? *reinterpret_cast<const uint2*>(q + 16 * k) : make_uint2(0u, 0u);
         }
-        if (rc == 0) s_rf[(segs & 1) * TC_ROWS + r] = fmaxf(a.scale * 1.4426950408889634f * pow2(e - 13), 1.17549435e-38f);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int r = (warp - 4) * 32 + rb + 8 * h + rg;
+          unsigned top = 0;                                  // of the magnitudes' upper halves: all of a bf16
+#pragma unroll
+          for (int k = 0; k < P / 16; ++k) top = __vmaxu2(top, __vmaxu2(x[h][k].x & 0x7fff7fffu, x[h][k].y & 0x7fff7fffu));
+          top = max(top >> 16, top & 0xffffu);
+          top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          const int e = top >= 0x7f80u ? 140 : min(max((int)(top >> 7), 27), 254);         // a row that is not finite is left as it is
+          const float up = pow2(267 - e);
+#pragma unroll
+          for (int k = 0; k < P / 16; ++k) {
+            auto two = [&](unsigned w) { return pack_f16(__uint_as_float(w << 16) * up, __uint_as_float(w & 0xffff0000u) * up); };
+            const int c = 16 * k + 4 * rc;
+            *reinterpret_cast<uint2*>(smem + C::Q + (c / 64) * TC_ROWS * 128 + r * 128 + (((c % 64 / 8) ^ (r & 7)) << 4) + (c % 8) * 2) = make_uint2(two(x[h][k].x), two(x[h][k].y));
+          }
+          if (rc == 0) s_rf[(segs & 1) * TC_ROWS + r] = fmaxf(a.scale * 1.4426950408889634f * pow2(e - 13), 1.17549435e-38f);
+        }
       }
       fence_to_async();
       __syncwarp();
@@ -362,12 +373,12 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) qkv_attn_tc_kernel(QkvAtt
 #pragma unroll
         for (int c = 0; c < TC_KEYS; c += 4) {
           const float4 w = *reinterpret_cast<const float4*>(s_w + c);
-          float p[4], g[4] = {w.x, w.y, w.z, w.w};
+          float g[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
           for (int y = 0; y < 4; ++y) {
-            p[y] = ex2(fmaf(x[c + y], rf, -base));
-            sum[y] += p[y];
-            g[y] *= p[y];
+            const float p = ex2(fmaf(x[c + y], rf, -base));
+            sum[y] += p;
+            g[y] *= p;
             if (!full && x[c + y] == -CUDART_INF_F) g[y] = 0.f;                            // unseen: any scale, NaN too
           }
           pk[c / 2] = pack_f16(g[0], g[1]);
@@ -406,24 +417,38 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) qkv_attn_tc_kernel(QkvAtt
       const float r_inv = pow2(R - 10), inv = whole ? (l == 0.f ? 0.f : r_inv / l) : r_inv;
       bf16* out = reinterpret_cast<bf16*>(a.out) + ((long long)(u.r0 + max(tok, 0)) * v.H + sh.head * G + (f - max(tok, 0) * G)) * v.d;
       float* part_o = a.part_o + ((long long)part * TC_ROWS + tid) * P;
+      const bool wide = v.d % 16 == 0 && (reinterpret_cast<unsigned long long>(a.out) & 31) == 0;           // rows begin at whole sectors
 #pragma unroll 1
       for (int c = 0; c < P; c += 32) {
         unsigned o[32];
         __syncwarp();
         tc_ld(lanes + C::O_COL + c, o);
         tc_wait_ld();
+        if (tok >= 0) {
 #pragma unroll
-        for (int y = 0; y < 32; y += 8) {
-          if (tok < 0) break;
-          float r[8];
-#pragma unroll
-          for (int x = 0; x < 8; ++x) r[x] = l == 0.f ? 0.f : __uint_as_float(o[y + x]) * inv;       // nothing seen: zero
+          for (int y = 0; y < 32; ++y) o[y] = __float_as_uint(l == 0.f ? 0.f : __uint_as_float(o[y]) * inv);     // nothing seen: zero
           if (!whole) {
-            store4(part_o + c + y, make_float4(r[0], r[1], r[2], r[3]));
-            store4(part_o + c + y + 4, make_float4(r[4], r[5], r[6], r[7]));
-          } else if (c + y < v.d) {
-            const __nv_bfloat162 h[4] = {__floats2bfloat162_rn(r[0], r[1]), __floats2bfloat162_rn(r[2], r[3]), __floats2bfloat162_rn(r[4], r[5]), __floats2bfloat162_rn(r[6], r[7])};
-            *reinterpret_cast<uint4*>(out + c + y) = *reinterpret_cast<const uint4*>(h);
+#pragma unroll
+            for (int y = 0; y < 32; y += 8) store32(part_o + c + y, o + y);
+          } else {
+            unsigned h[16];
+#pragma unroll
+            for (int y = 0; y < 16; ++y) {
+              const __nv_bfloat162 w = __floats2bfloat162_rn(__uint_as_float(o[2 * y]), __uint_as_float(o[2 * y + 1]));
+              h[y] = *reinterpret_cast<const unsigned*>(&w);
+            }
+            if (wide) {
+#pragma unroll
+              for (int y = 0; y < 32; y += 16)
+                if (c + y < v.d) store32(out + c + y, h + y / 2);
+            } else {
+#pragma unroll
+              for (int y = 0; y < 32; y += 8)
+                if (c + y < v.d) {
+                  *reinterpret_cast<uint2*>(out + c + y) = make_uint2(h[y / 2], h[y / 2 + 1]);
+                  *reinterpret_cast<uint2*>(out + c + y + 4) = make_uint2(h[y / 2 + 2], h[y / 2 + 3]);
+                }
+            }
           }
         }
       }
