@@ -3,8 +3,8 @@
 // A CTA has nine warps.  Four convert: a page (64 positions) of codes, brought in by one bulk copy, becomes 16-bit floats in shared memory, keys
 // and values alike with 128-byte rows of 64 channels and the 128-byte swizzle -- the layout of a K-major operand for the keys
 // (S = Q K^T) and of an MN-major one for the values (O += P V).  One warp issues the products.  Four do the soft-max, a thread for a row: S
-// from TMEM, weights back to TMEM as the second product's A operand, results in TMEM.  S of the next page is computed while the weights of
-// this one are, and two CTAs share an SM.
+// from TMEM (twice, 32 columns at a time: all 64 in registers spilled), weights back to TMEM as the second product's A operand, results in
+// TMEM.  S of the next page is computed while the weights of this one are, and two CTAs share an SM.
 //
 // A row's reference maximum is moved only when a page's is more than 2^4 above it, so that the results in TMEM are seldom rescaled; weights
 // are at most 2^4 then, and taken relative to R (at least the largest scale of values, with room of 2^2) times 2^11: a half holds them down
@@ -23,7 +23,7 @@ struct TcCfg {
   static constexpr int Q = 0, K = Q + PANELS * TC_ROWS * 128, V = K + PANELS * TC_KEYS * 128, RAW = V + PANELS * TC_KEYS * 128, SCALES = RAW + STAGES * PAGE,
                        WEIGHTS = SCALES + 3 * 2 * TC_KEYS * 4, META = WEIGHTS + 4 * TC_KEYS * 4, FACTORS = META + 64, BARS = FACTORS + 2 * TC_ROWS * 4, SLOT = BARS + 16 * 8, PLAN = SLOT + 16,
                        SMEM = PLAN + (THREADS + 8) * 4 + 1024;        // the first 1024: the swizzle's alignment
-  static constexpr unsigned S_COL = 0, P_COL = 64, O_COL = 128;
+  static constexpr unsigned S_COL = 0, O_COL = 128;          // scores of even and odd pages, whose first half the weights take over; results
   static_assert(P % 64 == 0 && O_COL + P <= 256, "256 columns of TMEM for each of two CTAs");
   static_assert(TC_CTAS * TC_ROWS * P <= QKV_PART, "parts fit their place");
 };
@@ -61,6 +61,11 @@ __device__ __forceinline__ void tc_st(unsigned at, const unsigned* x) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
                "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};" ::QKV_I32(x), "r"(at) : "memory");
 }
+__device__ __forceinline__ void tc_st16(unsigned at, const unsigned* x) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15};"
+               ::"r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(x[4]), "r"(x[5]), "r"(x[6]), "r"(x[7]), "r"(x[8]), "r"(x[9]), "r"(x[10]), "r"(x[11]), "r"(x[12]), "r"(x[13]), "r"(x[14]),
+                 "r"(x[15]), "r"(at) : "memory");
+}
 #undef QKV_R32
 #undef QKV_I32
 // 32 bytes, a whole sector, of a row
@@ -94,16 +99,15 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) qkv_attn_tc_kernel(QkvAtt
   const unsigned s_base = (unsigned)__cvta_generic_to_shared(smem);
   const QkvView& v = a.v;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, G = v.H / v.KH;
-  enum { RAW_FULL = 0, K_READY = 4, V_READY, Q_READY, S_FULL, S_FREE, P_FULL, PV_DONE };
+  enum { RAW_FULL = 0, K_READY = 4, V_READY, Q_READY, S_FULL, P_FULL = S_FULL + 2, PV_DONE = P_FULL + 2, ALL_DONE = PV_DONE + 2 };         // the last three: of even and odd pages, as their waiters may be a page late
   auto bar = [&](int i) { return s_base + C::BARS + 8 * i; };
   float* s_scales = reinterpret_cast<float*>(smem + C::SCALES);            // [3][keys | values][64]: page t + 1's are written while t - 1's may still be read
   float* s_rf = reinterpret_cast<float*>(smem + C::FACTORS);               // [2][rows] r of a segment's rows
   int* s_meta = reinterpret_cast<int*>(smem + C::META);                    // [3][4]: page there, largest exponent of values' scales of either half
   if (tid == 0) {
     for (int i = 0; i < ST; ++i) mbar_init(bar(RAW_FULL + i), 1);
-    for (int i : {(int)K_READY, (int)V_READY, (int)Q_READY, (int)S_FREE, (int)P_FULL}) mbar_init(bar(i), 4);
-    mbar_init(bar(S_FULL), 1);
-    mbar_init(bar(PV_DONE), 1);
+    for (int i : {(int)K_READY, (int)V_READY, (int)Q_READY, (int)P_FULL, (int)P_FULL + 1}) mbar_init(bar(i), 4);
+    for (int i : {(int)S_FULL, (int)S_FULL + 1, (int)PV_DONE, (int)PV_DONE + 1, (int)ALL_DONE}) mbar_init(bar(i), 1);
   }
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   pdl_wait();
@@ -123,6 +127,8 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) qkv_attn_tc_kernel(QkvAtt
   auto wait = [&](int b, unsigned parity) {
     if (!mbar_try1(bar(b), parity) && !mbar_wait_long(bar(b), parity, dead ? 1000000ull : WAIT_CYCLES)) { dead = true; v.status[2] = 1; }
   };
+  auto wait_scores = [&](unsigned t) { wait(S_FULL + (t & 1), (t >> 1) & 1); };
+  auto wait_results = [&](unsigned t) { wait(PV_DONE + (t & 1), (t >> 1) & 1); };
   unsigned n = 0;                                            // pages gone through, the same count for all roles
   int seg_a, seg_n, segs = 0;
   auto begin = [&]() {
@@ -147,25 +153,24 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) qkv_attn_tc_kernel(QkvAtt
       const unsigned idesc_s = 1u << 4 | (unsigned)(TC_KEYS >> 3) << 17 | (unsigned)(TC_ROWS >> 4) << 24;
       const unsigned idesc_o = 1u << 4 | 1u << 16 | (unsigned)(P >> 3) << 17 | (unsigned)(TC_ROWS >> 4) << 24;
       auto scores = [&](unsigned t) {
-        wait(K_READY, t & 1);
-        if (t) wait(S_FREE, (t - 1) & 1);
+        wait(K_READY, t & 1);                                // the columns are free: O of page t - 2 was issued before
         tc_fence_after();
 #pragma unroll
         for (int p = 0; p < PANELS; ++p) {
           const unsigned long long da = tc_desc(s_base + C::Q + p * TC_ROWS * 128, 16), db = tc_desc(s_base + C::K + p * TC_KEYS * 128, 16);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) tc_mma_ss(tmem + C::S_COL, da + 2 * k, db + 2 * k, idesc_s, p || k);
+          for (int k = 0; k < 4; ++k) tc_mma_ss(tmem + C::S_COL + 64 * (t & 1), da + 2 * k, db + 2 * k, idesc_s, p || k);
         }
-        tc_commit(bar(S_FULL));
+        tc_commit(bar(S_FULL + (t & 1)));
       };
       auto results = [&](unsigned t, bool add) {
         wait(V_READY, t & 1);
-        wait(P_FULL, t & 1);
+        wait(P_FULL + (t & 1), (t >> 1) & 1);
         tc_fence_after();
         const unsigned long long db = tc_desc(s_base + C::V, TC_KEYS * 128);
 #pragma unroll
-        for (int k = 0; k < TC_KEYS / 16; ++k) tc_mma_ts(tmem + C::O_COL, tmem + C::P_COL + 8 * k, db + 128 * k, idesc_o, add || k);
-        tc_commit(bar(PV_DONE));
+        for (int k = 0; k < TC_KEYS / 16; ++k) tc_mma_ts(tmem + C::O_COL, tmem + C::S_COL + 64 * (t & 1) + 8 * k, db + 128 * k, idesc_o, add || k);
+        tc_commit(bar(PV_DONE + (t & 1)));
       };
       do {
         begin();
@@ -178,6 +183,8 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) qkv_attn_tc_kernel(QkvAtt
         results(n + seg_n - 1, seg_n > 1);
         n += seg_n;
       } while (advance());
+      tc_commit(bar(ALL_DONE));                              // no product is under way when the memory is given back, whatever became of the waits
+      wait(ALL_DONE, 0);
     }
   } else if (warp >= 4) {
     // ---- queries and codes to halves: the keys of page i + 1 before the values of page i
@@ -200,7 +207,7 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) qkv_attn_tc_kernel(QkvAtt
       };
       if (warp == 4)
         for (int i = 0; i < min(ST, seg_n); ++i) ask(i);
-      if (n) wait(S_FULL, (n - 1) & 1);                      // the queries and keys before these have been multiplied
+      if (n) wait_scores(n - 1);                      // the queries and keys before these have been multiplied
       // a warp's 32 rows, 16 asked for at a time: four lanes a row, channels 16 k + 4 rc .. + 3 each
 #pragma unroll 1
       for (int rb = 0; rb < 32; rb += 16) {
@@ -256,7 +263,7 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) qkv_attn_tc_kernel(QkvAtt
         if (i < seg_n) {                                     // keys of page i
           none = page(i) < 0;
           const unsigned char* raw = smem + C::RAW + t % ST * C::PAGE;
-          if (i) wait(S_FULL, (t - 1) & 1);
+          if (i) wait_scores(t - 1);
           wait(RAW_FULL + t % ST, (t / ST) & 1);
           // scales, and the largest exponent of those of values that count: 32 positions for each of two warps
           if (ct < TC_KEYS) {
@@ -278,7 +285,7 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) qkv_attn_tc_kernel(QkvAtt
         }
         if (i) {                                             // values of the page before
           const unsigned t1 = t - 1;
-          if (t1) wait(PV_DONE, (t1 - 1) & 1);
+          if (t1) wait_results(t1 - 1);
           convert(1, smem + C::RAW + t1 % ST * C::PAGE, none_before);
           asm volatile("bar.sync 1, 128;" ::: "memory");     // nobody reads the stage any more
           if (warp == 4 && i - 1 + ST < seg_n) ask(i - 1 + ST);
@@ -303,17 +310,11 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) qkv_attn_tc_kernel(QkvAtt
         const unsigned t = n + i;
         const float* sc = s_scales + t % 3 * 2 * TC_KEYS;
         const int* meta = s_meta + t % 3 * 4;
-        wait(S_FULL, t & 1);                                 // and with it the scales, written before the product was issued
+        wait_scores(t);                                      // and with them the scales, written before the product was issued
         __syncwarp();
         tc_fence_after();
         if (i == 0) rf = s_rf[(segs & 1) * TC_ROWS + tid];
-        float x[TC_KEYS];
-        tc_ld(lanes + C::S_COL, reinterpret_cast<unsigned*>(x));
-        tc_ld(lanes + C::S_COL + 32, reinterpret_cast<unsigned*>(x) + 32);
-        tc_wait_ld();
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive1(bar(S_FREE));
+        const unsigned at_s = lanes + C::S_COL + 64 * (t & 1);
         const int e = max(meta[1], meta[2]);
         float f_r = 1.f;
         if (e > R) {
@@ -324,42 +325,55 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) qkv_attn_tc_kernel(QkvAtt
         const float rs = pow2(264 - R);
         s_w[lane] = sc[TC_KEYS + lane] * rs;
         s_w[lane + 32] = sc[TC_KEYS + lane + 32] * rs;
-#pragma unroll
-        for (int c = 0; c < TC_KEYS; c += 4) {
-          const float4 k = *reinterpret_cast<const float4*>(sc + c);
-          x[c] *= k.x; x[c + 1] *= k.y; x[c + 2] *= k.z; x[c + 3] *= k.w;
-        }
         const int k0 = (seg_a + i) * TC_KEYS;
         const bool full = meta[0] && k0 >= u.full_lo && k0 + TC_KEYS <= u.full_hi;
+        unsigned see[2] = {~0u, ~0u};                        // which of the page's positions the row sees
         if (!full) {
-          // which of the page's positions the row sees, as bits
           auto range = [&](int lo, int hi) {                 // positions lo .. hi - 1
             const int p = min(max(lo - k0, 0), 64), q = min(max(hi - k0, 0), 64);
             return p >= q ? 0ull : (~0ull >> (64 - (q - p))) << p;
           };
-          unsigned long long see = 0;
+          unsigned long long all = 0;
           if (tok >= 0 && meta[0]) {
             const int from = a.window > 0 ? max(0, u.len + away - a.window + 1) : 0;
             if (a.tree.seen) {
               const int off = u.len - k0;                    // where the new rows begin in the page
               const unsigned long long rows = u.n >= 64 ? seen : seen & ((1ull << u.n) - 1);
-              see = range(from, u.len) | (off >= 64 || off <= -64 ? 0ull : off >= 0 ? rows << off : rows >> -off);
+              all = range(from, u.len) | (off >= 64 || off <= -64 ? 0ull : off >= 0 ? rows << off : rows >> -off);
             } else {
-              see = range(from, u.len + tok + 1);
+              all = range(from, u.len + tok + 1);
             }
-            see &= range(0, u.hi);
+            all &= range(0, u.hi);
           }
-          const unsigned lo = (unsigned)see, hi = (unsigned)(see >> 32);
-#pragma unroll
-          for (int c = 0; c < 32; ++c) {
-            if (!((lo >> c) & 1)) x[c] = -CUDART_INF_F;
-            if (!((hi >> c) & 1)) x[c + 32] = -CUDART_INF_F;
-          }
+          see[0] = (unsigned)all;
+          see[1] = (unsigned)(all >> 32);
         }
-        float mx[4] = {x[0], x[1], x[2], x[3]};
+        // scores of 32 positions, times the keys' scales; unseen: -inf
+        auto scores = [&](int h, float (&x)[32]) {
+          tc_ld(at_s + 32 * h, reinterpret_cast<unsigned*>(x));
+          tc_wait_ld();
 #pragma unroll
-        for (int c = 4; c < TC_KEYS; ++c) mx[c & 3] = fmaxf(mx[c & 3], x[c]);
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * rf;
+          for (int c = 0; c < 32; c += 4) {
+            const float4 k = *reinterpret_cast<const float4*>(sc + 32 * h + c);
+            x[c] *= k.x; x[c + 1] *= k.y; x[c + 2] *= k.z; x[c + 3] *= k.w;
+          }
+          if (!full)
+#pragma unroll
+            for (int c = 0; c < 32; ++c)
+              if (!((see[h] >> c) & 1)) x[c] = -CUDART_INF_F;
+          __syncwarp();
+        };
+        float top = -CUDART_INF_F;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          float x[32];
+          scores(h, x);
+          float mx[4] = {x[0], x[1], x[2], x[3]};
+#pragma unroll
+          for (int c = 4; c < 32; ++c) mx[c & 3] = fmaxf(mx[c & 3], x[c]);
+          top = fmaxf(top, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
+        }
+        top *= rf;
         float f_m = 1.f;
         if (top > m + 4.f || (m == -CUDART_INF_F && top > m)) {
           f_m = ex2(m - top);                                // from nothing: zero
@@ -367,29 +381,34 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) qkv_attn_tc_kernel(QkvAtt
           l *= f_m;
         }
         const float base = m == -CUDART_INF_F ? 0.f : m;     // nothing seen yet: every weight becomes exp2(-inf) = 0
-        unsigned pk[TC_KEYS / 2];
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
-        __syncwarp();                                        // s_w
 #pragma unroll
-        for (int c = 0; c < TC_KEYS; c += 4) {
-          const float4 w = *reinterpret_cast<const float4*>(s_w + c);
-          float g[4] = {w.x, w.y, w.z, w.w};
+        for (int h = 0; h < 2; ++h) {
+          float x[32];
+          unsigned pk[16];
+          scores(h, x);
 #pragma unroll
-          for (int y = 0; y < 4; ++y) {
-            const float p = ex2(fmaf(x[c + y], rf, -base));
-            sum[y] += p;
-            g[y] *= p;
-            if (!full && x[c + y] == -CUDART_INF_F) g[y] = 0.f;                            // unseen: any scale, NaN too
+          for (int c = 0; c < 32; c += 4) {
+            const float4 w = *reinterpret_cast<const float4*>(s_w + 32 * h + c);
+            float g[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+              const float p = ex2(fmaf(x[c + y], rf, -base));
+              sum[y] += p;
+              g[y] *= p;
+              if (!full && x[c + y] == -CUDART_INF_F) g[y] = 0.f;                          // unseen: any scale, NaN too
+            }
+            pk[c / 2] = pack_f16(g[0], g[1]);
+            pk[c / 2 + 1] = pack_f16(g[2], g[3]);
           }
-          pk[c / 2] = pack_f16(g[0], g[1]);
-          pk[c / 2 + 1] = pack_f16(g[2], g[3]);
+          tc_st16(at_s + 16 * h, pk);                        // over scores that have been read
         }
         l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
-        if (t) wait(PV_DONE, (t - 1) & 1);
-        __syncwarp();
-        tc_fence_after();
         const float f_o = f_m * f_r;
         if (i && __any_sync(0xffffffffu, f_o != 1.f)) {
+          wait_results(t - 1);
+          __syncwarp();
+          tc_fence_after();
 #pragma unroll 1
           for (int c = 0; c < P; c += 32) {
             unsigned o[32];
@@ -400,15 +419,14 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) qkv_attn_tc_kernel(QkvAtt
             tc_st(lanes + C::O_COL + c, o);
           }
         }
-        tc_st(lanes + C::P_COL, pk);
         tc_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive1(bar(P_FULL));
+        if (lane == 0) mbar_arrive1(bar(P_FULL + (t & 1)));
       }
       n += seg_n;
       // ---- a row's results
-      wait(PV_DONE, (n - 1) & 1);
+      wait_results(n - 1);
       __syncwarp();
       tc_fence_after();
       const int u_begin = sh.at - sh.tile;
