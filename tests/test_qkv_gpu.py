@@ -165,7 +165,7 @@ def check_attention(c, rng, lens, counts, dtype, parents=None, window=0, scale=N
         k = np.concatenate([old[b][0], R.in_8_bits(kv[at:at + n, 0], c.scheme)])
         v = np.concatenate([old[b][1], R.in_8_bits(kv[at:at + n, 1], c.scheme)])
         out, weight, reach = R.attention(q[at:at + n], k, v, lens[b], depth, seen, window, d ** -0.5 if scale is None else scale)
-        tol = R.tolerance(out, weight, reach, d, lens[b] + n, dtype)
+        tol = R.tolerance(out, weight, reach, d, lens[b] + n, dtype, c.scheme == "int8")
         worst = np.abs(got[at:at + n] - out) / tol
         assert np.isfinite(got[at:at + n]).all() and (worst <= 1).all(), (b, float(np.nanmax(worst)))
         at += n
@@ -469,3 +469,83 @@ def test_two_caches_on_one_context_do_not_meet():
     for x, y in outs:
         np.testing.assert_array_equal(x.numpy(), wa)
         np.testing.assert_array_equal(y.numpy(), wb)
+
+
+# ---- many rows of bf16, and shapes one after another ---------------------------------------------------------------------
+@pytest.mark.parametrize("scheme", ["int8", "fp8"])
+@pytest.mark.parametrize("H,KH,d,lens,T", [
+    (8, 2, 64, [4300, 5], 70),                             # units of 68 pages, cut among shares
+    (24, 1, 128, [9000], 5), (20, 1, 64, [6100, 0, 63], 1),  # one row block, few units: a unit in many shares
+    (4, 4, 128, [700, 64, 0, 1], 33), (2, 1, 40, [500], 20), (6, 2, 120, [129, 300], 9), (17, 1, 8, [400], 1),
+    (12, 3, 56, [3, 900], 31), (4, 1, 64, [0], 300)])
+def test_many_rows(scheme, H, KH, d, lens, T):
+    rng = np.random.default_rng(H * T + d)
+    c = new(len(lens), max(lens) + T, H, KH, d, scheme=scheme)
+    c.set_pages(rng.permutation(c.pages).reshape(len(lens), -1))
+    check_attention(c, rng, lens, [T] * len(lens), "bf16")
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("window", [1, 64, 100, 5000])
+def test_windows_of_many_rows(d, window):
+    rng = np.random.default_rng(window + d)
+    c = new(3, 900, 4, 2, d)
+    check_attention(c, rng, [800, 0, 90], [70] * 3, "bf16", window=window)
+    check_attention(c, rng, [800, 0, 90], [1, 70, 33], "bf16", window=window, ragged=True)
+
+
+def test_steps_of_every_shape_one_after_another():
+    """Units of 8 rows leave a list of cuts with high share numbers behind; those of 128 rows come next, with other places for their parts."""
+    rng = np.random.default_rng(15)
+    few, many = new(16, 2200, 16, 8, 64), new(4, 1500, 8, 1, 128, scheme="fp8")
+    exact = new(2, 900, 4, 1, 64, dtype="f32")
+    for _ in range(2):
+        check_attention(few, rng, [int(x) for x in rng.integers(1500, 2100, 16)], [1] * 16, "bf16")
+        check_attention(many, rng, [1300, 0, 70, 900], [16] * 4, "bf16", parents=R.TREE16)
+        check_attention(few, rng, [2100] * 4 + [30] * 12, [4] * 16, "bf16", window=1000)
+        check_attention(exact, rng, [600, 800], [40] * 2, "f32")
+        check_attention(many, rng, [1400, 3, 0, 600], [60] * 4, "bf16")
+        check_attention(few, rng, [2000] + [0] * 15, [10] * 16, "bf16")
+
+
+def test_shapes_in_turn_give_the_same_bits_without_waits_between_them():
+    """Launched back to back, nothing read between: each as by itself."""
+    rng = np.random.default_rng(16)
+    few, many = new(32, 3000, 16, 8, 64), new(8, 1600, 16, 4, 64)
+    fill(few, rng, [2900] * 32, "bf16", loud=False)
+    fill(many, rng, [1500] * 8, "bf16", loud=False)
+    few.set_lengths([2900 - 5] * 32)
+    many.set_lengths([1500 - 64] * 8)
+    rows = lambda *s: few.ctx.from_numpy(rng.integers(0x3c00, 0x4000, s).astype(np.uint16))
+    q1, q5, q16, q64 = rows(32, 1, 16, 64), rows(32, 5, 16, 64), rows(8, 16, 16, 64), rows(8, 64, 16, 64)
+    tree = many.tree(R.TREE16)
+    calls = [lambda: few.attention(q1), lambda: many.attention(q16, tree=tree), lambda: few.attention(q5, window=700), lambda: many.attention(q64), lambda: many.attention(q16, tree=tree)]
+    want = [f().numpy() for f in calls]
+    for _ in range(10):
+        for w, g in zip(want, [f() for f in calls]):
+            np.testing.assert_array_equal(g.numpy(), w)
+    few.check()
+    many.check()
+
+
+@pytest.mark.parametrize("scheme", ["int8", "fp8"])
+@pytest.mark.parametrize("d", [64, 128])
+def test_bad_heads_and_many_rows_of_bf16(scheme, d):
+    rng = np.random.default_rng(17)
+    for which in (0, 1):
+        c = new(1, 400, 4, 2, d, scheme=scheme)
+        kv = rng.normal(0, 1, (300, 2, 2, d)).astype(np.float32)
+        kv[20, which, 1, 5] = np.inf
+        kv[285, which, 0, 3] = np.nan
+        c.append(stored(kv, "bf16").reshape(1, 300, -1), queries=False)
+        c.set_lengths([270])
+        q = stored(rng.normal(0, 1, (1, 30, 4, d)), "bf16")
+        bad = np.isnan(back(c.attention(q, window=100))[0])
+        assert bad[15:, :2].all() and not bad[:15].any() and not bad[:, 2:].any()
+        bad = np.isnan(back(c.attention(q))[0])
+        assert bad[:, 2:].all() and bad[15:, :2].all() and not bad[:15, :2].any()
+    q[0, 14, 2, 0] = np.inf
+    q[0, 4, 0, 7] = np.nan
+    c.set_lengths([0])
+    bad = np.isnan(back(c.attention(q))[0]).any(-1)
+    assert bad[14, 2] and bad[4, 0] and bad[:20].sum() == 2 and bad[20:, 2:].all() and not bad[20:, :2].any()

@@ -524,7 +524,9 @@ __global__ void __launch_bounds__(THREADS, (AttnCfg<T, P, NT, RS>::CTAS)) qkv_at
 
 // Parts of the units that were cut, in the order of their shares: a warp for a row, or, with many parts, a CTA.  The last CTA empties
 // the lists.  The kernel begins while the shares end; it goes through the motions once before it waits for them, so that its
-// instructions are there (without that a row took 3 us, most of it fetching them).  rmax: rows of a unit at most
+// instructions are there (without that a row took 3 us, most of it fetching them).  That first pass takes a cut of constants, never one from
+// the list: what stands there then is an earlier call's, whose shares with other rows lie beyond this call's parts.  Parts are read from L2, as the
+// first pass has brought some of them before they were written.  rmax: rows of a unit at most
 template <typename T, int P>
 __global__ void __launch_bounds__(32 * MERGE_WARPS) qkv_merge_kernel(QkvAttnArgs a, int RT, int rmax) {
   constexpr int Y = P > 128 ? 2 : 1, IN = Y > 1 ? 8 : 16;    // parts asked for at a time
@@ -547,7 +549,7 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) qkv_merge_kernel(QkvAttnArgs
       const bool many = x0 >= 0;
       if (!many && few >= n_few) continue;
       if (many) o = a.cuts[a.max_cuts - 1 - x0 / rmax];
-      else if (item != blockIdx.x) o = a.cuts[few / rmax];
+      else if (pass && item != blockIdx.x) o = a.cuts[few / rmax];
       const int r = many ? x0 % rmax : few % rmax;
       if (r >= min(RT, o.nf - o.f0)) continue;               // many: the same for all warps
       const int step = many ? MERGE_WARPS : 1, own = many ? warp : 0;        // this warp's parts: own, own + step, ..
@@ -560,7 +562,7 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) qkv_merge_kernel(QkvAttnArgs
         for (int j0 = lane; j0 < o.n; j0 += 256) {
           float x[8];
 #pragma unroll
-          for (int e = 0; e < 8; ++e) x[e] = a.part_ml[at(min(j0 + 32 * e, o.n - 1))].x;
+          for (int e = 0; e < 8; ++e) x[e] = __ldcg(a.part_ml + at(min(j0 + 32 * e, o.n - 1))).x;
 #pragma unroll
           for (int e = 0; e < 8; ++e) m = fmaxf(m, x[e]);
         }
@@ -572,10 +574,10 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) qkv_merge_kernel(QkvAttnArgs
 #pragma unroll
           for (int y = 0; y < Y; ++y) {
             const int c = 4 * lane + 128 * y;
-            x[j][y] = c < P ? *reinterpret_cast<const float4*>(a.part_o + at(min(j0 + j * step, o.n - 1)) * P + c) : make_float4(0.f, 0.f, 0.f, 0.f);
+            x[j][y] = c < P ? __ldcg(reinterpret_cast<const float4*>(a.part_o + at(min(j0 + j * step, o.n - 1)) * P + c)) : make_float4(0.f, 0.f, 0.f, 0.f);
           }
         float2 ml = make_float2(-CUDART_INF_F, 0.f);
-        if (lane < IN && j0 + lane * step < o.n) ml = a.part_ml[at(j0 + lane * step)];
+        if (lane < IN && j0 + lane * step < o.n) ml = __ldcg(a.part_ml + at(j0 + lane * step));
         if (j0 == own) {
           m = fmaxf(m, ml.x);
 #pragma unroll
