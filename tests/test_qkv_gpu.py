@@ -491,6 +491,7 @@ def test_windows_of_many_rows(d, window):
     rng = np.random.default_rng(window + d)
     c = new(3, 900, 4, 2, d)
     check_attention(c, rng, [800, 0, 90], [70] * 3, "bf16", window=window)
+    check_attention(c, rng, [800, 0, 90], [16] * 3, "bf16", window=window, parents=R.TREE16)
     check_attention(c, rng, [800, 0, 90], [1, 70, 33], "bf16", window=window, ragged=True)
 
 

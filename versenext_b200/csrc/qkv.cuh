@@ -77,6 +77,13 @@ struct QkvTree {
   const int* depth = nullptr;
   int per_row = 0;                                  // the tables go by the row of the step, else by its place in its entry
   __device__ __forceinline__ int away(int row, int i) const { return depth ? depth[per_row ? row : i] : i; }
+  // rows that a row sees through a window: of a path, parents before children, the last ones
+  __device__ __forceinline__ unsigned long long sees(int row, int i, int window) const {
+    unsigned long long s = seen[per_row ? row : i];
+    if (window > 0)
+      for (int n = __popcll(s); n > window; --n) s &= s - 1;
+    return s;
+  }
 };
 
 struct vn_qkv {

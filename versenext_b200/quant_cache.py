@@ -253,7 +253,7 @@ class QuantKVCache:
     def attention(self, q, step: Optional[Step] = None, tree: Optional[Tree] = None, window: int = 0, scale: Optional[float] = None, out: Optional[DeviceArray] = None) -> DeviceArray:
         """softmax(scale q k^T) v of a step's queries (.., n_head, head_dim) over the committed positions and the step's own rows, which
         `append` has written: row i of an entry sees the rows up to itself, or its ancestors in `tree`.  window > 0: only the last
-        `window` positions.  scale: 1 / sqrt(head_dim) unless given.  A row that sees nothing gets zeros."""
+        `window` positions, of its path where there is a tree.  scale: 1 / sqrt(head_dim) unless given.  A row that sees nothing gets zeros."""
         q = self._in(q)
         E, ents, row_ent, T, M = self._rows(q.shape, (self.n_head, self.head_dim), step)
         seen, depth, per_row = self._tree(tree, step, T, M)
