@@ -574,7 +574,8 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS) qkv_merge_kernel(QkvAttnArgs
 #pragma unroll
           for (int y = 0; y < Y; ++y) {
             const int c = 4 * lane + 128 * y;
-            x[j][y] = c < P ? __ldcg(reinterpret_cast<const float4*>(a.part_o + at(min(j0 + j * step, o.n - 1)) * P + c)) : make_float4(0.f, 0.f, 0.f, 0.f);
+            x[j][y] = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (c < P && j0 + j * step < o.n) x[j][y] = __ldcg(reinterpret_cast<const float4*>(a.part_o + at(j0 + j * step) * P + c));
           }
         float2 ml = make_float2(-CUDART_INF_F, 0.f);
         if (lane < IN && j0 + lane * step < o.n) ml = __ldcg(a.part_ml + at(j0 + lane * step));

@@ -1,10 +1,11 @@
 // Attention over the 8-bit cache for many rows (prompts, trees): 128 rows of a unit on tcgen05.
 //
-// A CTA has nine warps.  Four convert: a page (64 positions) of codes, brought in by one bulk copy, becomes 16-bit floats in shared memory, keys
+// A CTA has thirteen warps.  Four convert: a page (64 positions) of codes, brought in by one bulk copy, becomes 16-bit floats in shared memory, keys
 // and values alike with 128-byte rows of 64 channels and the 128-byte swizzle -- the layout of a K-major operand for the keys
-// (S = Q K^T) and of an MN-major one for the values (O += P V).  One warp issues the products.  Four do the soft-max, a thread for a row: S
-// from TMEM (twice, 32 columns at a time: all 64 in registers spilled), weights back to TMEM as the second product's A operand, results in
-// TMEM.  S of the next page is computed while the weights of this one are, and two CTAs share an SM.
+// (S = Q K^T) and of an MN-major one for the values (O += P V).  One warp issues the products.  Eight do the soft-max, two threads for a row, 32
+// columns each: S from TMEM, weights back to TMEM as the second product's A operand, results in TMEM (2 x 1000
+// rows behind 1500 positions, 16 heads of 128 channels: 73 us; four warps with 64 columns a thread 76).  S of the next page is computed while the weights of this one are, and two
+// CTAs share an SM.
 //
 // A row's reference maximum is moved only when a page's is more than 2^4 above it, so that the results in TMEM are seldom rescaled; weights
 // are at most 2^4 then, and taken relative to R (at least the largest scale of values, with room of 2^2) times 2^11: a half holds them down
@@ -14,14 +15,14 @@
 
 namespace qkv_detail {
 
-constexpr int TC_ROWS = 128, TC_KEYS = KV_PAGE, TC_THREADS = 288, TC_CTAS = 2;
+constexpr int TC_ROWS = 128, TC_KEYS = KV_PAGE, TC_SOFT = 8, TC_THREADS = 32 * (TC_SOFT + 5), TC_CTAS = 2;      // TC_SOFT warps, four that convert, one that issues
 constexpr int TC_MIN_SHARE = 2, TC_UNCUT = 4;       // pages of a share at least; of a unit that is never cut
 
 template <int P>
 struct TcCfg {
   static constexpr int PANELS = P / 64, PAGE = 2 * QKV_BLOCK * (2 * P + 8), STAGES = P > 64 ? 2 : 3;
   static constexpr int Q = 0, K = Q + PANELS * TC_ROWS * 128, V = K + PANELS * TC_KEYS * 128, RAW = V + PANELS * TC_KEYS * 128, SCALES = RAW + STAGES * PAGE,
-                       WEIGHTS = SCALES + 3 * 2 * TC_KEYS * 4, META = WEIGHTS + 4 * TC_KEYS * 4, FACTORS = META + 64, BARS = FACTORS + 2 * TC_ROWS * 4, SLOT = BARS + 16 * 8, PLAN = SLOT + 16,
+                       WEIGHTS = SCALES + 3 * 2 * TC_KEYS * 4, META = WEIGHTS + TC_SOFT * 32 * 4, FACTORS = META + 64, PAIRS = FACTORS + 2 * TC_ROWS * 4, BARS = PAIRS + 2 * 2 * TC_ROWS * 4, SLOT = BARS + 16 * 8, PLAN = SLOT + 16,
                        SMEM = PLAN + (THREADS + 8) * 4 + 1024;        // the first 1024: the swizzle's alignment
   static constexpr unsigned S_COL = 0, O_COL = 128;          // scores of even and odd pages, whose first half the weights take over; results
   static_assert(P % 64 == 0 && O_COL + P <= 256, "256 columns of TMEM for each of two CTAs");
@@ -106,7 +107,8 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) qkv_attn_tc_kernel(QkvAtt
   int* s_meta = reinterpret_cast<int*>(smem + C::META);                    // [3][4]: page there, largest exponent of values' scales of either half
   if (tid == 0) {
     for (int i = 0; i < ST; ++i) mbar_init(bar(RAW_FULL + i), 1);
-    for (int i : {(int)K_READY, (int)V_READY, (int)Q_READY, (int)P_FULL, (int)P_FULL + 1}) mbar_init(bar(i), 4);
+    for (int i : {(int)K_READY, (int)V_READY, (int)Q_READY}) mbar_init(bar(i), 4);
+    for (int i : {(int)P_FULL, (int)P_FULL + 1}) mbar_init(bar(i), TC_SOFT);
     for (int i : {(int)S_FULL, (int)S_FULL + 1, (int)PV_DONE, (int)PV_DONE + 1, (int)ALL_DONE}) mbar_init(bar(i), 1);
   }
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -115,7 +117,7 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) qkv_attn_tc_kernel(QkvAtt
   Share sh;
   if (!find_share<TC_ROWS, TC_KEYS>(a, rts, split, TC_MIN_SHARE, blockIdx.x, gridDim.x, reinterpret_cast<int*>(smem + C::PLAN), u, sh)) return;
   unsigned* s_slot = reinterpret_cast<unsigned*>(smem + C::SLOT);
-  if (warp == 8) {
+  if (warp == TC_SOFT + 4) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s_base + C::SLOT), "r"(256u) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
@@ -147,7 +149,7 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) qkv_attn_tc_kernel(QkvAtt
     return true;
   };
 
-  if (warp == 8) {
+  if (warp == TC_SOFT + 4) {
     // ---- products: S of page i + 1 before O of page i
     if (lane == 0) {
       const unsigned idesc_s = 1u << 4 | (unsigned)(TC_KEYS >> 3) << 17 | (unsigned)(TC_ROWS >> 4) << 24;
@@ -186,9 +188,9 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) qkv_attn_tc_kernel(QkvAtt
       tc_commit(bar(ALL_DONE));                              // no product is under way when the memory is given back, whatever became of the waits
       wait(ALL_DONE, 0);
     }
-  } else if (warp >= 4) {
+  } else if (warp >= TC_SOFT) {
     // ---- queries and codes to halves: the keys of page i + 1 before the values of page i
-    const int ct = tid - 128, rg = lane >> 2, rc = lane & 3;
+    const int ct = tid - 32 * TC_SOFT, cw = warp - TC_SOFT, rg = lane >> 2, rc = lane & 3;
     unsigned asked = 0;                                      // pages asked for in all
     do {
       begin();
@@ -205,7 +207,7 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) qkv_attn_tc_kernel(QkvAtt
         if (pg >= 0 && !dead) fetch_block(s_base + C::RAW + s * C::PAGE, v.block(pg, sh.head, 0), C::PAGE, bar(RAW_FULL + s));
         else mbar_arrive1(bar(RAW_FULL + s));
       };
-      if (warp == 4)
+      if (cw == 0)
         for (int i = 0; i < min(ST, seg_n); ++i) ask(i);
       if (n) wait_scores(n - 1);                      // the queries and keys before these have been multiplied
       // a warp's 32 rows, 16 asked for at a time: four lanes a row, channels 16 k + 4 rc .. + 3 each
@@ -214,7 +216,7 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) qkv_attn_tc_kernel(QkvAtt
         uint2 x[2][P / 16];
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int f = u.f0 + (warp - 4) * 32 + rb + 8 * h + rg, t = f / G;
+          const int f = u.f0 + cw * 32 + rb + 8 * h + rg, t = f / G;
           const bool ok = f < u.nf;
           const bf16* q = reinterpret_cast<const bf16*>(a.q) + ((long long)(u.r0 + (ok ? t : 0)) * v.H + sh.head * G + (ok ? f - t * G : 0)) * v.d + 4 * rc;
 #pragma unroll
@@ -222,7 +224,7 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) qkv_attn_tc_kernel(QkvAtt
         }
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const int r = (warp - 4) * 32 + rb + 8 * h + rg;
+          const int r = cw * 32 + rb + 8 * h + rg;
           unsigned top = 0;                                  // of the magnitudes' upper halves: all of a bf16
 #pragma unroll
           for (int k = 0; k < P / 16; ++k) top = __vmaxu2(top, __vmaxu2(x[h][k].x & 0x7fff7fffu, x[h][k].y & 0x7fff7fffu));
@@ -287,34 +289,48 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) qkv_attn_tc_kernel(QkvAtt
           const unsigned t1 = t - 1;
           if (t1) wait_results(t1 - 1);
           convert(1, smem + C::RAW + t1 % ST * C::PAGE, none_before);
+          __syncwarp();
           asm volatile("bar.sync 1, 128;" ::: "memory");     // nobody reads the stage any more
-          if (warp == 4 && i - 1 + ST < seg_n) ask(i - 1 + ST);
+          if (cw == 0 && i - 1 + ST < seg_n) ask(i - 1 + ST);
         }
       }
       n += seg_n;
     } while (advance());
   } else {
-    // ---- soft-max: thread = row
-    const unsigned lanes = tmem + ((unsigned)(warp * 32) << 16);
-    float* s_w = reinterpret_cast<float*>(smem + C::WEIGHTS) + warp * TC_KEYS;             // the page's scales of values, relative to R
+    // ---- soft-max: warps w and w + 4 have the two halves of the columns of rows 32 (w mod 4) ..
+    const int half = warp >> 2, row = tid & 127;
+    const unsigned lanes = tmem + ((unsigned)(warp % 4 * 32) << 16);
+    float* s_w = reinterpret_cast<float*>(smem + C::WEIGHTS) + warp * 32;                  // the page's scales of values, relative to R
+    float* s_pair = reinterpret_cast<float*>(smem + C::PAIRS);                             // [2][halves][rows], turn about
+    unsigned turn = 0;
+    auto exchange = [&](float x) {                           // the other half's
+      float* p = s_pair + (turn++ & 1) * 2 * TC_ROWS;
+      p[half * TC_ROWS + row] = x;
+      tc_fence_before();
+      __syncwarp();
+      asm volatile("bar.sync %0, 64;" ::"r"(2 + warp % 4) : "memory");
+      tc_fence_after();
+      return p[(half ^ 1) * TC_ROWS + row];
+    };
     do {
       begin();
-      const int f = u.f0 + tid, tok = f < u.nf ? f / G : -1;
+      const int f = u.f0 + row, tok = f < u.nf ? f / G : -1;
       const int away = tok < 0 ? 0 : a.tree.away(u.r0 + tok, tok);
       const unsigned long long seen = a.tree.seen && tok >= 0 ? a.tree.sees(u.r0 + tok, tok, a.window) : 0;
-      float rf = 0.f;
-      float m = -CUDART_INF_F, l = 0.f;
+      float rf = 0.f, m = -CUDART_INF_F, l = 0.f;
       int R = 16;
 #pragma unroll 1
       for (int i = 0; i < seg_n; ++i) {
         const unsigned t = n + i;
-        const float* sc = s_scales + t % 3 * 2 * TC_KEYS;
+        const float* sc = s_scales + t % 3 * 2 * TC_KEYS + 32 * half;
         const int* meta = s_meta + t % 3 * 4;
         wait_scores(t);                                      // and with them the scales, written before the product was issued
         __syncwarp();
         tc_fence_after();
-        if (i == 0) rf = s_rf[(segs & 1) * TC_ROWS + tid];
+        if (i == 0) rf = s_rf[(segs & 1) * TC_ROWS + row];
         const unsigned at_s = lanes + C::S_COL + 64 * (t & 1);
+        float x[32];
+        tc_ld(at_s + 32 * half, reinterpret_cast<unsigned*>(x));
         const int e = max(meta[1], meta[2]);
         float f_r = 1.f;
         if (e > R) {
@@ -322,58 +338,42 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) qkv_attn_tc_kernel(QkvAtt
           f_r = pow2(127 + R - to);
           R = to;
         }
-        const float rs = pow2(264 - R);
-        s_w[lane] = sc[TC_KEYS + lane] * rs;
-        s_w[lane + 32] = sc[TC_KEYS + lane + 32] * rs;
+        s_w[lane] = sc[TC_KEYS + lane] * pow2(264 - R);
         const int k0 = (seg_a + i) * TC_KEYS;
         const bool full = meta[0] && k0 >= u.full_lo && k0 + TC_KEYS <= u.full_hi;
-        unsigned see[2] = {~0u, ~0u};                        // which of the page's positions the row sees
-        if (!full) {
+        tc_wait_ld();
+#pragma unroll
+        for (int c = 0; c < 32; c += 4) {
+          const float4 k = *reinterpret_cast<const float4*>(sc + c);
+          x[c] *= k.x; x[c + 1] *= k.y; x[c + 2] *= k.z; x[c + 3] *= k.w;
+        }
+        if (!full) {                                         // which of the positions the row sees, as bits
+          const int h0 = k0 + 32 * half;
           auto range = [&](int lo, int hi) {                 // positions lo .. hi - 1
-            const int p = min(max(lo - k0, 0), 64), q = min(max(hi - k0, 0), 64);
-            return p >= q ? 0ull : (~0ull >> (64 - (q - p))) << p;
+            const int p = min(max(lo - h0, 0), 32), q = min(max(hi - h0, 0), 32);
+            return p >= q ? 0u : (~0u >> (32 - (q - p))) << p;
           };
-          unsigned long long all = 0;
+          unsigned see = 0;
           if (tok >= 0 && meta[0]) {
             const int from = a.window > 0 ? max(0, u.len + away - a.window + 1) : 0;
             if (a.tree.seen) {
-              const int off = u.len - k0;                    // where the new rows begin in the page
+              const int off = u.len - h0;                    // where the new rows begin
               const unsigned long long rows = u.n >= 64 ? seen : seen & ((1ull << u.n) - 1);
-              all = range(from, u.len) | (off >= 64 || off <= -64 ? 0ull : off >= 0 ? rows << off : rows >> -off);
+              see = range(from, u.len) | (off >= 32 || off <= -64 ? 0u : off >= 0 ? (unsigned)(rows << off) : (unsigned)(rows >> -off));
             } else {
-              all = range(from, u.len + tok + 1);
+              see = range(from, u.len + tok + 1);
             }
-            all &= range(0, u.hi);
+            see &= range(0, u.hi);
           }
-          see[0] = (unsigned)all;
-          see[1] = (unsigned)(all >> 32);
+#pragma unroll
+          for (int c = 0; c < 32; ++c)
+            if (!((see >> c) & 1)) x[c] = -CUDART_INF_F;
         }
-        // scores of 32 positions, times the keys' scales; unseen: -inf
-        auto scores = [&](int h, float (&x)[32]) {
-          tc_ld(at_s + 32 * h, reinterpret_cast<unsigned*>(x));
-          tc_wait_ld();
+        float mx[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
-          for (int c = 0; c < 32; c += 4) {
-            const float4 k = *reinterpret_cast<const float4*>(sc + 32 * h + c);
-            x[c] *= k.x; x[c + 1] *= k.y; x[c + 2] *= k.z; x[c + 3] *= k.w;
-          }
-          if (!full)
-#pragma unroll
-            for (int c = 0; c < 32; ++c)
-              if (!((see[h] >> c) & 1)) x[c] = -CUDART_INF_F;
-          __syncwarp();
-        };
-        float top = -CUDART_INF_F;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float x[32];
-          scores(h, x);
-          float mx[4] = {x[0], x[1], x[2], x[3]};
-#pragma unroll
-          for (int c = 4; c < 32; ++c) mx[c & 3] = fmaxf(mx[c & 3], x[c]);
-          top = fmaxf(top, fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])));
-        }
-        top *= rf;
+        for (int c = 4; c < 32; ++c) mx[c & 3] = fmaxf(mx[c & 3], x[c]);
+        float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+        top = fmaxf(top, exchange(top)) * rf;                // both halves come to the same
         float f_m = 1.f;
         if (top > m + 4.f || (m == -CUDART_INF_F && top > m)) {
           f_m = ex2(m - top);                                // from nothing: zero
@@ -382,35 +382,31 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) qkv_attn_tc_kernel(QkvAtt
         }
         const float base = m == -CUDART_INF_F ? 0.f : m;     // nothing seen yet: every weight becomes exp2(-inf) = 0
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        unsigned pk[16];
+        __syncwarp();                                        // s_w
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          float x[32];
-          unsigned pk[16];
-          scores(h, x);
+        for (int c = 0; c < 32; c += 4) {
+          const float4 w = *reinterpret_cast<const float4*>(s_w + c);
+          float g[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-          for (int c = 0; c < 32; c += 4) {
-            const float4 w = *reinterpret_cast<const float4*>(s_w + 32 * h + c);
-            float g[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-            for (int y = 0; y < 4; ++y) {
-              const float p = ex2(fmaf(x[c + y], rf, -base));
-              sum[y] += p;
-              g[y] *= p;
-              if (!full && x[c + y] == -CUDART_INF_F) g[y] = 0.f;                          // unseen: any scale, NaN too
-            }
-            pk[c / 2] = pack_f16(g[0], g[1]);
-            pk[c / 2 + 1] = pack_f16(g[2], g[3]);
+          for (int y = 0; y < 4; ++y) {
+            const float p = ex2(fmaf(x[c + y], rf, -base));
+            sum[y] += p;
+            g[y] *= p;
+            if (!full && x[c + y] == -CUDART_INF_F) g[y] = 0.f;                            // unseen: any scale, NaN too
           }
-          tc_st16(at_s + 16 * h, pk);                        // over scores that have been read
+          pk[c / 2] = pack_f16(g[0], g[1]);
+          pk[c / 2 + 1] = pack_f16(g[2], g[3]);
         }
+        tc_st16(at_s + 16 * half, pk);                       // over the first half's scores, which that half has read: both have exchanged their maxima
         l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
         const float f_o = f_m * f_r;
-        if (i && __any_sync(0xffffffffu, f_o != 1.f)) {
+        if (i && __any_sync(0xffffffffu, f_o != 1.f)) {      // the same for both halves
           wait_results(t - 1);
           __syncwarp();
           tc_fence_after();
 #pragma unroll 1
-          for (int c = 0; c < P; c += 32) {
+          for (int c = half * (P / 2); c < (half + 1) * (P / 2); c += 32) {
             unsigned o[32];
             tc_ld(lanes + C::O_COL + c, o);
             tc_wait_ld();
@@ -425,7 +421,8 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) qkv_attn_tc_kernel(QkvAtt
         if (lane == 0) mbar_arrive1(bar(P_FULL + (t & 1)));
       }
       n += seg_n;
-      // ---- a row's results
+      // ---- a row's results, half of the channels each
+      l += exchange(l);
       wait_results(n - 1);
       __syncwarp();
       tc_fence_after();
@@ -434,10 +431,10 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) qkv_attn_tc_kernel(QkvAtt
       const int last = whole ? 0 : (u_begin + u.tiles - 1) / sh.share, part = 2 * blockIdx.x + (begun ? 1 : 0);
       const float r_inv = pow2(R - 10), inv = whole ? (l == 0.f ? 0.f : r_inv / l) : r_inv;
       bf16* out = reinterpret_cast<bf16*>(a.out) + ((long long)(u.r0 + max(tok, 0)) * v.H + sh.head * G + (f - max(tok, 0) * G)) * v.d;
-      float* part_o = a.part_o + ((long long)part * TC_ROWS + tid) * P;
+      float* part_o = a.part_o + ((long long)part * TC_ROWS + row) * P;
       const bool wide = v.d % 16 == 0 && (reinterpret_cast<unsigned long long>(a.out) & 31) == 0;           // rows begin at whole sectors
 #pragma unroll 1
-      for (int c = 0; c < P; c += 32) {
+      for (int c = half * (P / 2); c < (half + 1) * (P / 2); c += 32) {
         unsigned o[32];
         __syncwarp();
         tc_ld(lanes + C::O_COL + c, o);
@@ -470,7 +467,7 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) qkv_attn_tc_kernel(QkvAtt
           }
         }
       }
-      if (!whole && tok >= 0) a.part_ml[part * TC_ROWS + tid] = make_float2(m, l);
+      if (!whole && tok >= 0 && half == 0) a.part_ml[part * TC_ROWS + row] = make_float2(m, l);
       if (begun && tid == 0) {                               // a unit to merge: in any order, each by itself
         const int cnt = last - (int)blockIdx.x + 1;
         const bool many = cnt > MANY;
@@ -482,7 +479,7 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) qkv_attn_tc_kernel(QkvAtt
   tc_fence_before();
   __syncthreads();
   __syncwarp();
-  if (warp == 8) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256u) : "memory");
+  if (warp == TC_SOFT + 4) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(256u) : "memory");
 }
 
 template <int SCHEME, int P>
