@@ -446,7 +446,7 @@ int32_t vn_qkv_lengths(vn_qkv* c, int32_t* out_host);                           
 int32_t vn_qkv_set_lengths(vn_qkv* c, const int32_t* lens, int32_t on_device);         /* [max_batch] */
 /* Conditions met by kernels since the last call, read after a stream synchronisation and cleared: *no_room: a position behind
  * the capacity or without a page was to be written or read (VN_ERR_OVERFLOW); *bad_index: a sequence, row, count or kept row
- * out of range (VN_ERR_INDEX). */
+ * out of range (VN_ERR_INDEX).  VN_ERR_TIMEOUT: a copy from the cache did not arrive; that call's results are no good. */
 int32_t vn_qkv_status(vn_qkv* c, int32_t* no_room, int32_t* bad_index);
 /* Writes a step's keys and values at positions length + offset + i; lengths stay.  rows_dev [M][ld]: the H query heads (only with
  * queries != 0), the KH key heads, the KH value heads.  In the same pass, for query and key heads: x / sqrt(mean x^2 + eps) * norm
@@ -458,7 +458,8 @@ int32_t vn_qkv_append(vn_qkv* c, const void* rows_dev, int64_t ld, int32_t queri
                       int32_t interleaved, void* q_out_dev);
 /* out = softmax(scale q k^T) v over the committed positions and the rows of the same step (appended at offset 0); query head h
  * reads key/value head h / (H / KH).  window > 0: row at position p sees position j only if p - j < window (in a tree too:
- * of a row and its ancestors, parents before children, the last `window`).  A row that sees nothing gets zeros.  q_dev, out_dev [M, H, head_dim], 16-byte (float32) / 8-byte aligned. */
+ * of a row and its ancestors, parents before children, the last `window`).  A row that sees nothing gets zeros.  q_dev, out_dev
+ * [M, H, head_dim], 16-byte (float32) / 8-byte aligned.  All caches of a context share one workspace, on its stream. */
 int32_t vn_qkv_attention(vn_qkv* c, const void* q_dev, int32_t n_ent, const int32_t* ents_dev, const int32_t* row_ent_dev, int32_t T, int32_t M,
                          const uint64_t* seen_dev, const int32_t* depth_dev, int32_t tree_per_row, int32_t window, float scale, void* out_dev);
 /* Values of a step's positions, [M, KH, head_dim] each, dtype VN_F32 or VN_BF16.  Row i of an entry reads position start + i;
