@@ -550,3 +550,12 @@ def test_bad_heads_and_many_rows_of_bf16(scheme, d):
     c.set_lengths([0])
     bad = np.isnan(back(c.attention(q))[0]).any(-1)
     assert bad[14, 2] and bad[4, 0] and bad[:20].sum() == 2 and bad[20:, 2:].all() and not bad[20:, :2].any()
+
+
+def test_commit_of_more_rows_than_a_length_can_count():
+    c = new(2, 64, 1, 1, 8, dtype="f32")
+    c.set_lengths([62, 10])
+    c.commit(2 ** 31 - 1, np.array([2 ** 31 - 1, 1], np.int32))
+    with pytest.raises(IndexError):
+        c.check()
+    assert c.per_seq_lens.tolist() == [64, 11]

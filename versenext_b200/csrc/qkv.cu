@@ -317,7 +317,7 @@ __global__ void __launch_bounds__(256) qkv_commit_kernel(QkvView v, int n_new, c
   pdl_wait();
   const int len = v.len(slot);
   int n = n_keep[slot] + keep_add;
-  if (n < 0 || n > n_new || len + n > v.capacity()) {
+  if (n < 0 || n > n_new || n > v.capacity() - len) {
     if (tid == 0) v.status[1] = 1;
     n = min(max(n, 0), min(n_new, v.capacity() - len));
   }
