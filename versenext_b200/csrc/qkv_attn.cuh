@@ -22,8 +22,9 @@ namespace qkv_detail {
 using bf16 = __nv_bfloat16;
 constexpr int WARPS = 4, THREADS = 32 * WARPS;
 constexpr int MIN_SHARE = 4;                        // blocks of a share at least
-constexpr int MERGE_WARPS = 8, MANY = 16;           // warps of a merging CTA; parts that one of them takes
+constexpr int MERGE_WARPS = 8, MANY = 8;           // warps of a merging CTA; parts that one of them takes
 constexpr int UNCUT = 8;                            // blocks of a unit that is never cut
+constexpr int MERGE_CTAS = 4;                       // merging CTAs on an SM
 constexpr unsigned long long WAIT_CYCLES = 4000000000ull;   // a copy that has not come after about two seconds never will
 
 template <typename T, int P, int NT, int RS>
@@ -528,8 +529,8 @@ __global__ void __launch_bounds__(THREADS, (AttnCfg<T, P, NT, RS>::CTAS)) qkv_at
 // the list: what stands there then is an earlier call's, whose shares with other rows lie beyond this call's parts.  Parts are read from L2, as the
 // first pass has brought some of them before they were written.  rmax: rows of a unit at most
 template <typename T, int P>
-__global__ void __launch_bounds__(32 * MERGE_WARPS) qkv_merge_kernel(QkvAttnArgs a, int RT, int rmax) {
-  constexpr int Y = P > 128 ? 2 : 1, IN = Y > 1 ? 8 : 16;    // parts asked for at a time
+__global__ void __launch_bounds__(32 * MERGE_WARPS, P > 128 ? MERGE_CTAS - 1 : MERGE_CTAS) qkv_merge_kernel(QkvAttnArgs a, int RT, int rmax) {
+  constexpr int Y = P > 128 ? 2 : 1, IN = Y > 1 ? 4 : 8;      // parts asked for at a time
   __shared__ float4 s_sum[MERGE_WARPS][32 * Y];
   __shared__ float s_l[MERGE_WARPS];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, G = a.v.H / a.v.KH;
@@ -643,10 +644,21 @@ struct Launch {
   long long most(int least) const { return split ? ceil_div(units * tiles, (long long)least) : units; }
 };
 
+// No more CTAs than there can be rows to merge.  Four on an SM, eight parts of a row asked for at a time, against two and sixteen: 2 x 1000
+// rows of a prompt 82 for 90 us in all, their merge 18 for 25.  Few of them with many parts each would all go to the SMs that are free
+// first; they ask for memory that lets only two onto an SM (a sequence of 120000 positions: 59 us, 64 with four)
+constexpr int MERGE_SPREAD = 76 << 10;
 template <typename T, int P>
-int32_t merge(vn_qkv* c, const QkvAttnArgs& a, int RT) {
-  VN_LAUNCH_PDL_LEVEL(c->ctx, 1, "qkv_merge_kernel", (qkv_merge_kernel<T, P>), dim3((unsigned)c->ctx->sm_count * 2), 32 * MERGE_WARPS, 0, a, RT,
-                      (int)min((long long)RT, (long long)a.step.T * (a.v.H / a.v.KH)));
+int32_t merge_ready(vn_qkv* c) {
+  VN_CUDA(c->ctx, cudaFuncSetAttribute(qkv_merge_kernel<T, P>, cudaFuncAttributeMaxDynamicSharedMemorySize, MERGE_SPREAD));
+  VN_CUDA(c->ctx, cudaFuncSetAttribute(qkv_merge_kernel<T, P>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
+  return VN_OK;
+}
+template <typename T, int P>
+int32_t merge(vn_qkv* c, const QkvAttnArgs& a, int RT, long long units) {
+  const int rmax = (int)min((long long)RT, (long long)a.step.T * (a.v.H / a.v.KH)), sms = c->ctx->sm_count;
+  const long long rows = units * rmax;
+  VN_LAUNCH_PDL_LEVEL(c->ctx, 1, "qkv_merge_kernel", (qkv_merge_kernel<T, P>), dim3((unsigned)min((long long)sms * MERGE_CTAS, rows)), 32 * MERGE_WARPS, rows <= 2 * sms ? MERGE_SPREAD : 0, a, RT, rmax);
   return VN_OK;
 }
 
@@ -664,14 +676,14 @@ int32_t launch(vn_qkv* c, const QkvAttnArgs& a) {
     VN_REQUIRE(ctx, n > 0, "qkv_attn_kernel does not fit an SM");
     // the same division of the SMs' memory for both, so that neither has to wait for another one
     VN_CUDA(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
-    VN_CUDA(ctx, cudaFuncSetAttribute(qkv_merge_kernel<T, P>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
+    if (int32_t st = merge_ready<T, P>(c)) return st;
     occ = min(n, C::CTAS);
   }
   Launch l;
   if (int32_t st = l.of(c, a, C::RT, QKV_BLOCK, UNCUT)) return st;
   const unsigned grid = (unsigned)min((long long)occ * ctx->sm_count, ceil_div(l.most(MIN_SHARE), (long long)C::RINGS));
   VN_LAUNCH_PDL_LEVEL(ctx, 1, "qkv_attn_kernel", kernel, grid, THREADS, C::SMEM, a, (int)l.rts, l.split);
-  return l.split ? merge<T, P>(c, a, C::RT) : VN_OK;
+  return l.split ? merge<T, P>(c, a, C::RT, l.units) : VN_OK;
 }
 
 template <int SCHEME, int P> int32_t launch_tc(vn_qkv* c, const QkvAttnArgs& a);      // qkv_attn_tc.cuh

@@ -491,14 +491,14 @@ int32_t launch_tc(vn_qkv* c, const QkvAttnArgs& a) {
   if (!ready[ctx->device & 63]) {
     VN_CUDA(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
     VN_CUDA(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
-    VN_CUDA(ctx, cudaFuncSetAttribute(qkv_merge_kernel<bf16, P>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
+    if (int32_t st = merge_ready<bf16, P>(c)) return st;
     ready[ctx->device & 63] = true;
   }
   Launch l;
   if (int32_t st = l.of(c, a, TC_ROWS, TC_KEYS, TC_UNCUT)) return st;
   const unsigned grid = (unsigned)min((long long)TC_CTAS * ctx->sm_count, l.most(TC_MIN_SHARE));
   VN_LAUNCH_PDL_LEVEL(ctx, 1, "qkv_attn_tc_kernel", kernel, grid, TC_THREADS, C::SMEM, a, (int)l.rts, l.split);
-  return l.split ? merge<bf16, P>(c, a, TC_ROWS) : VN_OK;
+  return l.split ? merge<bf16, P>(c, a, TC_ROWS, l.units) : VN_OK;
 }
 
 }  // namespace qkv_detail
