@@ -1,0 +1,50 @@
+"""QuantKVCache on the device where it is easiest to get wrong."""
+
+import numpy as np
+import pytest
+
+import qkv_cases as R
+from test_qkv_gpu import back, new, stored
+
+pytestmark = pytest.mark.gpu
+
+
+def write(c, k, v):
+    """Positions 0 .. of sequence 0; k, v (n, KH, d)."""
+    n = len(k)
+    c.append(np.concatenate([k.reshape(n, -1), v.reshape(n, -1)], 1), step=c.step([0], [n]), queries=False)
+
+
+def check_one(c, q, k, v, n_com, dtype, parents=None, window=0):
+    """Attention of sequence 0 over `n_com` committed positions and the rows q brings, against 64 bits."""
+    n, d = len(q), c.head_dim
+    write(c, k, v)
+    c.set_lengths([n_com] + [0] * (c.max_batch - 1))
+    tree = c.tree(parents) if parents is not None else None
+    got = back(c.attention(q[None], tree=tree, window=window))[0]
+    c.check()
+    depth, seen = R.depth_and_seen(parents, n)
+    out, weight, reach = R.attention(q, R.in_8_bits(k, c.scheme), R.in_8_bits(v, c.scheme), n_com, depth, seen, window, d ** -0.5)
+    tol = R.tolerance(out, weight, reach, d, n_com + n, dtype, c.scheme == "int8")
+    assert np.isfinite(got).all()
+    assert (np.abs(got - out) <= tol).all(), float(np.max(np.abs(got - out) / tol))
+
+
+# ---- parts of a sequence whose scores lie far apart ---------------------------------------------------------------------
+@pytest.mark.parametrize("scheme", ["int8", "fp8"])
+@pytest.mark.parametrize("dtype,H,KH,d,T", [("f32", 1, 1, 256, 1), ("bf16", 2, 1, 256, 1), ("bf16", 4, 2, 192, 2), ("f32", 3, 1, 248, 1), ("bf16", 5, 1, 136, 4), ("f32", 2, 1, 192, 24),
+                                            ("bf16", 8, 2, 128, 1), ("f32", 2, 1, 64, 1), ("bf16", 2, 1, 64, 20), ("bf16", 6, 1, 128, 5), ("bf16", 4, 1, 96, 9)])
+@pytest.mark.parametrize("n,hot", [(620, [(619, 110)]), (700, [(650, 380)]), (1000, [(990, 150)]), (1000, [(560, 120), (999, 260)]), (1000, [(3, 200)]), (1400, [(1390, 300)]),
+                                   (2600, [(1300, 130), (2590, 270)]), (1000, [(700, 60)])])
+def test_a_score_far_above_those_of_the_other_parts(scheme, dtype, H, KH, d, T, n, hot):
+    """A sequence of n positions is cut into parts of at least four blocks of 32 (two pages of 64 for many rows): 5 to 21 of them here.
+    One or two positions have a score of `hot` above the others', which are small."""
+    rng = np.random.default_rng(n + d)
+    c = new(1, n + T, H, KH, d, scheme=scheme, dtype=dtype)
+    along = rng.normal(0, 1, (KH, d))
+    along /= np.linalg.norm(along, axis=-1, keepdims=True)
+    q = stored(np.repeat(along, H // KH, 0)[None] * 4 + rng.normal(0, 0.1, (T, H, d)), dtype)
+    k = rng.normal(0, 0.3, (n + T, KH, d))
+    for at, gap in hot:
+        k[at] = along * gap * d ** 0.5 / 4
+    check_one(c, q, stored(k, dtype), stored(rng.normal(0, 1, (n + T, KH, d)), dtype), n, dtype)

@@ -531,6 +531,7 @@ __global__ void __launch_bounds__(THREADS, (AttnCfg<T, P, NT, RS>::CTAS)) qkv_at
 template <typename T, int P>
 __global__ void __launch_bounds__(32 * MERGE_WARPS, P > 128 ? MERGE_CTAS - 1 : MERGE_CTAS) qkv_merge_kernel(QkvAttnArgs a, int RT, int rmax) {
   constexpr int Y = P > 128 ? 2 : 1, IN = Y > 1 ? 4 : 8;      // parts asked for at a time
+  static_assert(IN <= MANY, "eight warps on a row's parts know the maximum of all of them");
   __shared__ float4 s_sum[MERGE_WARPS][32 * Y];
   __shared__ float s_l[MERGE_WARPS];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, G = a.v.H / a.v.KH;
@@ -559,7 +560,9 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS, P > 128 ? MERGE_CTAS - 1 : M
       float m = -CUDART_INF_F, l = 0.f;
 #pragma unroll
       for (int y = 0; y < Y; ++y) sum[y] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (many)
+      // the maximum of all parts comes first where they do not all come in one go: against a maximum of some of them, the weight of
+      // another may be more than 32 bits hold
+      if (o.n > IN)
         for (int j0 = lane; j0 < o.n; j0 += 256) {
           float x[8];
 #pragma unroll
