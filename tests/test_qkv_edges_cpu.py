@@ -1,0 +1,45 @@
+"""QuantKVCache without a GPU: numbers that the library's 32 bits do not hold, and arrays that it cannot read, are refused before a call."""
+
+import numpy as np
+import pytest
+
+from test_qkv_cpu import cache
+
+
+@pytest.mark.parametrize("name,call", [
+    ("vn_qkv_append", lambda c, n: c.append(np.zeros((2, 3, 128), np.float32), offset=n)),
+    ("vn_qkv_attention", lambda c, n: c.attention(np.zeros((2, 3, 4, 16), np.float32), window=n)),
+    ("vn_qkv_read", lambda c, n: c.read((1, 2), start=n)),
+    ("vn_qkv_read", lambda c, n: c.read((1, 2), offset=n)),
+    ("vn_qkv_read", lambda c, n: c.read(c.step([1], [2]), offset=n)),
+    ("vn_qkv_commit", lambda c, n: c.commit(n, [1, 2, 3])),
+    ("vn_qkv_commit", lambda c, n: c.commit(3, [1, 2, 3], keep_add=n)),
+    ("vn_qkv_commit", lambda c, n: c.commit(3, [1, n, 3])),
+    ("vn_qkv_commit", lambda c, n: c.commit(3, np.array([n, 2, 3]))),
+    ("vn_qkv_commit", lambda c, n: c.commit(3, [1, 2, 3], [[0, 1, 2], [0, 1, n], [0, 1, 2]])),
+])
+def test_numbers_of_more_than_32_bits(name, call):
+    c = cache(dtype="f32")
+    call(c, 2)
+    assert c.ctx.lib.calls[-1][0] == name
+    n = len(c.ctx.lib.calls)
+    for bad in (1 << 31, 1 << 32, (1 << 32) + 5, (1 << 62) + 1, -(1 << 31) - 1, -(1 << 32)):
+        with pytest.raises(ValueError):
+            call(c, bad)
+    assert len(c.ctx.lib.calls) == n
+
+
+@pytest.mark.parametrize("which", ["max_batch", "max_seq", "n_head", "n_kv_head", "head_dim", "pages"])
+@pytest.mark.parametrize("n", [1 << 31, (1 << 32) + 8, 8 - (1 << 32), -1])
+def test_sizes_of_more_than_32_bits(which, n):
+    with pytest.raises(ValueError):
+        cache(**{which: n})
+
+
+def test_rows_of_more_than_32_bits():
+    c = cache(dtype="f32")
+    n = len(c.ctx.lib.calls)
+    for step in ((1, 1 << 31), (0, 1 << 32), (3, 1 << 30)):
+        with pytest.raises(ValueError):
+            c.read(step, out=(None, None))
+    assert len(c.ctx.lib.calls) == n

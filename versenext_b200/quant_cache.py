@@ -22,6 +22,7 @@ from .device import Context, DeviceArray, as_device
 SCHEMES = ("int8", "fp8")
 PAGE = 64
 MAX_DRAFT = 64            # rows of a tree, and rows that commit may pick from
+_END = 1 << 31            # whole numbers go to the library in 32 bits
 _DTYPES = {"f32": (0, np.dtype(np.float32)), "bf16": (1, np.dtype(np.uint16))}
 
 
@@ -39,6 +40,23 @@ def from_bf16(x) -> np.ndarray:
 
 def _ptr(a):
     return None if a is None else a.ptr
+
+
+def _below_2_31(**numbers):
+    for name, n in numbers.items():
+        if not 0 <= n < _END:
+            raise ValueError(f"{name} {n} outside 0 .. 2^31 - 1")
+
+
+def _in_32_bits(ctx: Context, a, name: str) -> DeviceArray:
+    """Whole numbers on the device; those of the host have to fit."""
+    if hasattr(a, "requires_grad"):
+        a = a.data
+    if not isinstance(a, DeviceArray):
+        a = np.asarray(a)
+        if a.size and a.dtype != np.int32 and (a.min() < -_END or a.max() >= _END):
+            raise ValueError(f"{name} holds a number that 32 bits do not")
+    return as_device(ctx, a, np.int32)
 
 
 class Step:
@@ -106,6 +124,7 @@ class QuantKVCache:
         if dtype not in _DTYPES:
             raise ValueError(f"unknown dtype {dtype!r}, expected one of {tuple(_DTYPES)}")
         self.handle = None
+        _below_2_31(max_batch=max_batch, max_seq=max_seq, n_head=n_head, n_kv_head=n_kv_head, head_dim=head_dim, pages=pages)
         self.ctx, self.scheme, self.dtype = ctx, scheme, dtype
         self.max_batch, self.n_head, self.n_kv_head, self.head_dim = int(max_batch), int(n_head), int(n_kv_head), int(head_dim)
         self._code, self._np = _DTYPES[dtype]
@@ -179,8 +198,8 @@ class QuantKVCache:
             if m < step.rows:
                 raise ValueError(f"{m} rows for a step of {step.rows}")
             return step.entries, step.ents, step.row_ent, step.T, step.rows
-        if k != 2 or lead[0] > self.max_batch:
-            raise ValueError(f"rows of shape (sequences, rows, ..) with at most {self.max_batch} sequences, or a step, are needed")
+        if k != 2 or lead[0] > self.max_batch or lead[0] * lead[1] >= _END:
+            raise ValueError(f"rows of shape (sequences, rows, ..) with at most {self.max_batch} sequences and fewer than 2^31 rows, or a step, are needed")
         return lead[0], None, None, lead[1], lead[0] * lead[1]
 
     def _tree(self, tree, step, T, M):
@@ -226,6 +245,8 @@ class QuantKVCache:
         heads, the value heads, as one projection gives them.  q_norm / k_norm: weights (head_dim,) of an RMS norm of every
         query / key head; rope: (cos, sin) tables (positions, pairs) for rotating the first 2 * pairs dimensions of queries and keys
         (half-split, or neighbours when `interleaved`).  Lengths stay: `commit` moves them."""
+        if not 0 <= offset < _END:
+            _below_2_31(offset=offset)
         x = self._in(rows)
         H, d = self.n_head if queries else 0, self.head_dim
         width = (H + 2 * self.n_kv_head) * d
@@ -254,6 +275,8 @@ class QuantKVCache:
         """softmax(scale q k^T) v of a step's queries (.., n_head, head_dim) over the committed positions and the step's own rows, which
         `append` has written: row i of an entry sees the rows up to itself, or its ancestors in `tree`.  window > 0: only the last
         `window` positions, of its path where there is a tree.  scale: 1 / sqrt(head_dim) unless given.  A row that sees nothing gets zeros."""
+        if not 0 <= window < _END:
+            _below_2_31(window=window)
         q = self._in(q)
         E, ents, row_ent, T, M = self._rows(q.shape, (self.n_head, self.head_dim), step)
         seen, depth, per_row = self._tree(tree, step, T, M)
@@ -266,12 +289,14 @@ class QuantKVCache:
     def commit(self, n_new: int, n_keep, keep_idx=None, keep_add: int = 0):
         """Keep `n_keep[b] + keep_add` of the `n_new` positions appended to sequence b: the first ones (chain), or those listed in
         `keep_idx[b]` (tree path), as KVCache.commit."""
-        nk = as_device(self.ctx, n_keep, np.int32)
+        if not (0 <= n_new < _END and -_END <= keep_add < _END):
+            raise ValueError(f"n_new {n_new} outside 0 .. 2^31 - 1, or keep_add {keep_add} outside 32 bits")
+        nk = _in_32_bits(self.ctx, n_keep, "n_keep")
         if nk.size < self.max_batch:
             raise ValueError(f"n_keep must have {self.max_batch} values")
         ki, stride = None, 0
         if keep_idx is not None:
-            ki = as_device(self.ctx, keep_idx, np.int32)
+            ki = _in_32_bits(self.ctx, keep_idx, "keep_idx")
             if ki.ndim != 2 or ki.shape[0] < self.max_batch or ki.shape[1] < n_new:
                 raise ValueError(f"keep_idx must have shape ({self.max_batch}, {n_new})")
             stride = ki.shape[-1]
@@ -288,11 +313,13 @@ class QuantKVCache:
             lead = (M,)
         else:
             E, T = (int(n) for n in step)
-            if E < 0 or E > self.max_batch or T < 0:
-                raise ValueError(f"at most {self.max_batch} sequences")
+            if E < 0 or E > self.max_batch or T < 0 or max(T, E * T) >= _END:
+                raise ValueError(f"at most {self.max_batch} sequences and fewer than 2^31 rows")
             ents, row_ent, M, lead = None, None, E * T, (E, T)
-        if start is not None and (back or start < 0):
+        if start is not None and (back or not 0 <= start < _END):
             raise ValueError("start is a position, and excludes `back`")
+        if not 0 <= offset < _END:
+            _below_2_31(offset=offset)
         if dtype is not None and dtype not in _DTYPES:
             raise ValueError(f"unknown dtype {dtype!r}, expected one of {tuple(_DTYPES)}")
         code, kind = _DTYPES[dtype or self.dtype]
