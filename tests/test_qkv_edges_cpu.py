@@ -43,3 +43,15 @@ def test_rows_of_more_than_32_bits():
         with pytest.raises(ValueError):
             c.read(step, out=(None, None))
     assert len(c.ctx.lib.calls) == n
+
+
+def test_bf16_rows_are_not_taken_for_whole_numbers():
+    c = cache(dtype="f32")
+    n = len(c.ctx.lib.calls)
+    with pytest.raises(TypeError):
+        c.append(np.zeros((2, 3, 128), np.uint16))
+    with pytest.raises(TypeError):
+        c.attention(np.zeros((2, 3, 4, 16), np.uint16))
+    assert len(c.ctx.lib.calls) == n
+    c.append(np.zeros((2, 3, 128), np.int32))
+    c.attention(np.zeros((2, 3, 4, 16), np.float64))

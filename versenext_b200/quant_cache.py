@@ -222,6 +222,8 @@ class QuantKVCache:
         x = np.asarray(x)
         if self.dtype == "bf16" and x.dtype != np.uint16:
             x = to_bf16(x)
+        elif self.dtype == "f32" and x.dtype == np.uint16:
+            raise TypeError("bf16 rows for a cache of float32 ones")
         return as_device(self.ctx, x, self._np)
 
     def _out(self, out, shape, dtype):
