@@ -55,3 +55,21 @@ def test_bf16_rows_are_not_taken_for_whole_numbers():
     assert len(c.ctx.lib.calls) == n
     c.append(np.zeros((2, 3, 128), np.int32))
     c.attention(np.zeros((2, 3, 4, 16), np.float64))
+
+
+def test_a_tree_of_another_step():
+    """The tables go by the rows of the step: one with as many rows, but others for an entry, is another step."""
+    c = cache(dtype="f32")
+    a, b = c.step([0, 1], [1, 2]), c.step([0, 1], [2, 1])
+    t = c.tree([[-1], [-1, -1]], a)
+    x, q = np.zeros((3, 128), np.float32), np.zeros((3, 4, 16), np.float32)
+    n = len(c.ctx.lib.calls)
+    for step in (b, c.step([0], [3]), c.step([0, 1, 2], [1, 1, 1]), None):
+        with pytest.raises(ValueError):
+            c.append(x if step else x[None], step=step, tree=t)
+        with pytest.raises(ValueError):
+            c.attention(q if step else q[None], step=step, tree=t)
+    assert len(c.ctx.lib.calls) == n
+    for step in (a, c.step([2, 0], [1, 2]), c.step([2, 1, 0], [1, 0, 2])):     # other sequences, the same rows
+        c.append(x, step=step, tree=t)
+        c.attention(q, step=step, tree=t)

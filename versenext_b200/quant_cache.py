@@ -89,10 +89,11 @@ class Step:
 class Tree:
     """What the rows of a tree see of one another, on the device."""
 
-    __slots__ = ("T", "rows", "per_row", "_buf", "seen", "depth")
+    __slots__ = ("T", "counts", "per_row", "_buf", "seen", "depth")
 
-    def __init__(self, ctx: Context, seen: np.ndarray, depth: np.ndarray, T: int, rows: Optional[int]):
-        self.T, self.rows, self.per_row = T, rows, int(rows is not None)
+    def __init__(self, ctx: Context, seen: np.ndarray, depth: np.ndarray, T: int, counts: Optional[np.ndarray]):
+        """counts: rows of every entry of the step that the tables go by; None: one tree for all entries."""
+        self.T, self.counts, self.per_row = T, counts, int(counts is not None)
         self._buf = ctx.from_numpy(np.concatenate([seen.astype(np.uint64).view(np.uint8), depth.astype(np.int32).view(np.uint8), np.zeros(16, np.uint8)]))
         self.seen, self.depth = self._buf.ptr, self._buf.ptr + 8 * seen.size
 
@@ -183,7 +184,7 @@ class QuantKVCache:
             if len(parents) != step.entries or any(len(p) != n for p, n in zip(parents, step.counts)):
                 raise ValueError("a list of parents for every entry, one parent a row, is needed")
             made = [_tree_of(p) for p in parents]
-            return Tree(self.ctx, np.concatenate([m[0] for m in made]), np.concatenate([m[1] for m in made]), step.T, step.rows)
+            return Tree(self.ctx, np.concatenate([m[0] for m in made]), np.concatenate([m[1] for m in made]), step.T, step.counts)
         seen, depth = _tree_of(parents)
         return Tree(self.ctx, seen, depth, seen.size, None)
 
@@ -206,7 +207,7 @@ class QuantKVCache:
         if tree is None:
             return None, None, 0
         if tree.per_row:
-            if step is None or tree.rows != M:
+            if step is None or (tree.counts is not step.counts and not np.array_equal(tree.counts[tree.counts > 0], step.counts[step.counts > 0])):
                 raise ValueError("this tree was made for another step")
         elif tree.T < T:
             raise ValueError(f"a tree of {tree.T} rows for entries of {T}")
