@@ -73,3 +73,29 @@ def test_a_tree_of_another_step():
     for step in (a, c.step([2, 0], [1, 2]), c.step([2, 1, 0], [1, 0, 2])):     # other sequences, the same rows
         c.append(x, step=step, tree=t)
         c.attention(q, step=step, tree=t)
+
+
+def test_arrays_of_another_device():
+    """A kernel of this device cannot read them."""
+    c, other = cache(dtype="f32"), cache(dtype="f32")
+    other.ctx.device = 1
+    there = other.ctx.from_numpy
+    x, q, w = np.zeros((2, 3, 128), np.float32), np.zeros((2, 3, 4, 16), np.float32), np.ones(16, np.float32)
+    table = np.zeros((128, 8), np.float32)
+    i3 = np.zeros(3, np.int32)
+    step, far = c.step([0], [3]), other.step([0], [3])
+    calls = [
+        lambda f: c.append(f(x)), lambda f: c.append(x, out=f(q)), lambda f: c.append(x, q_norm=f(w)), lambda f: c.append(x, k_norm=f(w)),
+        lambda f: c.append(x, rope=(f(table), table)), lambda f: c.append(x, rope=(table, f(table))),
+        lambda f: c.append(x[0], step=far if f == there else step), lambda f: c.append(x, tree=(other if f == there else c).tree([-1, 0, 0])),
+        lambda f: c.attention(f(q)), lambda f: c.attention(q, out=f(q)), lambda f: c.attention(q[0], step=far if f == there else step),
+        lambda f: c.read((2, 3), out=(f(np.zeros((2, 3, 2, 16), np.float32)), None)), lambda f: c.read((2, 3), out=(None, f(np.zeros((2, 3, 2, 16), np.float32)))),
+        lambda f: c.read(far if f == there else step), lambda f: c.commit(3, f(i3)), lambda f: c.commit(3, i3, f(np.zeros((3, 3), np.int32))), lambda f: c.set_lengths(f(i3)),
+    ]
+    for call in calls:
+        n = len(c.ctx.lib.calls)
+        with pytest.raises(ValueError):
+            call(there)
+        assert len(c.ctx.lib.calls) == n
+        call(c.ctx.from_numpy)
+        assert len(c.ctx.lib.calls) == n + 1

@@ -138,6 +138,11 @@ class QuantKVCache:
         self.max_seq = self.max_pages * PAGE
         self.pages = int(pages) or self.max_batch * self.max_pages
 
+    def _here(self, a: DeviceArray) -> DeviceArray:
+        if a.ctx.device != self.ctx.device:
+            raise ValueError(f"an array on device {a.ctx.device} for a cache on device {self.ctx.device}")
+        return a
+
     # -- lengths and pages ---------------------------------------------------
     @property
     def per_seq_lens(self) -> np.ndarray:
@@ -150,7 +155,7 @@ class QuantKVCache:
         if isinstance(lens, DeviceArray):
             if lens.shape != (self.max_batch,) or lens.dtype != np.int32:
                 raise ValueError(f"lens must be int32 of shape ({self.max_batch},)")
-            self.ctx._check(self.ctx.lib.vn_qkv_set_lengths(self.handle, lens.ptr, 1))
+            self.ctx._check(self.ctx.lib.vn_qkv_set_lengths(self.handle, self._here(lens).ptr, 1))
             return
         lens = np.asarray(lens)
         if lens.shape != (self.max_batch,):
@@ -195,6 +200,7 @@ class QuantKVCache:
         if shape[k:] != tail or k < 0:
             raise ValueError(f"rows of shape {tuple(shape)} do not end in {tuple(tail)}")
         if step is not None:
+            self._here(step._buf)
             m = math.prod(lead)
             if m < step.rows:
                 raise ValueError(f"{m} rows for a step of {step.rows}")
@@ -213,13 +219,14 @@ class QuantKVCache:
             raise ValueError(f"a tree of {tree.T} rows for entries of {T}")
         if T > MAX_DRAFT:
             raise ValueError(f"a tree has at most {MAX_DRAFT} rows, not {T}")
+        self._here(tree._buf)
         return tree.seen, tree.depth, tree.per_row
 
     def _in(self, x):
         if isinstance(x, DeviceArray):
             if x.dtype != self._np:
                 raise TypeError(f"device array has dtype {x.dtype}, need {self._np}")
-            return x
+            return self._here(x)
         x = np.asarray(x)
         if self.dtype == "bf16" and x.dtype != np.uint16:
             x = to_bf16(x)
@@ -232,10 +239,10 @@ class QuantKVCache:
             return self.ctx.empty(shape, dtype)
         if not isinstance(out, DeviceArray) or out.dtype != dtype or out.size < math.prod(shape):
             raise ValueError(f"out must be a device array of {np.dtype(dtype)} with room for {tuple(shape)}")
-        return out
+        return self._here(out)
 
     def _weight(self, a, name):
-        a = as_device(self.ctx, a, np.float32)
+        a = self._here(as_device(self.ctx, a, np.float32))
         if a.shape != (self.head_dim,):
             raise ValueError(f"{name} must have shape ({self.head_dim},)")
         return a
@@ -261,7 +268,7 @@ class QuantKVCache:
         pairs = rope_rows = 0
         if rope is not None:
             cs, sn = rope
-            cs, sn = as_device(self.ctx, cs, np.float32), as_device(self.ctx, sn, np.float32)
+            cs, sn = self._here(as_device(self.ctx, cs, np.float32)), self._here(as_device(self.ctx, sn, np.float32))
             if cs.ndim != 2 or cs.shape != sn.shape or 2 * cs.shape[1] > d:
                 raise ValueError(f"rope: two tables (positions, pairs) with at most {d // 2} pairs are needed")
             rope_rows, pairs = cs.shape
@@ -294,12 +301,12 @@ class QuantKVCache:
         `keep_idx[b]` (tree path), as KVCache.commit."""
         if not (0 <= n_new < _END and -_END <= keep_add < _END):
             raise ValueError(f"n_new {n_new} outside 0 .. 2^31 - 1, or keep_add {keep_add} outside 32 bits")
-        nk = _in_32_bits(self.ctx, n_keep, "n_keep")
+        nk = self._here(_in_32_bits(self.ctx, n_keep, "n_keep"))
         if nk.size < self.max_batch:
             raise ValueError(f"n_keep must have {self.max_batch} values")
         ki, stride = None, 0
         if keep_idx is not None:
-            ki = _in_32_bits(self.ctx, keep_idx, "keep_idx")
+            ki = self._here(_in_32_bits(self.ctx, keep_idx, "keep_idx"))
             if ki.ndim != 2 or ki.shape[0] < self.max_batch or ki.shape[1] < n_new:
                 raise ValueError(f"keep_idx must have shape ({self.max_batch}, {n_new})")
             stride = ki.shape[-1]
@@ -312,6 +319,7 @@ class QuantKVCache:
         entry; those behind its committed ones (`offset` further on) when `start` is None; its last committed ones with `back`.
         step: a Step, or (sequences, rows of each)."""
         if isinstance(step, Step):
+            self._here(step._buf)
             E, ents, row_ent, T, M = step.entries, step.ents, step.row_ent, step.T, step.rows
             lead = (M,)
         else:
