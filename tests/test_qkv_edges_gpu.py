@@ -48,3 +48,36 @@ def test_a_score_far_above_those_of_the_other_parts(scheme, dtype, H, KH, d, T, 
     for at, gap in hot:
         k[at] = along * gap * d ** 0.5 / 4
     check_one(c, q, stored(k, dtype), stored(rng.normal(0, 1, (n + T, KH, d)), dtype), n, dtype)
+
+
+# ---- rows that are not finite -----------------------------------------------------------------------------------------
+def shown(c, seen, depth):
+    """A tree of rows that see what `seen` says, on the device."""
+    from versenext_b200.quant_cache import Tree
+    return Tree(c.ctx, np.asarray(seen, np.uint64), np.asarray(depth, np.int32), len(seen), None)
+
+
+@pytest.mark.parametrize("scheme", ["int8", "fp8"])
+@pytest.mark.parametrize("dtype,H,d,T", [("f32", 1, 64, 4), ("bf16", 1, 64, 4), ("bf16", 2, 64, 12), ("bf16", 4, 128, 40), ("bf16", 1, 256, 4), ("bf16", 4, 96, 30), ("f32", 2, 192, 20)])
+@pytest.mark.parametrize("bad", [-np.inf, np.inf, np.nan])
+def test_a_query_that_is_not_finite(scheme, dtype, H, d, T, bad):
+    """Every score of the row is then infinite or no number, of one sign too where all keys have the same sign in that channel: no soft-max
+    exists, and the row is NaN.  A row that sees nothing is zero whatever its query."""
+    rng = np.random.default_rng(d + T)
+    n = 200
+    c = new(1, n + T, H, 1, d, scheme=scheme, dtype=dtype)
+    k = rng.normal(0, 1, (n + T, 1, d))
+    k[..., 3] = rng.uniform(1, 2, (n + T, 1))
+    write(c, stored(k, dtype), stored(rng.normal(0, 1, (n + T, 1, d)), dtype))
+    c.set_lengths([n])
+    q = stored(rng.normal(0, 1, (1, T, H, d)), dtype)
+    good = back(c.attention(q))
+    q[0, 1, 0, 3] = bad
+    got = back(c.attention(q))
+    assert np.isnan(got[0, 1, 0]).all()
+    good[0, 1, 0] = got[0, 1, 0]
+    np.testing.assert_array_equal(got, good)
+    c.set_lengths([0])
+    out = back(c.attention(q, tree=shown(c, [0] * T, [0] * T)))
+    assert (out == 0).all()
+    c.check()

@@ -267,8 +267,8 @@ __global__ void __launch_bounds__(THREADS, (AttnCfg<T, P, NT, RS>::CTAS)) qkv_at
                            max(__float_as_uint(x[k].z) & 0x7fffffffu, __float_as_uint(x[k].w) & 0x7fffffffu)));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const int e = top >= 0x7f800000u ? 140 : min(max((int)(top >> 23), 27), 254);      // a row that is not finite is left as it is
-      const float up = pow2(267 - e);
+      const int e = min(max((int)(top >> 23), 27), 254);
+      const float up = top >= 0x7f800000u ? CUDART_NAN_F : pow2(267 - e);      // a query that is not finite has no soft-max: NaN for all it sees
       float sum = 0.f;
 #pragma unroll
       for (int k = 0; k < CH; ++k) {

@@ -231,8 +231,8 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) qkv_attn_tc_kernel(QkvAtt
           top = max(top >> 16, top & 0xffffu);
           top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
           top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-          const int e = top >= 0x7f80u ? 140 : min(max((int)(top >> 7), 27), 254);         // a row that is not finite is left as it is
-          const float up = pow2(267 - e);
+          const int e = min(max((int)(top >> 7), 27), 254);
+          const float up = top >= 0x7f80u ? CUDART_NAN_F : pow2(267 - e);                  // a query that is not finite has no soft-max: NaN for all it sees
 #pragma unroll
           for (int k = 0; k < P / 16; ++k) {
             auto two = [&](unsigned w) { return pack_f16(__uint_as_float(w << 16) * up, __uint_as_float(w & 0xffff0000u) * up); };
