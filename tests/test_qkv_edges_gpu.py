@@ -81,3 +81,17 @@ def test_a_query_that_is_not_finite(scheme, dtype, H, d, T, bad):
     out = back(c.attention(q, tree=shown(c, [0] * T, [0] * T)))
     assert (out == 0).all()
     c.check()
+
+
+# ---- device tables out of range -----------------------------------------------------------------------------------------
+def test_device_lengths_out_of_range_are_reported():
+    c = new(3, 100, 2, 1, 16, dtype="f32")
+    for bad, want in (([-1, 5, 128], [0, 5, 128]), ([3, 1 << 30, 129], [3, 128, 128]), ([-(1 << 31), 0, (1 << 31) - 1], [0, 0, 128])):
+        c.set_lengths(c.ctx.from_numpy(np.array(bad, np.int32)))
+        with pytest.raises(IndexError):
+            c.check()
+        assert c.per_seq_lens.tolist() == want
+    c.set_lengths(c.ctx.from_numpy(np.array([0, 128, 7], np.int32)))
+    c.check()
+    assert c.per_seq_lens.tolist() == [0, 128, 7]
+    assert c.get(1)[0].shape == (128, 1, 16)

@@ -359,10 +359,13 @@ __global__ void __launch_bounds__(256) qkv_commit_kernel(QkvView v, int n_new, c
   }
 }
 
-__global__ void set_lengths_kernel(int* __restrict__ lens, const int* __restrict__ from, int n) {
+__global__ void set_lengths_kernel(QkvView v, const int* __restrict__ from) {
   const int i = blockIdx.x * 256 + threadIdx.x;
   pdl_wait();
-  if (i < n) lens[i] = from[i];
+  if (i >= v.max_batch) return;
+  const int n = from[i];
+  if (n < 0 || n > v.capacity()) v.status[1] = 1;
+  v.lens[i] = min(max(n, 0), v.capacity());
 }
 
 // layout of vn_ctx::qkv_parts: two parts for every share (CTA, or warp with a quarter of the rows) that the attention kernel may have
@@ -482,7 +485,7 @@ int32_t vn_qkv_set_lengths(vn_qkv* c, const int32_t* lens, int32_t on_device) {
   VN_CHECK_QKV(c);
   VN_REQUIRE(c->ctx, lens, "lens is null");
   if (on_device) {
-    VN_LAUNCH_PDL_LEVEL(c->ctx, 1, "set_lengths_kernel", set_lengths_kernel, ceil_div(c->v.max_batch, 256), 256, 0, c->v.lens, lens, c->v.max_batch);
+    VN_LAUNCH_PDL_LEVEL(c->ctx, 1, "set_lengths_kernel", set_lengths_kernel, ceil_div(c->v.max_batch, 256), 256, 0, c->v, lens);
     return VN_OK;
   }
   for (int i = 0; i < c->v.max_batch; ++i)
