@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import qkv_cases as R
-from test_qkv_gpu import back, new, stored
+from test_qkv_gpu import back, new, stored, tables
 
 pytestmark = pytest.mark.gpu
 
@@ -95,3 +95,26 @@ def test_device_lengths_out_of_range_are_reported():
     c.check()
     assert c.per_seq_lens.tolist() == [0, 128, 7]
     assert c.get(1)[0].shape == (128, 1, 16)
+
+
+def test_positions_that_pass_32_bits_have_no_room():
+    far = (1 << 31) - 1
+    c = new(2, 128, 2, 1, 16, dtype="f32")
+    ones = np.ones((2, 3, 64), np.float32)
+    c.append(ones)
+    c.set_lengths([3, 100])
+    for start in (dict(start=far), dict(start=far - 1), dict(offset=far), dict(offset=far - 2), dict(offset=far, back=True)):
+        for step in ((2, 3), c.step([1, 0], [2, 3])):
+            k, v = c.read(step, dtype="f32", **start)
+            with pytest.raises(RuntimeError):
+                c.check()
+            assert (k.numpy() == 0).all() and (v.numpy() == 0).all()
+    before = [c.get(b, 128) for b in range(2)]
+    for offset in (far, far - 1, far - 102):
+        q = c.append(2 * ones, offset=offset, rope=tables(128, 8))
+        assert np.isfinite(q.numpy()).all()
+        with pytest.raises(RuntimeError):
+            c.check()
+    for b in range(2):
+        for x, y in zip(before[b], c.get(b, 128)):
+            np.testing.assert_array_equal(x, y)

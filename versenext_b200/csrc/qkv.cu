@@ -130,9 +130,11 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2) qkv_append_kernel
   ask(first);
   int slot, i, n;
   if (!a.step.row(a.v, row, &slot, &i, &n)) return;
-  const int len = a.v.len(slot), pos = len + a.off + i;
-  const int turn = min(max(len + a.off + a.tree.away(row, i), 0), a.rope_rows - 1);
-  const int page = pos >= 0 && pos < a.v.capacity() ? a.v.page(slot, pos / KV_PAGE) : -1, at = pos % QKV_BLOCK;
+  // the length and the offset, at most the capacity: then 32 bits hold the position, and, unsigned, one that there is no room for
+  const int len = a.v.len(slot), begin = len + min(a.off, a.v.capacity() - len);
+  const unsigned pos = (unsigned)begin + (unsigned)i;
+  const int turn = min(max(begin + min(a.tree.away(row, i), (1 << 30) - 1), 0), a.rope_rows - 1);
+  const int page = pos < (unsigned)a.v.capacity() ? a.v.page(slot, pos / KV_PAGE) : -1, at = pos % QKV_BLOCK;
   unsigned char* base = a.v.block(max(page, 0), 0, pos % KV_PAGE / QKV_BLOCK);
   const int to = at * P + (((c >> 4) ^ qkv_turn(P / 16, at)) << 4) + (c & 15), head_bytes = 2 * a.v.block_bytes(), np = a.pairs;
   // what the channels are turned by: half-split, those of the two halves by the same angles
@@ -248,11 +250,11 @@ __global__ void __launch_bounds__(256) qkv_read_kernel(QkvView v, QkvStep step, 
   if (lane < RB && row0 + lane < step.M) {
     int slot, i, n;
     if (step.row(v, row0 + lane, &slot, &i, &n)) {
-      const int pos = (start >= 0 ? start : v.len(slot) + off - (start == -2 ? n : 0)) + i;
-      const int page = pos >= 0 && pos < v.capacity() ? v.page(slot, pos / KV_PAGE) : -1;
-      own_at = page < 0 ? 0 : pos % QKV_BLOCK;
+      const long long pos = (start >= 0 ? start : (long long)v.len(slot) + off - (start == -2 ? n : 0)) + i;     // may pass 32 bits where there is no room
+      const int page = pos >= 0 && pos < v.capacity() ? v.page(slot, (int)(pos / KV_PAGE)) : -1;
+      own_at = page < 0 ? 0 : (int)(pos % QKV_BLOCK);
       if (page < 0) v.status[0] = 1;
-      else own_block = ((long long)page * v.KH * 2 + pos % KV_PAGE / QKV_BLOCK) * v.block_bytes();
+      else own_block = ((long long)page * v.KH * 2 + (int)(pos % KV_PAGE) / QKV_BLOCK) * v.block_bytes();
     }
   }
   const int head = it / per, c = it % per * C, CH = v.P / 16, scales = 2 * QKV_BLOCK * v.P;
