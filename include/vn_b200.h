@@ -445,8 +445,9 @@ int32_t vn_qkv_set_pages(vn_qkv* c, const int32_t* table_host);
 int32_t vn_qkv_lengths(vn_qkv* c, int32_t* out_host);                                  /* [max_batch] */
 int32_t vn_qkv_set_lengths(vn_qkv* c, const int32_t* lens, int32_t on_device);         /* [max_batch] */
 /* Conditions met by kernels since the last call, read after a stream synchronisation and cleared: *no_room: a position behind
- * the capacity or without a page was to be written or read (VN_ERR_OVERFLOW); *bad_index: a sequence, row, count, kept row or length
- * (which counts as the nearest in range) out of range (VN_ERR_INDEX).  VN_ERR_TIMEOUT: a copy from the cache did not arrive; that call's results are no good. */
+ * the capacity or without a page was to be written or read (VN_ERR_OVERFLOW); *bad_index: a sequence, row, count or kept row out of
+ * range, or a length, a depth under a window (0 .. 63) or a position to rotate by (the tables' rows), which count as the nearest in
+ * range (VN_ERR_INDEX).  VN_ERR_TIMEOUT: a copy from the cache did not arrive; that call's results are no good. */
 int32_t vn_qkv_status(vn_qkv* c, int32_t* no_room, int32_t* bad_index);
 /* Writes a step's keys and values at positions length + offset + i; lengths stay.  rows_dev [M][ld]: the H query heads (only with
  * queries != 0), the KH key heads, the KH value heads.  In the same pass, for query and key heads: x / sqrt(mean x^2 + eps) * norm

@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import qkv_cases as R
-from test_qkv_gpu import back, new, stored, tables
+from test_qkv_gpu import back, fill, new, stored, tables
 
 pytestmark = pytest.mark.gpu
 
@@ -118,3 +118,38 @@ def test_positions_that_pass_32_bits_have_no_room():
     for b in range(2):
         for x, y in zip(before[b], c.get(b, 128)):
             np.testing.assert_array_equal(x, y)
+
+
+@pytest.mark.parametrize("dtype,H,d", [("f32", 2, 64), ("bf16", 2, 64), ("bf16", 16, 64), ("bf16", 16, 128), ("bf16", 16, 96)])
+@pytest.mark.parametrize("wrong,counts_as", [([100, -10, 3], [63, 0, 3]), ([0, 1 << 30, -(1 << 31)], [0, 63, 0]), ([64, 2, (1 << 31) - 1], [63, 2, 63])])
+def test_depths_out_of_range_are_reported(dtype, H, d, wrong, counts_as):
+    """A row of a tree is 0 to 63 tokens behind the committed ones; what is outside counts as the nearest of them."""
+    rng = np.random.default_rng(d)
+    c = new(2, 500, H, 1, d, dtype=dtype)
+    fill(c, rng, [400, 90], dtype)
+    c.append(stored(rng.normal(0, 1, (2, 3, 2 * d)), dtype), queries=False)
+    q = stored(rng.normal(0, 1, (2, 3, H, d)), dtype)
+    seen = [1, 3, 5]
+    for window in (1, 40, 200):
+        want = back(c.attention(q, tree=shown(c, seen, counts_as), window=window))
+        c.check()
+        got = back(c.attention(q, tree=shown(c, seen, wrong), window=window))
+        with pytest.raises(IndexError):
+            c.check()
+        np.testing.assert_array_equal(got, want)
+
+
+def test_positions_outside_the_rotation_tables_are_reported():
+    rng = np.random.default_rng(1)
+    c = new(1, 64, 1, 1, 16, dtype="f32")
+    rope = tables(64, 8)
+    x = rng.normal(0, 1, (1, 2, 48)).astype(np.float32)
+    c.set_lengths([10])
+    c.append(x, tree=shown(c, [1, 3], [-10, 53]), rope=rope)     # positions 0 and 63
+    c.check()
+    for depth in ([0, 54], [-11, 0], [0, (1 << 31) - 1], [-(1 << 31), 0]):
+        c.append(x, tree=shown(c, [1, 3], depth), rope=rope)
+        with pytest.raises(IndexError):
+            c.check()
+        c.append(x, tree=shown(c, [1, 3], depth))
+        c.check()                                                 # without rotation there is no such position

@@ -133,13 +133,14 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2) qkv_append_kernel
   // the length and the offset, at most the capacity: then 32 bits hold the position, and, unsigned, one that there is no room for
   const int len = a.v.len(slot), begin = len + min(a.off, a.v.capacity() - len);
   const unsigned pos = (unsigned)begin + (unsigned)i;
-  const int turn = min(max(begin + min(a.tree.away(row, i), (1 << 30) - 1), 0), a.rope_rows - 1);
+  const int away = a.tree.away(row, i), turn = min(max(begin + min(away, (1 << 30) - 1), 0), a.rope_rows - 1);
   const int page = pos < (unsigned)a.v.capacity() ? a.v.page(slot, pos / KV_PAGE) : -1, at = pos % QKV_BLOCK;
   unsigned char* base = a.v.block(max(page, 0), 0, pos % KV_PAGE / QKV_BLOCK);
   const int to = at * P + (((c >> 4) ^ qkv_turn(P / 16, at)) << 4) + (c & 15), head_bytes = 2 * a.v.block_bytes(), np = a.pairs;
   // what the channels are turned by: half-split, those of the two halves by the same angles
   float cs[8], sn[8];
   const bool turned = c < 2 * np;
+  if (np && page >= 0 && turn - begin != away) a.v.status[1] = 1;      // no such angles: those of the nearest position
   if (turned) {
     const float *pc = a.cs + (long long)turn * np, *ps = a.sn + (long long)turn * np;
     if (a.vec_rope && !a.interleaved) {

@@ -77,6 +77,13 @@ struct QkvTree {
   const int* depth = nullptr;
   int per_row = 0;                                  // the tables go by the row of the step, else by its place in its entry
   __device__ __forceinline__ int away(int row, int i) const { return depth ? depth[per_row ? row : i] : i; }
+  // as attention takes it, whose windows rely on a path of at most QKV_MAX_DRAFT rows
+  __device__ __forceinline__ int behind(const QkvView& v, int row, int i) const {
+    const int n = away(row, i);
+    if (!depth || (n >= 0 && n < QKV_MAX_DRAFT)) return n;
+    v.status[1] = 1;
+    return n < 0 ? 0 : QKV_MAX_DRAFT - 1;
+  }
   // rows that a row sees through a window: of a path, parents before children, the last ones
   __device__ __forceinline__ unsigned long long sees(int row, int i, int window) const {
     unsigned long long s = seen[per_row ? row : i];

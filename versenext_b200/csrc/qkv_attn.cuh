@@ -380,7 +380,7 @@ __global__ void __launch_bounds__(THREADS, (AttnCfg<T, P, NT, RS>::CTAS)) qkv_at
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
-              const int tok = row_t[nt][x], away = tok < 0 ? 0 : a.tree.away(u.r0 + tok, tok);
+              const int tok = row_t[nt][x], away = tok < 0 || a.window == 0 ? 0 : a.tree.behind(v, u.r0 + tok, tok);
               const unsigned long long seen = a.tree.seen && tok >= 0 ? a.tree.sees(u.r0 + tok, tok, a.window) : 0;
 #pragma unroll
               for (int j = 0; j < 4; ++j) {

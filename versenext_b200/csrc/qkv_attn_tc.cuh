@@ -315,7 +315,7 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) qkv_attn_tc_kernel(QkvAtt
     do {
       begin();
       const int f = u.f0 + row, tok = f < u.nf ? f / G : -1;
-      const int away = tok < 0 ? 0 : a.tree.away(u.r0 + tok, tok);
+      const int away = tok < 0 || a.window == 0 ? 0 : a.tree.behind(v, u.r0 + tok, tok);
       const unsigned long long seen = a.tree.seen && tok >= 0 ? a.tree.sees(u.r0 + tok, tok, a.window) : 0;
       float rf = 0.f, m = -CUDART_INF_F, l = 0.f;
       int R = 16;
