@@ -153,3 +153,20 @@ def test_positions_outside_the_rotation_tables_are_reported():
             c.check()
         c.append(x, tree=shown(c, [1, 3], depth))
         c.check()                                                 # without rotation there is no such position
+
+
+def test_a_step_whose_rows_belong_to_nobody():
+    """No entries, and rows that name none: everything is left as it was."""
+    from versenext_b200._lib import VN_OK
+    for dtype, d in (("f32", 16), ("bf16", 64)):
+        c = new(2, 64, 2, 1, d, dtype=dtype)
+        ctx, lib = c.ctx, c.ctx.lib
+        nobody = ctx.from_numpy(np.full(4, -1, np.int32))
+        x = ctx.from_numpy(np.full((4, 4 * d), 1, c._np))
+        out = ctx.from_numpy(np.full((4, 2, d), 9, c._np))
+        for T in (1, 40):
+            assert lib.vn_qkv_append(c.handle, x.ptr, 4 * d, 1, 0, nobody.ptr, nobody.ptr, T, 4, 0, None, 0, None, None, 1e-6, None, None, 0, 0, 0, out.ptr) == VN_OK
+            assert lib.vn_qkv_attention(c.handle, x.ptr, 0, nobody.ptr, nobody.ptr, T, 4, None, None, 0, 0, 1.0, out.ptr) == VN_OK
+            assert lib.vn_qkv_read(c.handle, 0, nobody.ptr, nobody.ptr, T, 4, 0, 0, c._code, out.ptr, out.ptr) == VN_OK
+        c.check()
+        assert (out.numpy() == 9).all()

@@ -598,7 +598,7 @@ int32_t vn_qkv_attention(vn_qkv* c, const void* q, int32_t n_ent, const int32_t*
   VN_REQUIRE(c->ctx, !seen || T <= QKV_MAX_DRAFT, "a tree of %d rows, at most %d", T, QKV_MAX_DRAFT);
   VN_REQUIRE(c->ctx, window >= 0, "window %d", window);
   VN_REQUIRE(c->ctx, isfinite(scale) && scale > 0.f, "a scale above zero is needed");
-  if (M == 0 || T == 0) return VN_OK;
+  if (M == 0 || T == 0 || n_ent == 0) return VN_OK;          // no entries: rows of nobody stay as they were
   VN_REQUIRE(c->ctx, q && out, "null rows");
   const int es = c->dtype == VN_F32 ? 4 : 2;
   VN_REQUIRE(c->ctx, aligned(q, 4 * es) && aligned(out, 4 * es), "rows are not aligned to four values");
