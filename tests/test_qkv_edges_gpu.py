@@ -170,3 +170,16 @@ def test_a_step_whose_rows_belong_to_nobody():
             assert lib.vn_qkv_read(c.handle, 0, nobody.ptr, nobody.ptr, T, 4, 0, 0, c._code, out.ptr, out.ptr) == VN_OK
         c.check()
         assert (out.numpy() == 9).all()
+
+
+# ---- errors -------------------------------------------------------------------------------------------------------------
+def test_a_failed_allocation_is_told_once():
+    """The call that fails says so; the next one is good."""
+    c = new(1, 64, 2, 1, 16, dtype="f32")
+    x = c.ctx.from_numpy(np.ones((1, 3, 64), np.float32))
+    want = c.attention(c.append(x)).numpy()                       # (127 times 1 / 127 in 32 bits is not quite 1)
+    for _ in range(2):
+        with pytest.raises(MemoryError):
+            c.ctx.alloc(1 << 50)
+        np.testing.assert_array_equal(c.attention(c.append(x)).numpy(), want)
+    c.check()

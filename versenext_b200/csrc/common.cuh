@@ -66,9 +66,11 @@ inline int32_t vn_fail(vn_ctx* ctx, int32_t code, const char* fmt, ...) {
 #define VN_CUDA(ctx, expr)                                                            \
   do {                                                                                \
     cudaError_t _e = (expr);                                                          \
-    if (_e != cudaSuccess)                                                            \
+    if (_e != cudaSuccess) {                                                          \
+      cudaGetLastError();    /* told here: the runtime keeps it for the next launch's check otherwise */ \
       return vn_fail((ctx), _e == cudaErrorMemoryAllocation ? VN_ERR_OOM : VN_ERR_CUDA, \
                      "%s failed: %s (%s:%d)", #expr, cudaGetErrorString(_e), __FILE__, __LINE__); \
+    }                                                                                 \
   } while (0)
 
 #define VN_CHECK_CTX(ctx)                                             \
@@ -151,7 +153,8 @@ inline cudaError_t vn_launch_pdl(vn_ctx* ctx, int level, void (*kernel)(KArgs...
     cudaError_t _e = vn_launch_pdl((ctx), (level), kernel, dim3(grid), dim3(block), (smem), __VA_ARGS__); \
     if ((ctx)->profiling) vn_prof_end((ctx));                                           \
     (ctx)->launches++;                                                                  \
-    if (_e == cudaSuccess) _e = cudaGetLastError();                                     \
+    const cudaError_t _last = cudaGetLastError();                                       \
+    if (_e == cudaSuccess) _e = _last;                                                  \
     if (_e != cudaSuccess)                                                              \
       return vn_fail((ctx), VN_ERR_CUDA, "launch of %s failed: %s", (name), cudaGetErrorString(_e)); \
   } while (0)
@@ -162,7 +165,8 @@ inline cudaError_t vn_launch_pdl(vn_ctx* ctx, int level, void (*kernel)(KArgs...
     cudaError_t _e = vn_launch_cluster((ctx), (level), (cluster_y), kernel, dim3(grid), dim3(block), (smem), __VA_ARGS__); \
     if ((ctx)->profiling) vn_prof_end((ctx));                                           \
     (ctx)->launches++;                                                                  \
-    if (_e == cudaSuccess) _e = cudaGetLastError();                                     \
+    const cudaError_t _last = cudaGetLastError();                                       \
+    if (_e == cudaSuccess) _e = _last;                                                  \
     if (_e != cudaSuccess)                                                              \
       return vn_fail((ctx), VN_ERR_CUDA, "launch of %s failed: %s", (name), cudaGetErrorString(_e)); \
   } while (0)
