@@ -461,7 +461,8 @@ int32_t vn_qkv_append(vn_qkv* c, const void* rows_dev, int64_t ld, int32_t queri
  * reads key/value head h / (H / KH).  window > 0: row at position p sees position j only if p - j < window (in a tree too:
  * of a row and its ancestors, parents before children, the last `window`).  A row that sees nothing gets zeros; one that sees
  * something, with a query that is not finite or a position that reads as NaN, gets NaN.  q_dev, out_dev
- * [M, H, head_dim], 16-byte (float32) / 8-byte aligned.  All caches of a context share one workspace, on its stream. */
+ * [M, H, head_dim], 16-byte (float32) / 8-byte aligned.  All caches of a context share one workspace, on its stream.
+ * VN_ERR_INVALID, too: more rows over more room than the kernels count, 2^30 tiles (8 rows, 32 positions of max_seq) for every SM. */
 int32_t vn_qkv_attention(vn_qkv* c, const void* q_dev, int32_t n_ent, const int32_t* ents_dev, const int32_t* row_ent_dev, int32_t T, int32_t M,
                          const uint64_t* seen_dev, const int32_t* depth_dev, int32_t tree_per_row, int32_t window, float scale, void* out_dev);
 /* Values of a step's positions, [M, KH, head_dim] each, dtype VN_F32 or VN_BF16.  Row i of an entry reads position start + i;

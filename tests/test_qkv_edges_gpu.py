@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 import qkv_cases as R
-from test_qkv_gpu import back, fill, new, stored, tables
+from test_qkv_gpu import back, check_attention, fill, new, stored, tables
 
 pytestmark = pytest.mark.gpu
 
@@ -183,3 +183,36 @@ def test_a_failed_allocation_is_told_once():
             c.ctx.alloc(1 << 50)
         np.testing.assert_array_equal(c.attention(c.append(x)).numpy(), want)
     c.check()
+
+
+# ---- sequences that may be very long ------------------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype,H,KH,d,T", [("bf16", 8, 8, 16, 1), ("f32", 4, 2, 16, 30), ("bf16", 8, 2, 64, 40)])
+def test_room_for_2_30_positions(dtype, H, KH, d, T):
+    """A pool of a few pages under a table for 2^30 positions."""
+    rng = np.random.default_rng(T)
+    c = new(1, 1 << 30, H, KH, d, dtype=dtype, pages=6)
+    table = np.full((1, c.max_pages), -1, np.int32)
+    table[0, :6] = [5, 0, 3, 1, 4, 2]
+    c.set_pages(table)
+    check_attention(c, rng, [300], [T], dtype)
+
+
+def test_more_blocks_than_32_bits_count():
+    """65 heads of 2^30 - 64 positions whose pages are one page: 2.18 10^9 blocks.  Every key is zero, so the result is the
+    mean of the values, which are the head's own: sums of equal terms that 24 bits hold."""
+    KH, d = 65, 16
+    c = new(1, 1 << 30, KH, KH, d, pages=2)
+    table = np.zeros((1, c.max_pages), np.int32)
+    table[0, -1] = 1
+    c.set_pages(table)
+    sign = np.where(np.arange(KH) % 3 == 0, -1.0, 1.0) * 2.0 ** (np.arange(KH) % 7)
+    v = np.full((64, KH, d), 64.0) * sign[None, :, None]
+    v[..., 0] = 127.0 * sign                                      # the scale: the others have the code 64
+    write(c, np.zeros((64, KH, d), np.float32), v)
+    c.set_lengths([(1 << 30) - 64])
+    c.append(np.concatenate([np.zeros((1, KH, d)), v[:1]], 1).reshape(1, 1, -1), queries=False)
+    out = back(c.attention(np.ones((1, 1, KH, d), np.float32)))[0, 0]
+    c.check()
+    # sums of weights and values are exact in a part (a few 10^6 equal terms, in 32 at a time); parts join with 2^-24 for each of
+    # some 30, and the result is rounded to bf16
+    np.testing.assert_allclose(out[:, 1:], v[0, :, 1:], rtol=2.0 ** -8)

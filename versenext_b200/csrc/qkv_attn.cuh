@@ -36,7 +36,7 @@ struct AttnCfg {
   static constexpr bool QREG = NT * NQ <= 2 && NT * NQ * P <= (RS > 1 ? 128 : 256);      // query fragments in registers, else a thread's own in shared memory
   static constexpr int STAGES = RS > 1 ? 4 : P <= 64 ? 4 : CTAS == 2 && P * NT <= 256 && QREG ? 3 : 2;
   static constexpr int RING = 0, Q = RING + RINGS * STAGES * BLOCK, BARS = Q + (QREG ? 0 : WARPS * CH * NT * NQ * 256), PLAN = BARS + RINGS * STAGES * 16,
-                       SMEM = PLAN + (THREADS + 8) * 4;
+                       SMEM = PLAN + (THREADS + 8) * 8;
   static_assert(CTAS * WARPS * WR * P <= QKV_PART, "parts fit their place");
 };
 
@@ -137,14 +137,16 @@ __device__ __forceinline__ bool unit_of(const QkvAttnArgs& a, int rts, int z, Un
   return true;
 }
 
-// The line of tiles of all (entry, rows, head) units (or of the units, where they are not cut) and what of it a worker has: tiles at .. end,
-// the first of them tile `tile` of unit (z, head).  False: nothing.  Called by all threads of a CTA; s_plan: THREADS + 8 ints
+// The line of tiles of all (entry, rows, head) units (or of the units, where they are not cut) and what of it a worker has: `end` tiles,
+// the first of them tile `tile` of unit (z, head).  The line is counted in 64 bits (65 heads of 2^30 positions), a share, from its own first tile
+// on, in 32.  False: nothing.  Called by all threads of a CTA; s_plan: THREADS + 8 numbers
 struct Share { int z, head, tile, at, end, share; };
+__device__ __forceinline__ int quotient(long long x, int y) { return x >> 31 ? (int)(x / y) : (int)x / y; }      // x >= 0, y > 0
 template <int RT, int BLK>
-__device__ __forceinline__ bool find_share(const QkvAttnArgs& a, int rts, bool split, int least, int worker, int workers, int* s_plan, Unit& u, Share& s) {
+__device__ __forceinline__ bool find_share(const QkvAttnArgs& a, int rts, bool split, int least, int worker, int workers, long long* s_plan, Unit& u, Share& s) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, KH = a.v.KH, Z = a.step.n_ent * rts, zc = (Z + THREADS - 1) / THREADS;
-  auto weight = [&]() { return (split ? u.tiles : min(u.tiles, 1)) * KH; };
-  int up = 0;
+  auto weight = [&]() { return (long long)(split ? u.tiles : min(u.tiles, 1)) * KH; };
+  long long up = 0;
   if (tid < THREADS) {
     for (int z = tid * zc; z < min(Z, (tid + 1) * zc); ++z) {
       unit_of<RT, BLK>(a, rts, z, u);
@@ -152,7 +154,7 @@ __device__ __forceinline__ bool find_share(const QkvAttnArgs& a, int rts, bool s
     }
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int t = __shfl_up_sync(0xffffffffu, up, o);
+      const long long t = __shfl_up_sync(0xffffffffu, up, o);
       if (lane >= o) up += t;
     }
     if (lane == 31) s_plan[THREADS + 1 + warp] = up;
@@ -165,25 +167,26 @@ __device__ __forceinline__ bool find_share(const QkvAttnArgs& a, int rts, bool s
     if (tid == 0) s_plan[0] = 0;
   }
   __syncthreads();
-  const int W = s_plan[THREADS];
-  s.share = max((W + workers - 1) / workers, split ? least : 1);
-  s.at = (int)min((long long)worker * s.share, (long long)W);
-  s.end = (int)min((long long)s.at + s.share, (long long)W);
-  if (s.at >= s.end) return false;
+  const long long W = s_plan[THREADS];
+  s.share = max(quotient(W + workers - 1, workers), split ? least : 1);
+  const long long from = (long long)worker * s.share;
+  if (from >= W) return false;
+  s.at = 0;
+  s.end = (int)min((long long)s.share, W - from);
   int j = 0;
 #pragma unroll
   for (int o = THREADS / 2; o > 0; o >>= 1)
-    if (s_plan[j + o] <= s.at) j += o;
+    if (s_plan[j + o] <= from) j += o;
   s.z = j * zc;
-  int rem = s.at - s_plan[j];
+  long long rem = from - s_plan[j];
   for (;; ++s.z) {
     unit_of<RT, BLK>(a, rts, s.z, u);
-    const int n = weight();
+    const long long n = weight();
     if (rem < n) break;
     rem -= n;
   }
-  s.head = split ? rem / u.tiles : rem;
-  s.tile = split ? rem - s.head * u.tiles : 0;
+  s.head = split ? quotient(rem, u.tiles) : (int)rem;
+  s.tile = split ? (int)(rem - (long long)s.head * u.tiles) : 0;
   return true;
 }
 
@@ -201,7 +204,7 @@ __global__ void __launch_bounds__(THREADS, (AttnCfg<T, P, NT, RS>::CTAS)) qkv_at
   const unsigned s_base = (unsigned)__cvta_generic_to_shared(smem);
   unsigned char* ring = smem + C::RING + ring_no * ST * C::BLOCK;
   const unsigned ring_s = s_base + C::RING + ring_no * ST * C::BLOCK, bars = s_base + C::BARS + ring_no * ST * 16;   // a stage is full, is empty
-  int* s_plan = reinterpret_cast<int*>(smem + C::PLAN);
+  long long* s_plan = reinterpret_cast<long long*>(smem + C::PLAN);
   if (lane < ST && (RS == 1 || warp == 0)) { mbar_init(bars + 16 * lane, 1); mbar_init(bars + 16 * lane + 8, RS); }
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   pdl_wait();
@@ -470,9 +473,9 @@ __global__ void __launch_bounds__(THREADS, (AttnCfg<T, P, NT, RS>::CTAS)) qkv_at
     }
     // ---- the next segment's first blocks are on their way while this one is written
     const Unit du = u;
-    const int d_head = head, done = split ? seg_b - seg_a : 1, u_begin = at - tile;
+    const int d_head = head, done = split ? seg_b - seg_a : 1;
     const bool whole = !split || done == du.tiles, begun = !whole && tile == 0;      // begun: the unit's first part is here
-    const int last = whole ? worker : (u_begin + du.tiles - 1) / share;              // who has its last
+    const int last = worker + (begun ? (at + du.tiles - 1) / share : 0);             // who has its last
     at += done;
     const bool more = at < end;
     if (more) {
@@ -640,7 +643,9 @@ struct Launch {
     units = rts * a.step.n_ent * a.v.KH;
     tiles = a.v.capacity() / blk;
     split = tiles > uncut;
-    VN_REQUIRE(c->ctx, rts < (1ll << 31) && units < (1ll << 31) / tiles - THREADS, "%d rows over %d positions are too many for one call: bring them in portions", a.step.M, a.v.capacity());
+    // what the kernels count in 32 bits: rows of an entry, units, tiles of a share and of the unit that it ends in
+    VN_REQUIRE(c->ctx, (long long)a.step.T * (a.v.H / a.v.KH) <= (1ll << 30) && units < (1ll << 31) - THREADS && units * tiles / c->ctx->sm_count < (1ll << 30),
+               "%d rows over %d positions are too many for one call: bring them in portions", a.step.M, a.v.capacity());
     return VN_OK;
   }
   // shares that there can be

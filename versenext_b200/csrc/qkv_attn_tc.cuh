@@ -23,7 +23,7 @@ struct TcCfg {
   static constexpr int PANELS = P / 64, PAGE = 2 * QKV_BLOCK * (2 * P + 8), STAGES = P > 64 ? 2 : 3;
   static constexpr int Q = 0, K = Q + PANELS * TC_ROWS * 128, V = K + PANELS * TC_KEYS * 128, RAW = V + PANELS * TC_KEYS * 128, SCALES = RAW + STAGES * PAGE,
                        WEIGHTS = SCALES + 3 * 2 * TC_KEYS * 4, META = WEIGHTS + TC_SOFT * 32 * 4, FACTORS = META + 64, PAIRS = FACTORS + 2 * TC_ROWS * 4, BARS = PAIRS + 2 * 2 * TC_ROWS * 4, SLOT = BARS + 16 * 8, PLAN = SLOT + 16,
-                       SMEM = PLAN + (THREADS + 8) * 4 + 1024;        // the first 1024: the swizzle's alignment
+                       SMEM = PLAN + (THREADS + 8) * 8 + 1024;        // the first 1024: the swizzle's alignment
   static constexpr unsigned S_COL = 0, O_COL = 128;          // scores of even and odd pages, whose first half the weights take over; results
   static_assert(P % 64 == 0 && O_COL + P <= 256, "256 columns of TMEM for each of two CTAs");
   static_assert(TC_CTAS * TC_ROWS * P <= QKV_PART, "parts fit their place");
@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) qkv_attn_tc_kernel(QkvAtt
   pdl_wait();
   Unit u;
   Share sh;
-  if (!find_share<TC_ROWS, TC_KEYS>(a, rts, split, TC_MIN_SHARE, blockIdx.x, gridDim.x, reinterpret_cast<int*>(smem + C::PLAN), u, sh)) return;
+  if (!find_share<TC_ROWS, TC_KEYS>(a, rts, split, TC_MIN_SHARE, blockIdx.x, gridDim.x, reinterpret_cast<long long*>(smem + C::PLAN), u, sh)) return;
   unsigned* s_slot = reinterpret_cast<unsigned*>(smem + C::SLOT);
   if (warp == TC_SOFT + 4) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(s_base + C::SLOT), "r"(256u) : "memory");
@@ -426,9 +426,8 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) qkv_attn_tc_kernel(QkvAtt
       wait_results(n - 1);
       __syncwarp();
       tc_fence_after();
-      const int u_begin = sh.at - sh.tile;
       const bool whole = !split || seg_n == u.tiles, begun = !whole && sh.tile == 0;
-      const int last = whole ? 0 : (u_begin + u.tiles - 1) / sh.share, part = 2 * blockIdx.x + (begun ? 1 : 0);
+      const int part = 2 * blockIdx.x + (begun ? 1 : 0);
       const float r_inv = pow2(R - 10), inv = whole ? (l == 0.f ? 0.f : r_inv / l) : r_inv;
       bf16* out = reinterpret_cast<bf16*>(a.out) + ((long long)(u.r0 + max(tok, 0)) * v.H + sh.head * G + (f - max(tok, 0) * G)) * v.d;
       float* part_o = a.part_o + ((long long)part * TC_ROWS + row) * P;
@@ -469,7 +468,7 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) qkv_attn_tc_kernel(QkvAtt
       }
       if (!whole && tok >= 0 && half == 0) a.part_ml[part * TC_ROWS + row] = make_float2(m, l);
       if (begun && tid == 0) {                               // a unit to merge: in any order, each by itself
-        const int cnt = last - (int)blockIdx.x + 1;
+        const int cnt = (sh.at + u.tiles - 1) / sh.share + 1;
         const bool many = cnt > MANY;
         const int at = atomicAdd(a.n_cuts + (many ? 1 : 0), 1);
         a.cuts[many ? a.max_cuts - 1 - at : at] = {u.r0, u.f0, u.nf, sh.head, (int)blockIdx.x, cnt};
