@@ -1,4 +1,6 @@
-"""QuantKVCache on the device where it is easiest to get wrong."""
+"""QuantKVCache on the device where it is easiest to get wrong: scores that differ much between the parts of a sequence, values that differ
+much in size, rows that are not finite, tables out of range, very long sequences, trees of their own for every entry, offsets, narrow windows,
+graphs in turn, and a loop whose rounds are the plain cache's."""
 
 import numpy as np
 import pytest
@@ -216,3 +218,197 @@ def test_more_blocks_than_32_bits_count():
     # sums of weights and values are exact in a part (a few 10^6 equal terms, in 32 at a time); parts join with 2^-24 for each of
     # some 30, and the result is rounded to bf16
     np.testing.assert_allclose(out[:, 1:], v[0, :, 1:], rtol=2.0 ** -8)
+
+
+@pytest.mark.parametrize("scheme", ["int8", "fp8"])
+@pytest.mark.parametrize("dtype,H,d,T", [("bf16", 2, 64, 1), ("f32", 2, 64, 1), ("bf16", 4, 128, 16), ("bf16", 2, 256, 3), ("f32", 2, 80, 20)])
+@pytest.mark.parametrize("order", [1, -1, 0])
+def test_values_that_differ_much_in_size(scheme, dtype, H, d, T, order):
+    """Heads of values from 10^-15 to 10^15, smallest first, largest first, or mixed."""
+    rng = np.random.default_rng(d + order)
+    n = 900
+    size = np.linspace(-15, 15, n + T)[::order or 1]
+    size = 10.0 ** (rng.permutation(size) if order == 0 else size)
+    c = new(1, n + T, H, 1, d, scheme=scheme, dtype=dtype)
+    q, k = stored(rng.normal(0, 1, (T, H, d)), dtype), stored(rng.normal(0, 1, (n + T, 1, d)), dtype)
+    check_one(c, q, k, stored(rng.normal(0, 1, (n + T, 1, d)) * size[:, None, None], dtype), n, dtype)
+
+
+# ---- trees, windows, offsets ------------------------------------------------------------------------------------------
+def grown(rng, n):
+    return [int(rng.integers(-1, i)) if i else -1 for i in range(n)]
+
+
+@pytest.mark.parametrize("scheme", ["int8", "fp8"])
+@pytest.mark.parametrize("dtype,H,KH,d,most", [("bf16", 4, 4, 64, 15), ("bf16", 8, 2, 128, 40), ("f32", 2, 1, 64, 30), ("bf16", 4, 2, 96, 64)])
+@pytest.mark.parametrize("window", [0, 2, 50])
+def test_a_tree_for_every_entry(scheme, dtype, H, KH, d, most, window):
+    rng = np.random.default_rng(d + window)
+    B, lens, counts = 5, [200, 0, 31, 500, 64], [most, 1, 0, most // 2, 7]
+    slots = [3, 0, 4, 1, 2]
+    c = new(B, 600, H, KH, d, scheme=scheme, dtype=dtype)
+    lens = np.asarray(lens)
+    old = fill(c, rng, lens.tolist(), dtype)
+    trees = [grown(rng, n) for n in counts]
+    trees[0] = [i - 1 for i in range(most)]                # a path
+    M = sum(counts)
+    cs, sn = tables(c.max_seq, d // 2)
+    x = stored(rng.normal(0, 1, (M + 3, (H + 2 * KH) * d)), dtype)
+    step = c.step(slots, counts)
+    tree = c.tree(trees, step)
+    out = c.ctx.from_numpy(np.full((M + 3, H, d), 7, c._np))
+    q = c.append(x, step=step, tree=tree, rope=(cs, sn))
+    got = back(c.attention(q, step=step, tree=tree, window=window, out=out))
+    assert (out.numpy()[M:] == 7).all()
+    q = back(q)
+    k, v = (a.numpy() for a in c.read(step, dtype="f32"))
+    c.check()
+    at = 0
+    for b, n, parents in zip(slots, counts, trees):
+        if n:
+            depth, seen = R.depth_and_seen(parents, n)
+            h = x[at:at + n].reshape(n, H + 2 * KH, d)
+            both = R.heads_in(h[:, :H + KH], None, 0, lens[b] + depth, cs, sn, False)
+            # two products and a sum in 32 bits, relative to the larger of a pair's channels; half a step of the type, half a code
+            size = np.abs(both).max(-1, keepdims=True)
+            off = 2.0 ** -24 * 4 * 2 * size
+            assert (np.abs(q[at:at + n] - both[:, :H]) <= off[:, :H] + (2.0 ** -8 if dtype == "bf16" else 0) * np.abs(both[:, :H]) * 1.001).all()
+            code = size[:, H:] / 127 / 2 if scheme == "int8" else np.maximum(np.abs(both[:, H:]) * 2.0 ** -4, size[:, H:] / 448 * 2.0 ** -10)
+            assert (np.abs(k[at:at + n] - both[:, H:]) <= code * 1.001 + 2 * off[:, H:]).all()
+            np.testing.assert_array_equal(v[at:at + n], R.in_8_bits(h[:, H + KH:], scheme))
+            kk, vv = np.concatenate([old[b][0], k[at:at + n]]), np.concatenate([old[b][1], v[at:at + n]])
+            want, weight, reach = R.attention(q[at:at + n], kk, vv, lens[b], depth, seen, window, d ** -0.5)
+            tol = R.tolerance(want, weight, reach, d, lens[b] + n, dtype, scheme == "int8")
+            assert (np.abs(got[at:at + n] - want) <= tol).all(), (b, float(np.max(np.abs(got[at:at + n] - want) / tol)))
+        at += n
+
+
+@pytest.mark.parametrize("dtype,H,d", [("bf16", 1, 64), ("bf16", 1, 256), ("f32", 2, 64), ("f32", 1, 16)])
+@pytest.mark.parametrize("window", [1, 2, 3, 5, 17])
+def test_windows_narrower_than_a_path_with_few_rows(dtype, H, d, window):
+    rng = np.random.default_rng(window + d)
+    c = new(3, 300, H, 1, d, dtype=dtype)
+    check_attention(c, rng, [250, 0, 64], [8] * 3, dtype, parents=[-1, 0, 1, 2, 3, 1, 5, 6], window=window)
+    check_attention(c, rng, [250, 0, 64], [8] * 3, dtype, window=window)
+
+
+@pytest.mark.parametrize("scheme", ["int8", "fp8"])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_offsets(scheme, dtype):
+    """A step brought in three portions, each `offset` further on, is the step brought at once; `read` finds each portion."""
+    rng = np.random.default_rng(18)
+    B, H, KH, d, n = 3, 4, 2, 64, 70
+    lens = [0, 61, 130]
+    cs, sn = tables(256, 32)
+    w = rng.normal(1, 0.3, d).astype(np.float32)
+    x = stored(rng.normal(0, 1, (B, n, (H + 2 * KH) * d)), dtype)
+    kw = dict(q_norm=w, k_norm=w, rope=(cs, sn))
+    a, b = (new(B, 250, H, KH, d, scheme=scheme, dtype=dtype) for _ in "ab")
+    for c in (a, b):
+        fill(c, np.random.default_rng(19), lens, dtype)
+    whole = back(a.append(x, **kw))
+    ka, va = (t.numpy() for t in a.read((B, n), dtype="f32"))
+    for lo, hi in ((3, 40), (0, 3), (40, n)):
+        np.testing.assert_array_equal(back(b.append(np.ascontiguousarray(x[:, lo:hi]), offset=lo, **kw)), whole[:, lo:hi])
+        k, v = (t.numpy() for t in b.read((B, hi - lo), offset=lo, dtype="f32"))
+        np.testing.assert_array_equal(k, ka[:, lo:hi])
+        np.testing.assert_array_equal(v, va[:, lo:hi])
+    for i in range(B):
+        want = R.heads_in(x[i].reshape(n, H + 2 * KH, d)[:, :H], w, 1e-6, lens[i] + np.arange(n), cs, sn, False)
+        size = np.abs(want).max(-1, keepdims=True)
+        assert (np.abs(whole[i] - want) <= 2.0 ** -24 * 32 * size + (2.0 ** -8 if dtype == "bf16" else 0) * np.abs(want) * 1.001).all()     # as in the test of append
+    s = b.step([2, 0], [2, 5])
+    k, v = (t.numpy() for t in b.read(s, offset=7, dtype="f32"))
+    np.testing.assert_array_equal(k, np.concatenate([ka[2, 7:9], ka[0, 7:12]]))
+    np.testing.assert_array_equal(v, np.concatenate([va[2, 7:9], va[0, 7:12]]))
+    b.check()
+    np.testing.assert_array_equal(back(a.attention(whole)), back(b.attention(whole)))
+
+
+# ---- a loop: every round against the plain cache ------------------------------------------------------------------------
+@pytest.mark.parametrize("scheme,dtype,H,KH,d", [("int8", "f32", 8, 2, 64), ("fp8", "bf16", 4, 2, 128), ("int8", "bf16", 2, 2, 80)])
+def test_a_loop_whose_rounds_are_the_plain_caches(scheme, dtype, H, KH, d):
+    """Prompt, then rounds of a tree: norms, rotation, attention, commit.  Keys are within half a code of the formulas', values are the
+    definition's, and the attention is that of what the cache then holds."""
+    rng = np.random.default_rng(20)
+    B, n = 3, 16
+    c = new(B, 400, H, KH, d, scheme=scheme, dtype=dtype)
+    cs, sn = tables(c.max_seq, d // 2)
+    w = rng.normal(1, 0.2, (2, d)).astype(np.float32)
+    held = [np.zeros((2, 0, KH, d), np.float32) for _ in range(B)]
+    for r, T in enumerate([90, n, n, n, n]):
+        parents = R.TREE16 if r else None
+        x = stored(rng.normal(0, 1, (B, T, (H + 2 * KH) * d)), dtype)
+        tree = c.tree(parents) if r else None
+        q = c.append(x, tree=tree, q_norm=w[0], k_norm=w[1], rope=(cs, sn))
+        got = back(c.attention(q, tree=tree))
+        q = back(q)
+        k, v = (a.numpy() for a in c.read((B, T), dtype="f32"))
+        keep = np.zeros((B, T), np.int32)
+        if r:
+            paths = ([0, 1, 5, 13], [0], [0, 3, 10])
+            kept = [len(p) for p in paths]
+            for b, p in enumerate(paths):
+                keep[b, :len(p)] = p
+        else:
+            kept, paths = [90, 71, 0], [list(range(90)), list(range(71)), []]
+        c.commit(T, np.asarray(kept, np.int32), keep if r else None)
+        depth, seen = R.depth_and_seen(parents, T)
+        for b in range(B):
+            m = held[b].shape[1]
+            h = x[b].reshape(T, H + 2 * KH, d)
+            for key in (False, True):
+                want = R.heads_in(h[:, H:H + KH] if key else h[:, :H], w[int(key)], 1e-6, m + depth, cs, sn, False)
+                size = np.abs(want).max(-1, keepdims=True)
+                if key:
+                    step = size / 254 if scheme == "int8" else np.maximum(np.abs(want) * 2.0 ** -4, size / 448 * 2.0 ** -10)
+                else:
+                    step = (2.0 ** -8 if dtype == "bf16" else 0) * np.abs(want)
+                assert (np.abs((k if key else q)[b] - want) <= 2.0 ** -24 * 64 * size + step * 1.001).all()       # 32-bit steps as in the test of append
+            np.testing.assert_array_equal(v[b], R.in_8_bits(h[:, H + KH:], scheme))
+            kk, vv = np.concatenate([held[b][0], k[b]]), np.concatenate([held[b][1], v[b]])
+            out, weight, reach = R.attention(q[b], kk, vv, m, depth, seen, 0, d ** -0.5)
+            tol = R.tolerance(out, weight, reach, d, m + T, dtype, scheme == "int8")
+            assert (np.abs(got[b] - out) <= tol).all(), (r, b, float(np.max(np.abs(got[b] - out) / tol)))
+            held[b] = np.concatenate([held[b], np.stack([k[b], v[b]])[:, paths[b]]], 1)
+        assert c.per_seq_lens.tolist() == [x.shape[1] for x in held]
+        for b in range(B):
+            kb, vb = c.get(b)
+            np.testing.assert_array_equal(kb, held[b][0])
+            np.testing.assert_array_equal(vb, held[b][1])
+    c.check()
+
+
+def test_two_captured_graphs_in_turn():
+    """Both use the context's workspace; replayed in any order, with eager calls between, each gives what it gave eagerly."""
+    import ctypes as C
+    rng = np.random.default_rng(21)
+    few, many = new(16, 2200, 16, 8, 64), new(4, 1500, 8, 1, 128, scheme="fp8")
+    fill(few, rng, [2000] * 16, "bf16", loud=False)
+    fill(many, rng, [1400, 3, 0, 700], "bf16", loud=False)
+    few.set_lengths([2000 - 1] * 16)
+    many.set_lengths([1400 - 30, 3, 0, 600])
+    ctx, lib = few.ctx, few.ctx.lib
+    made = []
+    for c, T in ((few, 1), (many, 30)):
+        q = ctx.from_numpy(rng.integers(0x3c00, 0x4000, (c.max_batch, T, c.n_head, c.head_dim)).astype(np.uint16))
+        want = c.attention(q).numpy()
+        o = ctx.zeros(want.shape, np.uint16)
+        ctx._check(lib.vn_graph_begin(ctx.handle))
+        c.attention(q, out=o)
+        graph = C.c_void_p()
+        ctx._check(lib.vn_graph_end(ctx.handle, C.byref(graph)))
+        made.append((c, q, o, want, graph))
+    for which in rng.integers(0, 4, 40):
+        c, q, o, want, graph = made[which % 2]
+        if which < 2:
+            ctx._check(lib.vn_memset(ctx.handle, C.c_void_p(o.ptr), 0, o.nbytes))
+            ctx._check(lib.vn_graph_launch(ctx.handle, graph))
+        np.testing.assert_array_equal((o if which < 2 else c.attention(q)).numpy(), want)
+    for _ in range(20):                                           # nothing read between
+        for c, q, o, want, graph in made:
+            ctx._check(lib.vn_graph_launch(ctx.handle, graph))
+    for c, q, o, want, graph in made:
+        np.testing.assert_array_equal(o.numpy(), want)
+        ctx._check(lib.vn_graph_destroy(ctx.handle, graph))
+        c.check()
