@@ -449,6 +449,9 @@ int32_t vn_qkv_set_lengths(vn_qkv* c, const int32_t* lens, int32_t on_device);  
  * range, or a length, a depth under a window (0 .. 63) or a position to rotate by (the tables' rows), which count as the nearest in
  * range (VN_ERR_INDEX).  VN_ERR_TIMEOUT: a copy from the cache did not arrive; that call's results are no good. */
 int32_t vn_qkv_status(vn_qkv* c, int32_t* no_room, int32_t* bad_index);
+/* Diagnostic: one wait for a copy that nobody has asked for, of at most `cycles` (up to 4 10^9, the attention kernels' limit); it sets what a
+ * copy that does not arrive sets.  *waited_cycles: what it took. */
+int32_t vn_qkv_probe_wait(vn_qkv* c, uint64_t cycles, int64_t* waited_cycles);
 /* Writes a step's keys and values at positions length + offset + i; lengths stay.  rows_dev [M][ld]: the H query heads (only with
  * queries != 0), the KH key heads, the KH value heads.  In the same pass, for query and key heads: x / sqrt(mean x^2 + eps) * norm
  * (float32 [head_dim], NULL: none), then the rotation of `pairs` pairs (half-split, or neighbours with interleaved != 0) by

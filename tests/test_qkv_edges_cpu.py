@@ -99,3 +99,9 @@ def test_arrays_of_another_device():
         assert len(c.ctx.lib.calls) == n
         call(c.ctx.from_numpy)
         assert len(c.ctx.lib.calls) == n + 1
+
+
+def test_the_probe_refuses_null():
+    import ctypes as C
+    from versenext_b200 import _lib
+    assert _lib.load().vn_qkv_probe_wait(None, 1, C.byref(C.c_int64())) == _lib.VN_ERR_INVALID

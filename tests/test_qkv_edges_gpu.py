@@ -412,3 +412,23 @@ def test_two_captured_graphs_in_turn():
         np.testing.assert_array_equal(o.numpy(), want)
         ctx._check(lib.vn_graph_destroy(ctx.handle, graph))
         c.check()
+
+
+def test_a_copy_that_does_not_come_is_reported():
+    """A wait that runs out sets the condition; it is told once, and the next call is good."""
+    import ctypes as C
+    from versenext_b200._lib import VN_ERR_INVALID
+    rng = np.random.default_rng(22)
+    c = new(1, 300, 2, 1, 64, dtype="f32")
+    check_attention(c, rng, [200], [3], "f32")
+    q = rng.normal(0, 1, (1, 3, 2, 64)).astype(np.float32)
+    want = c.attention(q).numpy()
+    waited = C.c_int64()
+    c.ctx._check(c.ctx.lib.vn_qkv_probe_wait(c.handle, 2_000_000, C.byref(waited)))       # about a millisecond
+    assert 2_000_000 <= waited.value < 200_000_000
+    with pytest.raises(RuntimeError):
+        c.check()
+    c.check()
+    np.testing.assert_array_equal(c.attention(q).numpy(), want)
+    for cycles in (0, 1 << 40):
+        assert c.ctx.lib.vn_qkv_probe_wait(c.handle, cycles, None) == VN_ERR_INVALID

@@ -134,6 +134,7 @@ PROTOTYPES = {
     "vn_qkv_lengths": [_p, _p],
     "vn_qkv_set_lengths": [_p, _p, _i32],
     "vn_qkv_status": [_p, C.POINTER(_i32), C.POINTER(_i32)],
+    "vn_qkv_probe_wait": [_p, _u64, C.POINTER(_i64)],
     "vn_qkv_append": [_p, _p, _i64, _i32, _i32, _p, _p, _i32, _i32, _i32, _p, _i32, _p, _p, _f32, _p, _p, _i32, _i32, _i32, _p],
     "vn_qkv_attention": [_p, _p, _i32, _p, _p, _i32, _i32, _p, _p, _i32, _i32, _f32, _p],
     "vn_qkv_read": [_p, _i32, _p, _p, _i32, _i32, _i32, _i32, _i32, _p, _p],

@@ -4,7 +4,7 @@
 #include <algorithm>
 #include <new>
 
-#include "qkv.cuh"
+#include "qkv_attn.cuh"
 
 namespace {
 
@@ -371,6 +371,17 @@ __global__ void set_lengths_kernel(QkvView v, const int* __restrict__ from) {
   v.lens[i] = min(max(n, 0), v.capacity());
 }
 
+// a wait as the attention kernels', for what never comes
+__global__ void qkv_wait_probe_kernel(int* status, unsigned long long limit, long long* waited) {
+  __shared__ __align__(8) unsigned long long bar;
+  const unsigned b = (unsigned)__cvta_generic_to_shared(&bar);
+  qkv_detail::mbar_init(b, 1);
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  const long long t0 = clock64();
+  if (!qkv_detail::mbar_try1(b, 0) && !qkv_detail::mbar_wait_long(b, 0, limit)) status[2] = 1;
+  *waited = clock64() - t0;
+}
+
 // layout of vn_ctx::qkv_parts: two parts for every share (CTA, or warp with a quarter of the rows) that the attention kernel may have
 struct Parts { size_t ml, cuts, n_cuts, bytes; int max_cuts; };
 Parts parts_of(const vn_ctx* ctx) {
@@ -509,6 +520,23 @@ int32_t vn_qkv_status(vn_qkv* c, int32_t* no_room, int32_t* bad_index) {
   if (s[2]) return vn_fail(c->ctx, VN_ERR_TIMEOUT, "a copy from the cache did not arrive");
   if (s[0]) return vn_fail(c->ctx, VN_ERR_OVERFLOW, "a position behind the cache's end, or without a page, was written or read");
   if (s[1]) return vn_fail(c->ctx, VN_ERR_INDEX, "a sequence, row or count outside its range was met");
+  return VN_OK;
+}
+
+int32_t vn_qkv_probe_wait(vn_qkv* c, uint64_t cycles, int64_t* waited) {
+  VN_CHECK_QKV(c);
+  VN_REQUIRE(c->ctx, cycles > 0 && cycles <= qkv_detail::WAIT_CYCLES, "a wait of 1 to %llu cycles", qkv_detail::WAIT_CYCLES);
+  long long* d = nullptr;
+  VN_CUDA(c->ctx, cudaMalloc(&d, sizeof *d));
+  qkv_wait_probe_kernel<<<1, 1, 0, c->ctx->stream>>>(c->v.status, cycles, d);
+  c->ctx->launches++;
+  long long h = 0;
+  cudaError_t e = cudaGetLastError();
+  if (e == cudaSuccess) e = cudaMemcpyAsync(&h, d, sizeof h, cudaMemcpyDeviceToHost, c->ctx->stream);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(c->ctx->stream);
+  cudaFree(d);
+  VN_CUDA(c->ctx, e);
+  if (waited) *waited = h;
   return VN_OK;
 }
 

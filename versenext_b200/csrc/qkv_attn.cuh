@@ -25,7 +25,9 @@ constexpr int MIN_SHARE = 4;                        // blocks of a share at leas
 constexpr int MERGE_WARPS = 8, MANY = 8;           // warps of a merging CTA; parts that one of them takes
 constexpr int UNCUT = 8;                            // blocks of a unit that is never cut
 constexpr int MERGE_CTAS = 4;                       // merging CTAs on an SM
-constexpr unsigned long long WAIT_CYCLES = 4000000000ull;   // a copy that has not come after about two seconds never will
+// A copy that has not come after about two seconds is taken not to come.  The call is then no good and reported; whoever has met it asks for no more,
+// and before its memory goes to somebody else waits once more, LATE_CYCLES, for each copy that it has asked for
+constexpr unsigned long long WAIT_CYCLES = 4000000000ull, LATE_CYCLES = 1000000ull;
 
 template <typename T, int P, int NT, int RS>
 struct AttnCfg {
@@ -216,7 +218,7 @@ __global__ void __launch_bounds__(THREADS, (AttnCfg<T, P, NT, RS>::CTAS)) qkv_at
   int z = sh.z, head = sh.head, tile = sh.tile, at = sh.at;
   const int end = sh.end, share = sh.share;
 
-  unsigned it = 0, put = 0;                                  // blocks taken and asked for
+  unsigned it = 0, put = 0;                                  // blocks taken, and asked for (by the lane that asks)
   bool dead = false;                                         // a copy did not come: nothing is computed any more
   int page_cur = -1, page_nxt = -1;                          // pages of the next 32 and 64 blocks of a segment
   int seg_a = 0, seg_b = 0;
@@ -225,17 +227,18 @@ __global__ void __launch_bounds__(THREADS, (AttnCfg<T, P, NT, RS>::CTAS)) qkv_at
     return i < seg_b ? v.page(u.slot, i * QKV_BLOCK / KV_PAGE) : -1;
   };
   auto came = [&](unsigned bar, unsigned parity) {           // bounded wait
-    if (!mbar_try1(bar, parity) && !mbar_wait_long(bar, parity, dead ? 1000000ull : WAIT_CYCLES)) dead = true;
+    if (!dead && !mbar_try1(bar, parity) && !mbar_wait_long(bar, parity, WAIT_CYCLES)) dead = true;
   };
   auto ask = [&](int k, int page) {                          // block k of this segment
     if (RS > 1 && warp) return;
     if (lane == 0) {
       const unsigned s = put % ST, bar = bars + 16 * s;
       if (RS > 1 && put >= ST) came(bar + 8, (put / ST - 1) & 1);
-      if (page >= 0 && !dead) fetch_block(ring_s + s * C::BLOCK, v.block(page, head, (seg_a + k) & 1), C::BLOCK, bar);
+      if (dead) return;
+      if (page >= 0) fetch_block(ring_s + s * C::BLOCK, v.block(page, head, (seg_a + k) & 1), C::BLOCK, bar);
       else mbar_arrive1(bar);
+      ++put;
     }
-    ++put;
   };
   constexpr int AHEAD = RS > 1 ? ST - 1 : ST;                // blocks asked for before their turn; shared ones leave a stage to the slowest warp
   auto begin_segment = [&]() {
@@ -524,6 +527,8 @@ __global__ void __launch_bounds__(THREADS, (AttnCfg<T, P, NT, RS>::CTAS)) qkv_at
     }
     if (!more) break;
   }
+  if (dead)
+    for (unsigned s = 0; s < min(put, (unsigned)ST); ++s) mbar_wait_long(bars + 16 * s, ((put - 1 - s) / ST) & 1, LATE_CYCLES);
 }
 
 // Parts of the units that were cut, in the order of their shares: a warp for a row, or, with many parts, a CTA.  The last CTA empties

@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) qkv_attn_tc_kernel(QkvAtt
   const unsigned tmem = *s_slot;
   bool dead = false;                                         // a wait ran out: the results are no good, but everybody comes to the end
   auto wait = [&](int b, unsigned parity) {
-    if (!mbar_try1(bar(b), parity) && !mbar_wait_long(bar(b), parity, dead ? 1000000ull : WAIT_CYCLES)) { dead = true; v.status[2] = 1; }
+    if (!mbar_try1(bar(b), parity) && !mbar_wait_long(bar(b), parity, dead ? LATE_CYCLES / 16 : WAIT_CYCLES)) { dead = true; v.status[2] = 1; }
   };
   auto wait_scores = [&](unsigned t) { wait(S_FULL + (t & 1), (t >> 1) & 1); };
   auto wait_results = [&](unsigned t) { wait(PV_DONE + (t & 1), (t >> 1) & 1); };
@@ -186,12 +186,12 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) qkv_attn_tc_kernel(QkvAtt
         n += seg_n;
       } while (advance());
       tc_commit(bar(ALL_DONE));                              // no product is under way when the memory is given back, whatever became of the waits
-      wait(ALL_DONE, 0);
+      if (!mbar_wait_long(bar(ALL_DONE), 0, WAIT_CYCLES)) v.status[2] = 1;
     }
   } else if (warp >= TC_SOFT) {
     // ---- queries and codes to halves: the keys of page i + 1 before the values of page i
     const int ct = tid - 32 * TC_SOFT, cw = warp - TC_SOFT, rg = lane >> 2, rc = lane & 3;
-    unsigned asked = 0;                                      // pages asked for in all
+    unsigned asked = 0;                                      // pages asked for in all, by the lane that asks
     do {
       begin();
       // pages of the segment, 32 at a time: lane j has that of page first + j
@@ -202,9 +202,9 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) qkv_attn_tc_kernel(QkvAtt
       auto page = [&](int i) { return __shfl_sync(0xffffffffu, i - first < 32 ? pages : next_pages, (i - first) & 31); };
       auto ask = [&](int i) {                                // by one warp: nobody reads the stage any more
         const int pg = page(i);
+        if (lane || dead) return;
         const unsigned s = asked++ % ST;
-        if (lane) return;
-        if (pg >= 0 && !dead) fetch_block(s_base + C::RAW + s * C::PAGE, v.block(pg, sh.head, 0), C::PAGE, bar(RAW_FULL + s));
+        if (pg >= 0) fetch_block(s_base + C::RAW + s * C::PAGE, v.block(pg, sh.head, 0), C::PAGE, bar(RAW_FULL + s));
         else mbar_arrive1(bar(RAW_FULL + s));
       };
       if (cw == 0)
@@ -296,6 +296,8 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) qkv_attn_tc_kernel(QkvAtt
       }
       n += seg_n;
     } while (advance());
+    if (dead)
+      for (unsigned s = 0; s < min(asked, (unsigned)ST); ++s) mbar_wait_long(bar(RAW_FULL + s), ((asked - 1 - s) / ST) & 1, LATE_CYCLES);
   } else {
     // ---- soft-max: warps w and w + 4 have the two halves of the columns of rows 32 (w mod 4) ..
     const int half = warp >> 2, row = tid & 127;
