@@ -50,10 +50,8 @@ def _below_2_31(**numbers):
 
 def _in_32_bits(ctx: Context, a, name: str) -> DeviceArray:
     """Whole numbers on the device; those of the host have to fit."""
-    if hasattr(a, "requires_grad"):
-        a = a.data
     if not isinstance(a, DeviceArray):
-        a = np.asarray(a)
+        a = np.asarray(a.data if hasattr(a, "requires_grad") else a)
         if a.size and a.dtype != np.int32 and (a.min() < -_END or a.max() >= _END):
             raise ValueError(f"{name} holds a number that 32 bits do not")
     return as_device(ctx, a, np.int32)
@@ -139,7 +137,7 @@ class QuantKVCache:
         self.pages = int(pages) or self.max_batch * self.max_pages
 
     def _here(self, a: DeviceArray) -> DeviceArray:
-        if a.ctx.device != self.ctx.device:
+        if a.ctx is not self.ctx and a.ctx.device != self.ctx.device:
             raise ValueError(f"an array on device {a.ctx.device} for a cache on device {self.ctx.device}")
         return a
 
@@ -200,7 +198,8 @@ class QuantKVCache:
         if shape[k:] != tail or k < 0:
             raise ValueError(f"rows of shape {tuple(shape)} do not end in {tuple(tail)}")
         if step is not None:
-            self._here(step._buf)
+            if step._buf.ctx is not self.ctx:
+                self._here(step._buf)
             m = math.prod(lead)
             if m < step.rows:
                 raise ValueError(f"{m} rows for a step of {step.rows}")
@@ -219,14 +218,15 @@ class QuantKVCache:
             raise ValueError(f"a tree of {tree.T} rows for entries of {T}")
         if T > MAX_DRAFT:
             raise ValueError(f"a tree has at most {MAX_DRAFT} rows, not {T}")
-        self._here(tree._buf)
+        if tree._buf.ctx is not self.ctx:
+            self._here(tree._buf)
         return tree.seen, tree.depth, tree.per_row
 
     def _in(self, x):
         if isinstance(x, DeviceArray):
             if x.dtype != self._np:
                 raise TypeError(f"device array has dtype {x.dtype}, need {self._np}")
-            return self._here(x)
+            return x if x.ctx is self.ctx else self._here(x)
         x = np.asarray(x)
         if self.dtype == "bf16" and x.dtype != np.uint16:
             x = to_bf16(x)
@@ -239,7 +239,7 @@ class QuantKVCache:
             return self.ctx.empty(shape, dtype)
         if not isinstance(out, DeviceArray) or out.dtype != dtype or out.size < math.prod(shape):
             raise ValueError(f"out must be a device array of {np.dtype(dtype)} with room for {tuple(shape)}")
-        return self._here(out)
+        return out if out.ctx is self.ctx else self._here(out)
 
     def _weight(self, a, name):
         a = self._here(as_device(self.ctx, a, np.float32))
