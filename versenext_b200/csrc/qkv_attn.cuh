@@ -709,16 +709,19 @@ int32_t pick(vn_qkv* c, const QkvAttnArgs& a) {
 #define GO(P, NT, RS) return c->dtype == VN_F32 ? launch<float, SCHEME, P, NT, RS>(c, a) : launch<bf16, SCHEME, P, NT, RS>(c, a)
 #define GO2(P) do { if (rows <= 8) GO(P, 1, 1); else if (rows <= 16) GO(P, 2, 1); else GO(P, 2, 4); } while (0)
 #define GO4(P) do { if (rows <= 8) GO(P, 1, 1); else if (rows <= 16) GO(P, 2, 1); else if (rows <= 64) GO(P, 2, 4); else GO(P, 4, 4); } while (0)
+// (bf16 rows that are many have gone to tcgen05)
+#define GOF(P) do { if (rows <= 8) GO(P, 1, 1); else if (rows <= 16) GO(P, 2, 1); else return rows <= 64 ? launch<float, SCHEME, P, 2, 4>(c, a) : launch<float, SCHEME, P, 4, 4>(c, a); } while (0)
   switch (a.v.P) {
     case 32: GO4(32);
-    case 64: GO4(64);
+    case 64: GOF(64);
     case 80: GO4(80);
     case 96: GO4(96);
-    case 128: GO4(128);
+    case 128: GOF(128);
     case 192: GO2(192);
     case 256: GO2(256);
     default: return vn_fail(c->ctx, VN_ERR_UNSUPPORTED, "pitch %d", a.v.P);
   }
+#undef GOF
 #undef GO4
 #undef GO2
 #undef GO
