@@ -105,8 +105,9 @@ __device__ __forceinline__ void put_eight(bf16* p, const float (&x)[8], bool who
 }
 
 // A warp takes `per` tasks of a row, four asked for at a time: a task is 32 / L neighbouring heads, whose lanes hold eight channels each.
-// Heads pass through shared memory only for half-split rotation, where a channel meets the one `pairs` further on.  Bound by
-// instructions for many rows (with four channels a lane a prompt of 8000 rows of 2048 values took 48 us, twice as long); for few, the
+// Heads pass through shared memory only for half-split rotation, where a channel meets the one `pairs` further on.  For many
+// rows it is bound by instructions (rotation, maxima, quotients: two thirds of the issue slots) and by waits for the row, its entry, length and
+// page (a prompt of 8000 rows of 2048 values takes 37 us with events around it, 48 with four channels a lane); for few, by the
 // chain entry, length, page, store (the row's values are asked for first).  grid ceil(M ceil(tasks / per) / 8), block 256
 template <typename T, int SCHEME, int L>
 __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 4 : 2) qkv_append_kernel(AppendArgs a, int tasks, int per) {

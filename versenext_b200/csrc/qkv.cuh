@@ -122,11 +122,3 @@ constexpr int QKV_MAX_CTAS = 3;                     // of the attention kernel o
 constexpr int QKV_PART = 2 * 128 * 128;             // values of parts: CTAs on an SM x rows x padded head size, at most
 int32_t qkv_attention_i8(vn_qkv* c, const QkvAttnArgs& a);
 int32_t qkv_attention_e4m3(vn_qkv* c, const QkvAttnArgs& a);
-
-// value of one code
-template <int SCHEME> __device__ __forceinline__ float qkv_value(unsigned char c) {
-  if (SCHEME == QKV_I8) return (float)((int)c - 128);
-  // e4m3 in a half: the same sign, exponent and mantissa fields, 2^8 apart
-  const unsigned short h = (unsigned short)((c & 0x80) << 8 | (c & 0x7f) << 7);
-  return __half2float(__ushort_as_half(h)) * 256.f;
-}

@@ -23,7 +23,7 @@ using bf16 = __nv_bfloat16;
 constexpr int WARPS = 4, THREADS = 32 * WARPS;
 constexpr int MIN_SHARE = 4;                        // blocks of a share at least
 constexpr int MERGE_WARPS = 8, MANY = 8;           // warps of a merging CTA; parts that one of them takes
-constexpr int UNCUT = 8;                            // blocks of a unit that is never cut
+constexpr int UNCUT = 8;                            // in caches with room for no more blocks, units are not cut
 constexpr int MERGE_CTAS = 4;                       // merging CTAs on an SM
 // A copy that has not come after about two seconds is taken not to come.  The call is then no good and reported; whoever has met it asks for no more,
 // and before its memory goes to somebody else waits once more, LATE_CYCLES, for each copy that it has asked for
@@ -639,7 +639,8 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS, P > 128 ? MERGE_CTAS - 1 : M
   if (threadIdx.x == 0 && atomicAdd(a.n_cuts + 2, 1) == (int)gridDim.x - 1) { a.n_cuts[0] = 0; a.n_cuts[1] = 0; a.n_cuts[2] = 0; }
 }
 
-// row blocks of an entry, and whether units are cut: those of a few tiles stay whole, as cutting them saves less than the merge costs
+// Row blocks of an entry, and whether units are cut.  They are not where the cache has room for a few tiles only, as cutting them would save
+// less than the merge costs; with more room they are, short ones too (the host does not know the lengths)
 struct Launch {
   long long rts = 0, units = 0, tiles = 0;
   bool split = false;

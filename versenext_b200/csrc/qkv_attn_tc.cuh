@@ -4,7 +4,7 @@
 // and values alike with 128-byte rows of 64 channels and the 128-byte swizzle -- the layout of a K-major operand for the keys
 // (S = Q K^T) and of an MN-major one for the values (O += P V).  One warp issues the products.  Eight do the soft-max, two threads for a row, 32
 // columns each: S from TMEM, weights back to TMEM as the second product's A operand, results in TMEM (2 x 1000
-// rows behind 1500 positions, 16 heads of 128 channels: 73 us; four warps with 64 columns a thread 76).  S of the next page is computed while the weights of this one are, and two
+// rows behind 1500 positions, 16 heads of 128 channels: 72 us; four warps with 64 columns a thread 76).  S of the next page is computed while the weights of this one are, and two
 // CTAs share an SM.
 //
 // A row's reference maximum is moved only when a page's is more than 2^4 above it, so that the results in TMEM are seldom rescaled; weights
@@ -16,7 +16,7 @@
 namespace qkv_detail {
 
 constexpr int TC_ROWS = 128, TC_KEYS = KV_PAGE, TC_SOFT = 8, TC_THREADS = 32 * (TC_SOFT + 5), TC_CTAS = 2;      // TC_SOFT warps, four that convert, one that issues
-constexpr int TC_MIN_SHARE = 2, TC_UNCUT = 4;       // pages of a share at least; of a unit that is never cut
+constexpr int TC_MIN_SHARE = 2, TC_UNCUT = 4;       // pages of a share at least; room up to which units are not cut
 
 template <int P>
 struct TcCfg {

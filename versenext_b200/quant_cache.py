@@ -4,7 +4,8 @@
 that drive their own layers: one byte a value with an fp32 scale per head and position, in pages of 64 positions.  A step
 brings rows: `append` normalises, rotates and quantises them, `attention` answers their queries over everything committed
 and the rows themselves (a chain, or a `tree` of drafted tokens), `commit` keeps the accepted ones and `read` gives values back.
-Lengths live on the device; all of these are asynchronous on the context's stream and can be captured.
+Lengths live on the device; all of these are asynchronous on the context's stream and can be captured: with device arrays, `out` arrays, and
+steps and trees that live as long as the graph (a call without `out`, or with host arrays, takes memory that a replay would not have).
 
 bf16 rows are `np.uint16` arrays, the upper halves of float32 (a torch tensor's memory as it is); `to_bf16` / `from_bf16` convert on the host.
 """
