@@ -432,3 +432,34 @@ def test_a_copy_that_does_not_come_is_reported():
     np.testing.assert_array_equal(c.attention(q).numpy(), want)
     for cycles in (0, 1 << 40):
         assert c.ctx.lib.vn_qkv_probe_wait(c.handle, cycles, None) == VN_ERR_INVALID
+
+
+# ---- large values that a row does not see -------------------------------------------------------------------------------
+@pytest.mark.parametrize("scheme", ["int8", "fp8"])
+@pytest.mark.parametrize("dtype,H,d,T", [("f32", 2, 64, 4), ("bf16", 1, 64, 6), ("bf16", 2, 128, 8), ("bf16", 2, 64, 20), ("bf16", 4, 128, 30), ("bf16", 4, 96, 20), ("bf16", 2, 256, 20), ("f32", 2, 128, 40)])
+@pytest.mark.parametrize("size", [1e4, 1e10, 1e18, 1e30, 3e38])
+@pytest.mark.parametrize("where", ["chain", "tree", "window"])
+def test_values_that_a_row_does_not_see_do_not_touch_it(scheme, dtype, H, d, T, size, where):
+    """A later row of a chain, a row of a tree that no other sees, a position behind the window of the later rows, with values `size` times as
+    large as the others'.  A row's weights are held relative to the largest scale that it sees itself, or to 2^-117 of the largest that one of
+    its neighbours sees: on tcgen05 2^-150 of that is lost at most for every key, as 2^-33 of the row's own largest, else 2^-156 and 2^-39."""
+    rng = np.random.default_rng(T + d)
+    n = 300
+    c = new(1, n + T, H, 1, d, scheme=scheme, dtype=dtype)
+    q, k, v = (stored(rng.normal(0, 1, s), dtype) for s in ((T, H, d), (n + T, 1, d), (n + T, 1, d)))
+    window, parents, at = 0, None, n + T - 1
+    if where == "tree":
+        parents, at = [-1] + [0] * (T - 1), n + T // 2
+    if where == "window":
+        window, at = 200, n - 200 + T // 2                        # seen by the first half of the rows
+    v[at] = stored(v[at] / np.abs(v[at]).max() * size, dtype)
+    write(c, k, v)
+    c.set_lengths([n])
+    got = back(c.attention(q[None], tree=c.tree(parents) if parents else None, window=window))[0]
+    c.check()
+    depth, seen = R.depth_and_seen(parents, T)
+    out, weight, reach = R.attention(q, R.in_8_bits(k, scheme), R.in_8_bits(v, scheme), n, depth, seen, window, d ** -0.5)
+    tol = R.tolerance(out, weight, reach, d, n + T, dtype, scheme == "int8")
+    if dtype == "bf16":
+        tol = tol + 2.0 ** -150 * size * (n + T)
+    assert np.isfinite(got).all() and (np.abs(got - out) <= tol).all(), float(np.max(np.abs(got - out) / tol))

@@ -4,8 +4,11 @@
 // scales, q' the query times a power of two that brings its largest channel to [2^13, 2^14), r what undoes that times
 // scale * log2(e).  Codes are whole numbers or e4m3, both exact in 16-bit floats, so the products run on the tensor cores
 // (mma.sync m16n8k16, fp32 sums) with no rounding of keys and values; queries and weights are rounded to 11 bits for bf16 rows and
-// split into two halves of 11 bits for fp32 rows.  A weight p_j s_j is taken relative to a power of two R above every s_j met so
-// far, times 2^15, so that a half holds weights down to 2^-39 of the largest.
+// split into two halves of 11 bits for fp32 rows.  A weight p_j s_j is taken relative to a power of two R above every s_j that the row has seen so
+// far, times 2^15, so that a half holds weights down to 2^-39 of the largest (2^-37 beside rows that see one up to four times as large).  Scales
+// are brought to the largest R of the warp's rows; by what a row's own is below that, its weights' exponents are higher (up to 2^BELOW, so
+// that their sums are numbers): what a row does not see takes no bits from it.
+// 32 x 5 rows behind 1500 positions: 28.9 us, 29.3 with a factor for every weight and row, 27.3 with one R for all rows.
 //
 // What bounds it is the memory of the codes (few rows) or the mma.sync rate and the conversions (many).  Positions are the rows of the
 // products and queries their columns (8 at a time): S = K q^T, O = V^T p^T, with p transposed by movmatrix between.  A warp takes
@@ -24,6 +27,7 @@ constexpr int WARPS = 4, THREADS = 32 * WARPS;
 constexpr int MIN_SHARE = 4;                        // blocks of a share at least
 constexpr int MERGE_WARPS = 8, MANY = 8;           // warps of a merging CTA; parts that one of them takes
 constexpr int UNCUT = 8;                            // in caches with room for no more blocks, units are not cut
+constexpr int BELOW = 117;                          // a row's R is at most that many powers of two below the largest of its warp
 constexpr int MERGE_CTAS = 4;                       // merging CTAs on an SM
 // A copy that has not come after about two seconds is taken not to come.  The call is then no good and reported; whoever has met it asks for no more,
 // and before its memory goes to somebody else waits once more, LATE_CYCLES, for each copy that it has asked for
@@ -314,7 +318,12 @@ __global__ void __launch_bounds__(THREADS, (AttnCfg<T, P, NT, RS>::CTAS)) qkv_at
 #pragma unroll
       for (int x = 0; x < 2; ++x) { m_run[nt][x] = -CUDART_INF_F; l_run[nt][x] = 0.f; }
     }
-    int R = 16;                                              // biased exponent of the largest scale of values met
+    int R = 16;                                              // biased exponent of the largest scale of values that a row of the warp has seen
+    bool mixed = false;                                      // there are rows whose own is below it
+    unsigned R4[(NT + 1) / 2];                               // by how much: four rows in a register
+#pragma unroll
+    for (int i = 0; i < (NT + 1) / 2; ++i) R4[i] = 0u;
+    auto below = [&](int nt, int x) { return (int)((R4[nt / 2] >> (16 * (nt & 1) + 8 * x)) & 255u); };
 #pragma unroll 1
     for (int i = seg_a; i < seg_b; ++i, ++it) {
       const int k = i - seg_a;
@@ -355,20 +364,25 @@ __global__ void __launch_bounds__(THREADS, (AttnCfg<T, P, NT, RS>::CTAS)) qkv_at
               mma_f16(t[1][nt], ka[1], q[0], q[1]);
             }
         }
-        // ---- scales of the block: the largest of the values' that count
+        // ---- scales of the block: where the largest of the values' (numbers only) that some row sees is above R, all rows mostly see one of at least a
+        // quarter of it, and take it for theirs; if not, the rows' own are looked up when it is known what they see
+        bool odd = mixed;
         {
           const unsigned b = __float_as_uint(sc[QKV_BLOCK + lane]);
           const bool counts = (full || (k0 + lane >= u.lo && k0 + lane < u.hi)) && b < 0x7f800000u;
-          const int e = (int)(__reduce_max_sync(0xffffffffu, counts ? b : 0u) >> 23);
-          if (e > R) {
-            const float f = pow2(127 + R - e);
-            R = e;
+          const int all = (int)(__reduce_max_sync(0xffffffffu, counts ? b : 0u) >> 23);
+          if (all > R && !mixed) {
+            odd = !full && !__any_sync(0xffffffffu, counts && (int)(b >> 23) >= all - 2 && k0 + lane >= u.full_lo && k0 + lane < u.full_hi);
+            if (!odd) {
+              const float f = pow2(127 + R - all);
+              R = all;
 #pragma unroll
-            for (int c = 0; c < CH; ++c)
+              for (int c = 0; c < CH; ++c)
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
+                for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                for (int x = 0; x < 4; ++x) acc[c][nt][x] *= f;
+                  for (int x = 0; x < 4; ++x) acc[c][nt][x] *= f;
+            }
           }
         }
         const float rs = pow2(268 - R);
@@ -399,6 +413,49 @@ __global__ void __launch_bounds__(THREADS, (AttnCfg<T, P, NT, RS>::CTAS)) qkv_at
               }
             }
         }
+        if (__builtin_expect(odd, 0)) {                      // row by row
+          auto raw = [&](int j) { return __float_as_uint(sc[QKV_BLOCK + 8 * j + rg]); };
+          unsigned own[(NT + 1) / 2], most = R;
+#pragma unroll
+          for (int h = 0; h < (NT + 1) / 2; ++h) {
+            unsigned seen = 0, valid = 0;                  // bytes, as R4
+#pragma unroll
+            for (int y = 0; y < 4 && 2 * h + y / 2 < NT; ++y) {
+              const int nt = 2 * h + y / 2, x = y & 1;
+              unsigned top = 0;
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                if (t[j >> 1][nt][2 * (j & 1) + x] != -CUDART_INF_F && raw(j) < 0x7f800000u) top = max(top, raw(j));
+              seen |= (top >> 23) << (8 * y);
+              if (row_t[nt][x] >= 0) valid |= 255u << (8 * y);
+            }
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) seen = __vmaxu4(seen, __shfl_xor_sync(0xffffffffu, seen, o));
+            own[h] = __vmaxu4(0x01010101u * (unsigned)R - R4[h], seen) & valid;
+            most = max(max(most, max(own[h] & 255u, own[h] >> 24)), max((own[h] >> 8) & 255u, (own[h] >> 16) & 255u));
+            own[h] |= ~valid;                              // (rows that are none: 255)
+          }
+          most = __reduce_max_sync(0xffffffffu, most);
+          unsigned any = 0;
+#pragma unroll
+          for (int h = 0; h < (NT + 1) / 2; ++h) {
+            const unsigned to = __vminu4(0x01010101u * most - __vminu4(own[h], 0x01010101u * most), 0x01010101u * BELOW);
+#pragma unroll
+            for (int y = 0; y < 4 && 2 * h + y / 2 < NT; ++y) {
+              const int nt = 2 * h + y / 2, x = y & 1;
+              const float f = pow2(127 + R - (int)most + (int)((to >> (8 * y)) & 255u) - (int)((R4[h] >> (8 * y)) & 255u));
+#pragma unroll
+              for (int c = 0; c < CH; ++c) { acc[c][nt][x] *= f; acc[c][nt][2 + x] *= f; }
+            }
+            R4[h] = to;
+            any |= to;
+          }
+          R = (int)most;
+          mixed = __any_sync(0xffffffffu, any != 0);
+          const float rs = pow2(268 - R);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) vs[j] = sc[QKV_BLOCK + 8 * j + rg] * rs;
+        }
         // ---- weights
         unsigned pb[NT][NQ][4];                              // of positions 8 j + 2 rc, + 1 and row 8 nt + rg
         float base[NT][2], f[NT][2];
@@ -423,6 +480,11 @@ __global__ void __launch_bounds__(THREADS, (AttnCfg<T, P, NT, RS>::CTAS)) qkv_at
             m_run[nt][x] = m;
             grew |= f[nt][x] != 1.f;
           }
+        if (__builtin_expect(mixed, 0))
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) base[nt][x] -= (float)below(nt, x);
         if (__any_sync(0xffffffffu, grew))
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
@@ -433,14 +495,15 @@ __global__ void __launch_bounds__(THREADS, (AttnCfg<T, P, NT, RS>::CTAS)) qkv_at
               for (int c = 0; c < CH; ++c) { acc[c][nt][x] *= f[nt][x]; acc[c][nt][2 + x] *= f[nt][x]; }
             }
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int nt = 0; nt < NT; ++nt) {
+          float sum[2] = {0.f, 0.f};
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             float w[2];
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
               const float s1 = t[j >> 1][nt][2 * (j & 1) + x], p = ex2(fmaf(s1, rf[nt][x], -base[nt][x]));
-              l_run[nt][x] += p;                             // this lane's share; the eight lanes of a row are summed at the end
+              sum[x] += p;
               w[x] = p * vs[j];
               if (!full && s1 == -CUDART_INF_F) w[x] = 0.f;  // what a row does not see may have any scale, NaN too
             }
@@ -451,6 +514,12 @@ __global__ void __launch_bounds__(THREADS, (AttnCfg<T, P, NT, RS>::CTAS)) qkv_at
               pb[nt][NQ - 1][j] = transposed(pack_f16(w[0] - g.x, w[1] - g.y));
             }
           }
+#pragma unroll
+          for (int x = 0; x < 2; ++x) {                      // this lane's share; the eight lanes of a row are summed at the end
+            if (__builtin_expect(mixed, 0)) sum[x] *= pow2(127 - below(nt, x));
+            l_run[nt][x] += sum[x];
+          }
+        }
         // ---- values: register j of a transposed read holds channels 2 rg, 2 rg + 1 of positions 8 j + 2 rc, + 1; row m of the
         // product is channel 2 m (m < 8) or 2 (m - 8) + 1
 #pragma unroll
@@ -490,7 +559,6 @@ __global__ void __launch_bounds__(THREADS, (AttnCfg<T, P, NT, RS>::CTAS)) qkv_at
       begin_segment();
     }
     // ---- a warp's rows are its own: straight to memory, 32 bytes of a row (bf16) at a time
-    const float r_inv = pow2(R - 14);
     const int part = 2 * worker + (begun ? 1 : 0);
 #pragma unroll
     for (int o = 4; o < 32; o <<= 1)
@@ -505,6 +573,7 @@ __global__ void __launch_bounds__(THREADS, (AttnCfg<T, P, NT, RS>::CTAS)) qkv_at
         const int r = row0 + 8 * nt + 2 * rc + x, tok = row_t[nt][x];
         const float l = l_run[nt][x];
         if (tok < 0) continue;
+        const float r_inv = pow2(R - below(nt, x) - 14);
         const float inv = whole ? (l == 0.f ? 0.f : r_inv / l) : r_inv;      // nothing seen: zero
         T* out = reinterpret_cast<T*>(a.out) + ((long long)(du.r0 + tok) * v.H + d_head * G + (du.f0 + r - tok * G)) * v.d + 2 * rg;
         float* part_o = a.part_o + ((long long)part * RT + r) * P + 2 * rg;
@@ -535,9 +604,9 @@ __global__ void __launch_bounds__(THREADS, (AttnCfg<T, P, NT, RS>::CTAS)) qkv_at
 // the lists.  The kernel begins while the shares end; it goes through the motions once before it waits for them, so that its
 // instructions are there (without that a row took 3 us, most of it fetching them).  That first pass takes a cut of constants, never one from
 // the list: what stands there then is an earlier call's, whose shares with other rows lie beyond this call's parts.  Parts are read from L2, as the
-// first pass has brought some of them before they were written.  rmax: rows of a unit at most
+// first pass has brought some of them before they were written.  rmax: rows of a unit at most; up: what their results are to be multiplied by
 template <typename T, int P>
-__global__ void __launch_bounds__(32 * MERGE_WARPS, P > 128 ? MERGE_CTAS - 1 : MERGE_CTAS) qkv_merge_kernel(QkvAttnArgs a, int RT, int rmax) {
+__global__ void __launch_bounds__(32 * MERGE_WARPS, P > 128 ? MERGE_CTAS - 1 : MERGE_CTAS) qkv_merge_kernel(QkvAttnArgs a, int RT, int rmax, float up) {
   constexpr int Y = P > 128 ? 2 : 1, IN = Y > 1 ? 4 : 8;      // parts asked for at a time
   static_assert(IN <= MANY, "eight warps on a row's parts know the maximum of all of them");
   __shared__ float4 s_sum[MERGE_WARPS][32 * Y];
@@ -632,7 +701,7 @@ __global__ void __launch_bounds__(32 * MERGE_WARPS, P > 128 ? MERGE_CTAS - 1 : M
       T* out = reinterpret_cast<T*>(a.out) + ((long long)(o.r0 + f / G) * a.v.H + o.head * G + f % G) * a.v.d;
 #pragma unroll
       for (int y = 0; y < Y; ++y)
-        if (4 * lane + 128 * y < a.v.d) store4(out + 4 * lane + 128 * y, scaled(sum[y], l == 0.f ? 0.f : 1.f / l));
+        if (4 * lane + 128 * y < a.v.d) store4(out + 4 * lane + 128 * y, scaled(sum[y], l == 0.f ? 0.f : up / l));
     }
   }
   __syncthreads();
@@ -669,10 +738,10 @@ int32_t merge_ready(vn_qkv* c) {
   return VN_OK;
 }
 template <typename T, int P>
-int32_t merge(vn_qkv* c, const QkvAttnArgs& a, int RT, long long units) {
+int32_t merge(vn_qkv* c, const QkvAttnArgs& a, int RT, long long units, float up = 1.f) {
   const int rmax = (int)min((long long)RT, (long long)a.step.T * (a.v.H / a.v.KH)), sms = c->ctx->sm_count;
   const long long rows = units * rmax;
-  VN_LAUNCH_PDL_LEVEL(c->ctx, 1, "qkv_merge_kernel", (qkv_merge_kernel<T, P>), dim3((unsigned)min((long long)sms * MERGE_CTAS, rows)), 32 * MERGE_WARPS, rows <= 2 * sms ? MERGE_SPREAD : 0, a, RT, rmax);
+  VN_LAUNCH_PDL_LEVEL(c->ctx, 1, "qkv_merge_kernel", (qkv_merge_kernel<T, P>), dim3((unsigned)min((long long)sms * MERGE_CTAS, rows)), 32 * MERGE_WARPS, rows <= 2 * sms ? MERGE_SPREAD : 0, a, RT, rmax, up);
   return VN_OK;
 }
 

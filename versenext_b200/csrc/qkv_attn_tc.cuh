@@ -8,14 +8,15 @@
 // CTAs share an SM.
 //
 // A row's reference maximum is moved only when a page's is more than 2^4 above it, so that the results in TMEM are seldom rescaled; weights
-// are at most 2^4 then, and taken relative to R (at least the largest scale of values, with room of 2^2) times 2^11: a half holds them down
-// to 2^-33 of the largest.
+// are at most 2^4 then, and taken relative to R (at least the largest scale of the values that the row sees, with room of up to 2^2) times 2^11: a
+// half holds them down to 2^-33 of the largest.  Rows of a warp whose R differ: as in qkv_attn.cuh.
 #pragma once
 #include "qkv_attn.cuh"
 
 namespace qkv_detail {
 
 constexpr int TC_ROWS = 128, TC_KEYS = KV_PAGE, TC_SOFT = 8, TC_THREADS = 32 * (TC_SOFT + 5), TC_CTAS = 2;      // TC_SOFT warps, four that convert, one that issues
+constexpr float TC_PARTS = 16.f;                     // parts are kept that many times smaller: weights may be 2^4 then, and the largest values not
 constexpr int TC_MIN_SHARE = 2, TC_UNCUT = 4;       // pages of a share at least; room up to which units are not cut
 
 template <int P>
@@ -276,8 +277,12 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) qkv_attn_tc_kernel(QkvAtt
             sc[ct] = none ? 0.f : from[0];
             sc[TC_KEYS + ct] = vs;
             const unsigned b = __float_as_uint(vs);
-            const unsigned top = __reduce_max_sync(0xffffffffu, key >= u.lo && key < u.hi && b < 0x7f800000u ? b : 0u);
-            if (lane == 0) s_meta[t % 3 * 4 + 1 + ct / 32] = (int)(top >> 23);
+            const bool counts = key >= u.lo && key < u.hi && b < 0x7f800000u;
+            const unsigned top = __reduce_max_sync(0xffffffffu, counts ? b : 0u) >> 23;
+            const int k0 = (seg_a + i) * TC_KEYS;
+            unsigned shared = top;                           // of those that all rows see
+            if (k0 < u.full_lo || k0 + TC_KEYS > u.full_hi) shared = __reduce_max_sync(0xffffffffu, counts && key >= u.full_lo && key < u.full_hi ? b : 0u) >> 23;
+            if (lane == 0) s_meta[t % 3 * 4 + 1 + ct / 32] = (int)(shared << 8 | top);
             if (ct == 0) {
               s_meta[t % 3 * 4] = !none;
               if (none) v.status[0] = 1;
@@ -320,7 +325,8 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) qkv_attn_tc_kernel(QkvAtt
       const int away = tok < 0 || a.window == 0 ? 0 : a.tree.behind(v, u.r0 + tok, tok);
       const unsigned long long seen = a.tree.seen && tok >= 0 ? a.tree.sees(u.r0 + tok, tok, a.window) : 0;
       float rf = 0.f, m = -CUDART_INF_F, l = 0.f;
-      int R = 16;
+      int R = 16, below = 0;                                 // the largest of the warp's rows, which scales are brought to; what the row's own is below it
+      bool mixed = false;                                    // there are such rows
 #pragma unroll 1
       for (int i = 0; i < seg_n; ++i) {
         const unsigned t = n + i;
@@ -333,29 +339,17 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) qkv_attn_tc_kernel(QkvAtt
         const unsigned at_s = lanes + C::S_COL + 64 * (t & 1);
         float x[32];
         tc_ld(at_s + 32 * half, reinterpret_cast<unsigned*>(x));
-        const int e = max(meta[1], meta[2]);
-        float f_r = 1.f;
-        if (e > R) {
-          const int to = min(e + 2, 254);
-          f_r = pow2(127 + R - to);
-          R = to;
-        }
-        s_w[lane] = sc[TC_KEYS + lane] * pow2(264 - R);
+        const int e = max(meta[1] & 255, meta[2] & 255), e_all = max(meta[1], meta[2]) >> 8;         // of the largest scale that some row, that all rows see
         const int k0 = (seg_a + i) * TC_KEYS;
         const bool full = meta[0] && k0 >= u.full_lo && k0 + TC_KEYS <= u.full_hi;
-        tc_wait_ld();
-#pragma unroll
-        for (int c = 0; c < 32; c += 4) {
-          const float4 k = *reinterpret_cast<const float4*>(sc + c);
-          x[c] *= k.x; x[c + 1] *= k.y; x[c + 2] *= k.z; x[c + 3] *= k.w;
-        }
+        unsigned see = ~0u;
         if (!full) {                                         // which of the positions the row sees, as bits
+          see = 0;
           const int h0 = k0 + 32 * half;
           auto range = [&](int lo, int hi) {                 // positions lo .. hi - 1
             const int p = min(max(lo - h0, 0), 32), q = min(max(hi - h0, 0), 32);
             return p >= q ? 0u : (~0u >> (32 - (q - p))) << p;
           };
-          unsigned see = 0;
           if (tok >= 0 && meta[0]) {
             const int from = a.window > 0 ? max(0, u.len + away - a.window + 1) : 0;
             if (a.tree.seen) {
@@ -367,10 +361,44 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) qkv_attn_tc_kernel(QkvAtt
             }
             see &= range(0, u.hi);
           }
+        }
+        // where that is above R: for all rows the latter with its room, if that is enough for all, else row by row
+        float f_r = 1.f;
+        if (e > R && e_all >= e - 2 && !mixed) {
+          const int to = min(e_all + 2, 254);
+          f_r = pow2(127 + R - to);
+          R = to;
+        }
+        s_w[lane] = sc[TC_KEYS + lane] * pow2(264 - R);
+        if (__builtin_expect(e > R || mixed, 0)) {           // the same for both halves
+          int e_own = e;
+          if (!full) {
+            unsigned most = 0;                               // of the scales that the row sees, numbers only
+#pragma unroll 1
+            for (int c = 0; c < 32; ++c) {
+              const unsigned b = __float_as_uint(sc[TC_KEYS + c]);
+              if (((see >> c) & 1) && b < 0x7f800000u) most = max(most, b);
+            }
+            e_own = (int)(max(most, __float_as_uint(exchange(__uint_as_float(most)))) >> 23);
+          }
+          const int was = R - below, own = e_own > was ? min(e_own + 2, 254) : was;
+          R = __reduce_max_sync(0xffffffffu, own);
+          below = min(R - own, BELOW);
+          f_r = pow2(127 + was - (R - below));
+          mixed = __any_sync(0xffffffffu, below != 0);
+          __syncwarp();
+          s_w[lane] = sc[TC_KEYS + lane] * pow2(264 - R);
+        }
+        tc_wait_ld();
+#pragma unroll
+        for (int c = 0; c < 32; c += 4) {
+          const float4 k = *reinterpret_cast<const float4*>(sc + c);
+          x[c] *= k.x; x[c + 1] *= k.y; x[c + 2] *= k.z; x[c + 3] *= k.w;
+        }
+        if (!full)
 #pragma unroll
           for (int c = 0; c < 32; ++c)
             if (!((see >> c) & 1)) x[c] = -CUDART_INF_F;
-        }
         float mx[4] = {x[0], x[1], x[2], x[3]};
 #pragma unroll
         for (int c = 4; c < 32; ++c) mx[c & 3] = fmaxf(mx[c & 3], x[c]);
@@ -382,7 +410,8 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) qkv_attn_tc_kernel(QkvAtt
           m = top;
           l *= f_m;
         }
-        const float base = m == -CUDART_INF_F ? 0.f : m;     // nothing seen yet: every weight becomes exp2(-inf) = 0
+        float base = m == -CUDART_INF_F ? 0.f : m;           // nothing seen yet: every weight becomes exp2(-inf) = 0
+        if (__builtin_expect(mixed, 0)) base -= (float)below;
         float sum[4] = {0.f, 0.f, 0.f, 0.f};
         unsigned pk[16];
         __syncwarp();                                        // s_w
@@ -401,7 +430,9 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) qkv_attn_tc_kernel(QkvAtt
           pk[c / 2 + 1] = pack_f16(g[2], g[3]);
         }
         tc_st16(at_s + 16 * half, pk);                       // over the first half's scores, which that half has read: both have exchanged their maxima
-        l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        sum[0] = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+        if (__builtin_expect(mixed, 0)) sum[0] *= pow2(127 - below);
+        l += sum[0];
         const float f_o = f_m * f_r;
         if (i && __any_sync(0xffffffffu, f_o != 1.f)) {      // the same for both halves
           wait_results(t - 1);
@@ -430,7 +461,7 @@ __global__ void __launch_bounds__(TC_THREADS, TC_CTAS) qkv_attn_tc_kernel(QkvAtt
       tc_fence_after();
       const bool whole = !split || seg_n == u.tiles, begun = !whole && sh.tile == 0;
       const int part = 2 * blockIdx.x + (begun ? 1 : 0);
-      const float r_inv = pow2(R - 10), inv = whole ? (l == 0.f ? 0.f : r_inv / l) : r_inv;
+      const float r_inv = pow2(R - below - 10), inv = whole ? (l == 0.f ? 0.f : r_inv / l) : r_inv * (1.f / TC_PARTS);
       bf16* out = reinterpret_cast<bf16*>(a.out) + ((long long)(u.r0 + max(tok, 0)) * v.H + sh.head * G + (f - max(tok, 0) * G)) * v.d;
       float* part_o = a.part_o + ((long long)part * TC_ROWS + row) * P;
       const bool wide = v.d % 16 == 0 && (reinterpret_cast<unsigned long long>(a.out) & 31) == 0;           // rows begin at whole sectors
@@ -499,7 +530,7 @@ int32_t launch_tc(vn_qkv* c, const QkvAttnArgs& a) {
   if (int32_t st = l.of(c, a, TC_ROWS, TC_KEYS, TC_UNCUT)) return st;
   const unsigned grid = (unsigned)min((long long)TC_CTAS * ctx->sm_count, l.most(TC_MIN_SHARE));
   VN_LAUNCH_PDL_LEVEL(ctx, 1, "qkv_attn_tc_kernel", kernel, grid, TC_THREADS, C::SMEM, a, (int)l.rts, l.split);
-  return l.split ? merge<bf16, P>(c, a, TC_ROWS, l.units) : VN_OK;
+  return l.split ? merge<bf16, P>(c, a, TC_ROWS, l.units, TC_PARTS) : VN_OK;
 }
 
 }  // namespace qkv_detail
