@@ -463,7 +463,8 @@ int32_t vn_qkv_append(vn_qkv* c, const void* rows_dev, int64_t ld, int32_t queri
 /* out = softmax(scale q k^T) v over the committed positions and the rows of the same step (appended at offset 0); query head h
  * reads key/value head h / (H / KH).  window > 0: row at position p sees position j only if p - j < window (in a tree too:
  * of a row and its ancestors, parents before children, the last `window`).  A row that sees nothing gets zeros; one that sees
- * something, with a query that is not finite or a position that reads as NaN, gets NaN.  q_dev, out_dev
+ * something, with a query that is not finite or a position that reads as NaN, gets NaN.  Keys that a row sees are up to 8e31 in
+ * size (a score is summed before the scales of queries and `scale` come in).  q_dev, out_dev
  * [M, H, head_dim], 16-byte (float32) / 8-byte aligned.  All caches of a context share one workspace, on its stream.
  * VN_ERR_INVALID, too: more rows over more room than the kernels count, 2^30 tiles (8 rows, 32 positions of max_seq) for every SM. */
 int32_t vn_qkv_attention(vn_qkv* c, const void* q_dev, int32_t n_ent, const int32_t* ents_dev, const int32_t* row_ent_dev, int32_t T, int32_t M,

@@ -4,7 +4,8 @@
 // scales, q' the query times a power of two that brings its largest channel to [2^13, 2^14), r what undoes that times
 // scale * log2(e).  Codes are whole numbers or e4m3, both exact in 16-bit floats, so the products run on the tensor cores
 // (mma.sync m16n8k16, fp32 sums) with no rounding of keys and values; queries and weights are rounded to 11 bits for bf16 rows and
-// split into two halves of 11 bits for fp32 rows.  A weight p_j s_j is taken relative to a power of two R above every s_j that the row has seen so
+// split into two halves of 11 bits for fp32 rows: chosen as a second product for the rest of a weight would double those of the values, for a
+// result of 8 bits (bf16: 0.0017 from 64 bits either way) or 2^-22 of a weight (fp32: 2.0e-7 against 1.9e-7).  A weight p_j s_j is taken relative to a power of two R above every s_j that the row has seen so
 // far, times 2^15, so that a half holds weights down to 2^-39 of the largest (2^-37 beside rows that see one up to four times as large).  Scales
 // are brought to the largest R of the warp's rows; by what a row's own is below that, its weights' exponents are higher (up to 2^BELOW, so
 // that their sums are numbers): what a row does not see takes no bits from it.

@@ -4,7 +4,7 @@
 // and values alike with 128-byte rows of 64 channels and the 128-byte swizzle -- the layout of a K-major operand for the keys
 // (S = Q K^T) and of an MN-major one for the values (O += P V).  One warp issues the products.  Eight do the soft-max, two threads for a row, 32
 // columns each: S from TMEM, weights back to TMEM as the second product's A operand, results in TMEM (2 x 1000
-// rows behind 1500 positions, 16 heads of 128 channels: 72 us; four warps with 64 columns a thread 76).  S of the next page is computed while the weights of this one are, and two
+// rows behind 1500 positions, 16 heads of 128 channels: 74 us; when it was made 73, against 76 with four warps of 64 columns a thread).  S of the next page is computed while the weights of this one are, and two
 // CTAs share an SM.
 //
 // A row's reference maximum is moved only when a page's is more than 2^4 above it, so that the results in TMEM are seldom rescaled; weights
